@@ -49,7 +49,7 @@
 extern "C" {
 #endif
 
-#define BFA_ABI_VERSION 5
+#define BFA_ABI_VERSION 6
 
 typedef enum bfa_dtype {
   BFA_DTYPE_F32 = 0,
@@ -65,7 +65,9 @@ typedef enum bfa_status {
   BFA_ERR_WORKSPACE = -4,         /* workspace missing or too small */
   BFA_ERR_CUDA = -5,              /* a CUDA runtime/driver call failed */
   BFA_ERR_DEVICE_TIMEOUT = -6,    /* a device-side wait ran out (status word) */
-  BFA_ERR_SCRATCH_LIMIT = -7      /* bfa_bwd_noalloc: problem larger than its static scratch */
+  BFA_ERR_SCRATCH_LIMIT = -7,     /* bfa_bwd_noalloc: problem larger than its static scratch */
+  BFA_ERR_INDEX = -8              /* a position, page, node or token index on the device lies
+                                     outside its table (status word) */
 } bfa_status;
 
 /* Problem description: the reference host API's arguments
@@ -232,6 +234,146 @@ int bfa_merge_partial(int32_t batch, int32_t heads, int32_t seqlen, int32_t head
                       bfa_tensor o_acc, int32_t acc_dtype, float* lse_acc,
                       bfa_tensor o_part, int32_t part_dtype, const float* lse_part,
                       void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Operators around attention for decoding with a tree of drafted tokens (no
+ * reference counterpart). Conventions as above. All fields of their argument
+ * structures are 8 bytes wide. Indices that live on the device (positions,
+ * page numbers, parents, tokens, counts) are checked there: a kernel never
+ * reads or writes outside the tensors it was given, and reports an index
+ * outside its table as BFA_ERR_INDEX in `status`; what such a call leaves in
+ * the rows concerned is said at each entry point.
+ *
+ * A paged K/V cache is two tensors [num_pages, Hkv, page_size, D] (k_pages and
+ * v_pages, unit innermost stride), a page table int32 [B, max_pages] (row
+ * stride page_table_stride) and the cached lengths int32 [B]: token t of
+ * sequence b lies in page page_table[b, t / page_size], slot t % page_size.
+ * Table entries past a sequence's length are not read.
+ *
+ * A tree of `nodes` drafted tokens per sequence is given by the parent of each
+ * node, int32 [B, nodes] (row stride parents_stride, 0: one tree for all):
+ * node 0 is the root (the last decided token, whose K/V is not cached yet; its
+ * own entry is not read), 0 <= parents[n] < n otherwise, and -1 marks a node
+ * that is absent, with everything under it. A null `parents` is a chain
+ * (parents[n] = n - 1). Node n of sequence b stands at position
+ * lens[b] + (edges from the root to n). */
+
+typedef struct bfa_rope_args {
+  int64_t batch, heads_q, heads_k, seqlen, head_dim; /* heads_k 0: no k */
+  int64_t rotary_dim;       /* even, 2..head_dim: the dims that turn; the others are copied */
+  int64_t dtype;            /* bfa_dtype of q, k and the outputs */
+  int64_t interleaved;      /* 0: pairs (x[i], x[i + R/2]); 1: pairs (x[2i], x[2i + 1]) */
+  int64_t inverse;          /* 1: the transposed rotation (the backward) */
+  bfa_tensor q, k;          /* [B, H, S, D], any strides */
+  bfa_tensor q_out, k_out;  /* written; each may be its input itself (same data and strides) */
+  const float* cos;         /* [table_rows, R/2], unit inner stride, row stride table_stride */
+  const float* sin;
+  int64_t table_rows, table_stride;
+  const void* positions;    /* NULL: row s stands at s. Else integers [B, S] of positions_bytes
+                               (4 or 8) bytes at element strides positions_stride (0 broadcasts) */
+  int64_t positions_bytes;
+  int64_t positions_stride[2];
+  const void* offsets;      /* NULL: 0. Else integers [B] of offsets_bytes bytes, added to the positions */
+  int64_t offsets_bytes;
+  int32_t* status;          /* optional device status word */
+} bfa_rope_args;
+
+/* Rotary positions on q and k: with t the row's position and c = cos[t, i],
+ * s = sin[t, i], each pair (a, b) becomes (a·c - b·s, a·s + b·c), or with
+ * `inverse` (a·c + b·s, b·c - a·s). fp32 arithmetic, one rounding. A position
+ * outside [0, table_rows) gives NaN in the turning dims and BFA_ERR_INDEX. */
+int bfa_rope(const bfa_rope_args* args, void* stream);
+
+typedef struct bfa_tree_args {
+  int64_t batch, heads_q, heads_kv, nodes, head_dim; /* nodes 1..64 */
+  int64_t dtype;            /* bfa_dtype of q, k, v, o and the pages */
+  int64_t num_pages, page_size, max_pages;
+  int64_t sliding_window;   /* 0 = off; else keep i - j <= sliding_window (positions) */
+  double scale, soft_cap;   /* as in bfa_problem */
+  const float* alibi_slopes;/* NULL or fp32 [heads_q] */
+  bfa_tensor q;             /* [B, Hq, nodes, D] */
+  bfa_tensor k, v;          /* [B, Hkv, nodes, D]: the nodes' own K/V */
+  bfa_tensor o;             /* [B, Hq, nodes, D], written */
+  float* lse;               /* optional fp32 [B, Hq, nodes] contiguous, written */
+  bfa_tensor k_pages, v_pages;
+  const int32_t* page_table;
+  int64_t page_table_stride;
+  const int32_t* lens;
+  const int32_t* parents;
+  int64_t parents_stride;
+  int32_t* status;          /* optional device status word */
+  void* workspace;          /* at least bfa_tree_workspace_bytes(), 256-byte aligned */
+  int64_t workspace_bytes;
+} bfa_tree_args;
+
+/* Bytes of workspace bfa_tree_fwd needs for these sizes on the current device
+ * (the pointers are not looked at); 0 for invalid or empty problems. */
+size_t bfa_tree_workspace_bytes(const bfa_tree_args* args);
+
+/* Attention of a tree of drafted tokens over a paged cache: node n sees the
+ * sequence's cached tokens, itself and the nodes above it. O and natural-log
+ * LSE; rows of absent nodes get O = 0, LSE = -inf. A page number outside
+ * [0, num_pages) reads as zero keys and values, a length outside
+ * [0, max_pages * page_size] is clamped, a parent outside its range makes the
+ * node absent; each reports BFA_ERR_INDEX. */
+int bfa_tree_fwd(const bfa_tree_args* args, void* stream);
+
+typedef struct bfa_verify_args {
+  int64_t batch, nodes, vocab; /* nodes 1..64 */
+  int64_t dtype;            /* bfa_dtype of the probabilities */
+  const void* target;       /* [B, nodes, vocab]: row n is the target's law after node n */
+  int64_t target_stride[2]; /* batch, node; unit innermost stride */
+  const void* draft;        /* NULL (deterministic drafts) or [B, nodes, vocab]: row n is the law
+                               from which node n's children were drawn */
+  int64_t draft_stride[2];
+  const void* tokens;       /* integers [B, nodes] of tokens_bytes (4 or 8) bytes; node 0's is not read */
+  int64_t tokens_bytes, tokens_stride;
+  const int32_t* parents;
+  int64_t parents_stride;
+  const float* uniforms;    /* [B, nodes]: node n's number in [0, 1) */
+  int64_t uniforms_stride;
+  const float* noise;       /* [B, vocab]: standard exponential draws, > 0 */
+  int64_t noise_stride;
+  int32_t* path;            /* [B, nodes] contiguous, written: the accepted nodes from the root, then -1 */
+  int32_t* count;           /* [B], written: accepted nodes, the root among them */
+  int32_t* next_token;      /* [B], written */
+  int32_t* status;          /* optional device status word */
+} bfa_verify_args;
+
+/* Verification of drafted tokens: walks down the tree from the root, testing
+ * each node's children in index order against the target's law p and the
+ * draft's law q of that node. With a = 0, W = 1 at first, child n of token x
+ * is accepted when u[n]·W·q(x) < max(p(x) - a·q(x), 0); a rejection sets
+ * a += W, then W = sum_v max(p(v) - a·q(v), 0). Without q: accepted when
+ * u[n]·(1 - removed) < p(x); a rejection adds p(x) to `removed` and takes x out
+ * of p. When no child is accepted the next token is the lowest v that
+ * maximises residual(v) / noise(v), a draw from the residual (from p, where
+ * the residual is empty). Sums in fp32. A token outside [0, vocab) is
+ * rejected and reports BFA_ERR_INDEX. */
+int bfa_verify_tree(const bfa_verify_args* args, void* stream);
+
+typedef struct bfa_append_args {
+  int64_t batch, heads_kv, tokens, head_dim;
+  int64_t dtype;
+  int64_t num_pages, page_size, max_pages;
+  bfa_tensor k, v;          /* [B, Hkv, tokens, D] */
+  bfa_tensor k_pages, v_pages; /* written in place */
+  const int32_t* page_table;
+  int64_t page_table_stride;
+  const int32_t* lens;      /* [B], not written */
+  const int32_t* take;      /* NULL: token i. Else [B, tokens]: the i-th appended token is take[b, i] */
+  int64_t take_stride;
+  const int32_t* count;     /* NULL: all tokens. Else [B]: tokens that sequence b appends */
+  int32_t* lens_out;        /* [B], written: lens + count; must not be `lens` */
+  int32_t* status;          /* optional device status word */
+} bfa_append_args;
+
+/* Append tokens to a paged cache: for i < count[b], token take[b, i] of
+ * sequence b goes to slot lens[b] + i of its pages. Tokens that would pass
+ * the table's capacity, with a page number outside [0, num_pages) or a
+ * `take` outside [0, tokens) are not written; a count outside [0, tokens] or
+ * a length outside the capacity is clamped; each reports BFA_ERR_INDEX. */
+int bfa_cache_append(const bfa_append_args* args, void* stream);
 
 #ifdef __cplusplus
 }

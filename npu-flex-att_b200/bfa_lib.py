@@ -8,13 +8,14 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 import torch
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libbfa.so")
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 DEBUG_INJECT_STALL = 1
@@ -22,8 +23,10 @@ ERR_DEVICE_TIMEOUT = -6
 
 EXPORTED = ("bfa_abi_version", "bfa_launch_count", "bfa_strerror", "bfa_last_error", "bfa_fwd",
             "bfa_fwd_workspace_bytes", "bfa_bwd_workspace_bytes", "bfa_bwd_delta", "bfa_bwd", "bfa_bwd_noalloc",
-            "bfa_merge_partial")
+            "bfa_merge_partial", "bfa_rope", "bfa_tree_workspace_bytes", "bfa_tree_fwd", "bfa_verify_tree",
+            "bfa_cache_append")
 ERR_SCRATCH_LIMIT = -7
+ERR_INDEX = -8
 NOALLOC_MAX_ROWS = 1 << 21
 PHASE_DELTA, PHASE_DKDV, PHASE_DQ = 1, 2, 4
 
@@ -61,6 +64,51 @@ class BwdArgs(ctypes.Structure):
                 ("dk", Tensor), ("dv", Tensor), ("status", ctypes.c_void_p),
                 ("wait_timeout_ns", ctypes.c_int64), ("debug_flags", ctypes.c_uint32),
                 ("phases", ctypes.c_uint32), ("accumulate", ctypes.c_uint32)]
+
+
+def _wide(name, fields):
+    """A ctypes mirror of a structure whose fields are all 8 bytes wide, and
+    the struct.Struct that packs its fields in order, a tensor as its pointer
+    and four strides: one pack() call fills an argument block several times
+    faster than attribute by attribute, which is what a decoding step's calls
+    spend most of their host time on."""
+    cls = type(name, (ctypes.Structure,), {"_fields_": fields})
+    code = ""
+    for _, t in fields:
+        code += {Tensor: "5q", ctypes.c_int64: "q", ctypes.c_int64 * 2: "2q", ctypes.c_void_p: "q", ctypes.c_double: "d"}[t]
+    pack = struct.Struct("@" + code)
+    assert pack.size == ctypes.sizeof(cls)
+    return cls, pack.pack
+
+
+_i64, _ptr = ctypes.c_int64, ctypes.c_void_p
+
+RopeArgs, pack_rope = _wide("RopeArgs", [
+    ("batch", _i64), ("heads_q", _i64), ("heads_k", _i64), ("seqlen", _i64), ("head_dim", _i64),
+    ("rotary_dim", _i64), ("dtype", _i64), ("interleaved", _i64), ("inverse", _i64),
+    ("q", Tensor), ("k", Tensor), ("q_out", Tensor), ("k_out", Tensor), ("cos", _ptr), ("sin", _ptr),
+    ("table_rows", _i64), ("table_stride", _i64), ("positions", _ptr), ("positions_bytes", _i64),
+    ("positions_stride", _i64 * 2), ("offsets", _ptr), ("offsets_bytes", _i64), ("status", _ptr)])
+
+TreeArgs, pack_tree = _wide("TreeArgs", [
+    ("batch", _i64), ("heads_q", _i64), ("heads_kv", _i64), ("nodes", _i64), ("head_dim", _i64), ("dtype", _i64),
+    ("num_pages", _i64), ("page_size", _i64), ("max_pages", _i64), ("sliding_window", _i64),
+    ("scale", ctypes.c_double), ("soft_cap", ctypes.c_double), ("alibi_slopes", _ptr),
+    ("q", Tensor), ("k", Tensor), ("v", Tensor), ("o", Tensor), ("lse", _ptr), ("k_pages", Tensor), ("v_pages", Tensor),
+    ("page_table", _ptr), ("page_table_stride", _i64), ("lens", _ptr), ("parents", _ptr), ("parents_stride", _i64),
+    ("status", _ptr), ("workspace", _ptr), ("workspace_bytes", _i64)])
+
+VerifyArgs, pack_verify = _wide("VerifyArgs", [
+    ("batch", _i64), ("nodes", _i64), ("vocab", _i64), ("dtype", _i64), ("target", _ptr), ("target_stride", _i64 * 2),
+    ("draft", _ptr), ("draft_stride", _i64 * 2), ("tokens", _ptr), ("tokens_bytes", _i64), ("tokens_stride", _i64),
+    ("parents", _ptr), ("parents_stride", _i64), ("uniforms", _ptr), ("uniforms_stride", _i64), ("noise", _ptr),
+    ("noise_stride", _i64), ("path", _ptr), ("count", _ptr), ("next_token", _ptr), ("status", _ptr)])
+
+AppendArgs, pack_append = _wide("AppendArgs", [
+    ("batch", _i64), ("heads_kv", _i64), ("tokens", _i64), ("head_dim", _i64), ("dtype", _i64), ("num_pages", _i64),
+    ("page_size", _i64), ("max_pages", _i64), ("k", Tensor), ("v", Tensor), ("k_pages", Tensor), ("v_pages", Tensor),
+    ("page_table", _ptr), ("page_table_stride", _i64), ("lens", _ptr), ("take", _ptr), ("take_stride", _i64),
+    ("count", _ptr), ("lens_out", _ptr), ("status", _ptr)])
 
 
 _lib = None
@@ -105,6 +153,12 @@ def load() -> ctypes.CDLL:
         lib.bfa_merge_partial.argtypes = [ctypes.c_int32] * 4 + [
             Tensor, ctypes.c_int32, ctypes.c_void_p, Tensor, ctypes.c_int32, ctypes.c_void_p,
             ctypes.c_void_p]
+        # Packed argument blocks travel as bytes objects (a read-only pointer to them).
+        for name in ("bfa_rope", "bfa_tree_fwd", "bfa_verify_tree", "bfa_cache_append"):
+            fn = getattr(lib, name)
+            fn.restype, fn.argtypes = ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]
+        lib.bfa_tree_workspace_bytes.restype = ctypes.c_size_t
+        lib.bfa_tree_workspace_bytes.argtypes = [ctypes.c_char_p]
         ver = lib.bfa_abi_version()
         if ver != ABI_VERSION:
             raise RuntimeError(f"libbfa ABI version {ver}, expected {ABI_VERSION}")
@@ -140,6 +194,55 @@ def tensor(t: torch.Tensor | None) -> Tensor:
     for i, s in enumerate(t.stride()):
         out.stride[i] = s
     return out
+
+
+def flat(t: torch.Tensor | None) -> tuple:
+    """A [B, H, S, D] tensor's pointer and strides, as the packers take them."""
+    return (0, 0, 0, 0, 0) if t is None else (t.data_ptr(), *t.stride())
+
+
+def require_cuda(what: str, tensors, device=None) -> None:
+    """Every tensor is on one CUDA device (`device`, or the first one's)."""
+    for t in tensors:
+        if not t.is_cuda:
+            raise RuntimeError(f"{what} (B200 build) needs CUDA tensors; there is no CPU path")
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise RuntimeError(f"{what}: tensors on {device} and {t.device}; they must share a device")
+
+
+class on_device:
+    """torch.cuda.device for a device that is nearly always the current one:
+    it is entered only where it is not."""
+    __slots__ = ("guard",)
+
+    def __init__(self, device: torch.device):
+        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+CHECK_STATUS = os.environ.get("BFA_CHECK_STATUS", "0") == "1"
+
+
+def launch(name: str, packed: bytes, device: torch.device) -> None:
+    """One entry point that takes a packed argument block, on the device's
+    current stream."""
+    with on_device(device):
+        check(getattr(load(), name)(packed, stream_ptr(device)))
+    if CHECK_STATUS:
+        check(read_and_clear_status(device))
+
+
+def tree_workspace_bytes(packed: bytes) -> int:
+    return load().bfa_tree_workspace_bytes(packed)
 
 
 def stream_ptr(device: torch.device) -> int:

@@ -106,6 +106,8 @@ const char* bfa_strerror(int status) {
     case BFA_ERR_SCRATCH_LIMIT:
       return "bfa: problem exceeds bfa_bwd_noalloc's static scratch "
              "(batch*heads_q*ceil(seqlen_q/64)*64 > 2097152)";
+    case BFA_ERR_INDEX:
+      return "bfa: an index on the device (position, page, node, token, length or count) lies outside its table";
   }
   return "bfa: unknown status";
 }

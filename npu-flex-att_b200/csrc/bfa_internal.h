@@ -53,4 +53,13 @@ inline int dtype_bytes(int dt) {
   return dt == BFA_DTYPE_F32 ? 4 : (dt == BFA_DTYPE_F16 || dt == BFA_DTYPE_BF16) ? 2 : 0;
 }
 
+// Whether 16-byte vectors can address every row of a tensor (unit innermost
+// stride, 16-byte aligned base and outer strides).
+inline bool vector_rows(const bfa_tensor& t, int bytes) {
+  if (((uintptr_t)t.data & 15u) != 0 || t.stride[3] != 1) return false;
+  for (int i = 0; i < 3; ++i)
+    if (t.stride[i] * bytes % 16 != 0) return false;
+  return true;
+}
+
 }  // namespace bfa

@@ -1,0 +1,134 @@
+// cache_append.cu -- tokens into a paged K/V cache (a prompt, or the accepted
+// path of a tree of drafted tokens), K and V in one launch.
+//
+// For i < count[b], token take[b, i] (or i) of sequence b goes to position
+// lens[b] + i: page page_table[b, pos / page_size], slot pos % page_size. The
+// lengths are returned in a tensor of their own: every layer of a model
+// appends at the same old lengths, and no block reads a length that another
+// has already moved.
+//
+// Bound: HBM, 2 reads and 2 writes of count·Hkv·D elements. A thread owns one
+// 16-byte vector of a token's row (one element where strides or alignment do
+// not allow vectors), looks its page up once and copies K and V of kHeads
+// heads, all loads first: kHeads·2 vectors in flight. kHeads is 4 where that
+// still fills the GPU, else 1.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "bfa_internal.h"
+
+namespace bfa {
+namespace {
+
+struct AppendParams {
+  const void* k; const void* v; void* kp; void* vp;
+  int64_t sk[4], sv[4], skp[4], svp[4];
+  const int32_t* table; int64_t table_stride;
+  const int32_t* lens; const int32_t* take; int64_t take_stride;
+  const int32_t* count; int32_t* lens_out; int32_t* status;
+  int64_t num_pages;
+  int B, H, S, units, page, cap;  // cap: max_pages·page
+};
+
+template <typename U>  // what a thread copies at a time: 16 bytes, or one element
+__device__ __forceinline__ const U* row_at(const void* base, const int64_t* st, int64_t i0, int64_t i1, int64_t i2, int64_t u,
+                                           int per) {
+  // Strides are in elements; `per` elements make one U.
+  const int64_t e = i0 * st[0] + i1 * st[1] + i2 * st[2] + u * (per > 1 ? per : st[3]);
+  return reinterpret_cast<const U*>(static_cast<const char*>(base) + e * (int64_t)(sizeof(U) / per));
+}
+
+template <typename U, int kPer, int kHeads>
+__global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
+  const int idx = (int)(blockIdx.x * blockDim.x + threadIdx.x);
+  for (int b = blockIdx.z; b < p.B; b += gridDim.z) {
+    const int len0 = p.lens[b], n0 = p.count ? p.count[b] : p.S;
+    const int len = min(max(len0, 0), p.cap), n = min(max(n0, 0), p.S);
+    bool bad = len != len0 || n != n0;
+    if (idx == 0 && blockIdx.y == 0) {
+      p.lens_out[b] = (int)min((int64_t)len + n, (int64_t)p.cap);
+      if (bad && p.status) *p.status = BFA_ERR_INDEX;
+    }
+    const int i = idx / p.units, u = idx - i * p.units;
+    if (i >= n) continue;
+    const int node = p.take ? p.take[b * p.take_stride + i] : i;
+    const int64_t pos = (int64_t)len + i;
+    int32_t page = -1;
+    if (pos < p.cap) page = p.table[b * p.table_stride + pos / p.page];
+    if (node < 0 || node >= p.S || page < 0 || page >= p.num_pages) {
+      if (p.status) *p.status = BFA_ERR_INDEX;
+      continue;
+    }
+    const int slot = (int)pos % p.page;
+    const int h0 = blockIdx.y * kHeads;
+    U kx[kHeads], vx[kHeads];
+#pragma unroll
+    for (int j = 0; j < kHeads; ++j)
+      if (h0 + j < p.H) {
+        kx[j] = *row_at<U>(p.k, p.sk, b, h0 + j, node, u, kPer);
+        vx[j] = *row_at<U>(p.v, p.sv, b, h0 + j, node, u, kPer);
+      }
+#pragma unroll
+    for (int j = 0; j < kHeads; ++j)
+      if (h0 + j < p.H) {
+        *const_cast<U*>(row_at<U>(p.kp, p.skp, page, h0 + j, slot, u, kPer)) = kx[j];
+        *const_cast<U*>(row_at<U>(p.vp, p.svp, page, h0 + j, slot, u, kPer)) = vx[j];
+      }
+  }
+}
+
+template <typename U, int kPer>
+int launch_append(AppendParams& p, int D, cudaStream_t st) {
+  p.units = D / kPer;
+  const int64_t per_head = (int64_t)p.S * p.units;
+  if (per_head > INT32_MAX - 256) return BFA_ERR_UNSUPPORTED;
+  const bool four = per_head * p.B * ((p.H + 3) / 4) >= (int64_t)sm_count() * 2048;
+  const int heads = four ? (p.H + 3) / 4 : p.H;
+  if (heads > 65535) return BFA_ERR_UNSUPPORTED;
+  const int threads = (int)std::max<int64_t>(32, std::min<int64_t>(256, (per_head + 31) / 32 * 32));
+  const dim3 grid((unsigned)std::max<int64_t>(1, (per_head + threads - 1) / threads), (unsigned)heads,
+                  (unsigned)std::min(p.B, 65535));
+  if (four) append_kernel<U, kPer, 4><<<grid, threads, 0, st>>>(p);
+  else append_kernel<U, kPer, 1><<<grid, threads, 0, st>>>(p);
+  note_launch();
+  return launch_status("append kernel launch");
+}
+
+}  // namespace
+}  // namespace bfa
+
+extern "C" int bfa_cache_append(const bfa_append_args* a, void* stream) {
+  using namespace bfa;
+  if (!a || a->batch < 0 || a->heads_kv < 1 || a->tokens < 0 || a->head_dim < 1 || a->num_pages < 0 || a->page_size < 1 ||
+      a->max_pages < 0)
+    return BFA_ERR_INVALID_ARGUMENT;
+  const int bytes = a->dtype == (int)a->dtype ? dtype_bytes((int)a->dtype) : 0;
+  if (bytes == 0 || a->head_dim > 256) return BFA_ERR_UNSUPPORTED;
+  if (a->batch > INT32_MAX || a->heads_kv > INT32_MAX || a->tokens > INT32_MAX || a->page_size > INT32_MAX / 2 ||
+      a->max_pages > INT32_MAX / 2 / a->page_size)
+    return BFA_ERR_UNSUPPORTED;
+  if (a->batch == 0) return BFA_OK;
+  if (!a->lens || !a->lens_out || a->lens == a->lens_out) return BFA_ERR_INVALID_ARGUMENT;
+  if (a->tokens > 0 && a->max_pages > 0 && !a->page_table) return BFA_ERR_INVALID_ARGUMENT;
+  if (a->tokens > 0 && (!a->k.data || !a->v.data || (a->num_pages > 0 && (!a->k_pages.data || !a->v_pages.data))))
+    return BFA_ERR_INVALID_ARGUMENT;
+  AppendParams p{};
+  p.k = a->k.data; p.v = a->v.data; p.kp = a->k_pages.data; p.vp = a->v_pages.data;
+  for (int i = 0; i < 4; ++i) {
+    p.sk[i] = a->k.stride[i]; p.sv[i] = a->v.stride[i];
+    p.skp[i] = a->k_pages.stride[i]; p.svp[i] = a->v_pages.stride[i];
+  }
+  p.table = a->page_table; p.table_stride = a->page_table_stride;
+  p.lens = a->lens; p.take = a->take; p.take_stride = a->take_stride;
+  p.count = a->count; p.lens_out = a->lens_out; p.status = a->status;
+  p.num_pages = a->num_pages;
+  p.B = (int)a->batch; p.H = (int)a->heads_kv; p.S = (int)a->tokens; p.page = (int)a->page_size;
+  p.cap = (int)(a->max_pages * a->page_size);
+  const int D = (int)a->head_dim;
+  cudaStream_t st = (cudaStream_t)stream;
+  const bool vec = D * bytes % 16 == 0 && vector_rows(a->k, bytes) && vector_rows(a->v, bytes) &&
+                   vector_rows(a->k_pages, bytes) && vector_rows(a->v_pages, bytes);
+  if (bytes == 2) return vec ? launch_append<uint4, 8>(p, D, st) : launch_append<uint16_t, 1>(p, D, st);
+  return vec ? launch_append<uint4, 4>(p, D, st) : launch_append<uint32_t, 1>(p, D, st);
+}

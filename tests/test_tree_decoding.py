@@ -1,0 +1,100 @@
+"""Tree decoding, host side: argument blocks, C-level checks, depths, refusals
+(CPU only; the calls are rejected before any CUDA work)."""
+import ctypes
+import os
+import shutil
+import subprocess
+
+import pytest
+import torch
+
+import bfa_lib
+import tree_decoding as td
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def test_packed_blocks_match_header_layout(tmp_path):
+    if shutil.which("gcc") is None:
+        pytest.skip("gcc not available")
+    structs = {"bfa_rope_args": bfa_lib.RopeArgs, "bfa_tree_args": bfa_lib.TreeArgs, "bfa_verify_args": bfa_lib.VerifyArgs,
+               "bfa_append_args": bfa_lib.AppendArgs}
+    lines = ["#include <stdio.h>", "#include <stddef.h>", '#include "bfa.h"', "int main(void) {"]
+    for cname, cls in structs.items():
+        lines.append(f'  printf("{cname} size %zu\\n", sizeof({cname}));')
+        lines += [f'  printf("{cname} {f} %zu\\n", offsetof({cname}, {f}));' for f, _ in cls._fields_]
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    src.write_text("\n".join(lines + ["  return 0;", "}"]) + "\n")
+    subprocess.run(["gcc", "-std=c11", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout
+    got = {tuple(x.split()[:2]): int(x.split()[2]) for x in out.splitlines()}
+    for cname, cls in structs.items():
+        assert got[(cname, "size")] == ctypes.sizeof(cls)
+        for f, _ in cls._fields_:
+            assert got[(cname, f)] == getattr(cls, f).offset, (cname, f)
+
+
+def block(cls, **kw):
+    a = cls()
+    for key, x in kw.items():
+        setattr(a, key, x)
+    return bytes(a)
+
+
+TREE = dict(batch=1, heads_q=4, heads_kv=2, nodes=3, head_dim=64, dtype=2, num_pages=1, page_size=16, max_pages=1)
+VERIFY = dict(batch=1, nodes=3, vocab=10, dtype=0)
+APPEND = dict(batch=1, heads_kv=2, tokens=3, head_dim=64, dtype=2, num_pages=1, page_size=16, max_pages=1)
+ROPE = dict(batch=1, heads_q=1, heads_k=1, seqlen=4, head_dim=64, rotary_dim=64, dtype=2, table_rows=4)
+
+
+@pytest.mark.parametrize("name,cls,base,kw,code", [
+    ("bfa_tree_fwd", "TreeArgs", TREE, dict(heads_q=3), -2), ("bfa_tree_fwd", "TreeArgs", TREE, dict(nodes=65), -3),
+    ("bfa_tree_fwd", "TreeArgs", TREE, dict(nodes=0), -1), ("bfa_tree_fwd", "TreeArgs", TREE, dict(head_dim=257), -3),
+    ("bfa_tree_fwd", "TreeArgs", TREE, dict(dtype=5), -3), ("bfa_tree_fwd", "TreeArgs", TREE, dict(soft_cap=-1.0), -1),
+    ("bfa_tree_fwd", "TreeArgs", TREE, dict(soft_cap=float("nan")), -1), ("bfa_tree_fwd", "TreeArgs", TREE, dict(page_size=0), -1),
+    ("bfa_tree_fwd", "TreeArgs", TREE, dict(max_pages=2 ** 40), -3), ("bfa_tree_fwd", "TreeArgs", TREE, dict(), -1),
+    ("bfa_tree_fwd", "TreeArgs", TREE, dict(batch=0), 0),
+    ("bfa_verify_tree", "VerifyArgs", VERIFY, dict(nodes=65), -3), ("bfa_verify_tree", "VerifyArgs", VERIFY, dict(vocab=0), -1),
+    ("bfa_verify_tree", "VerifyArgs", VERIFY, dict(), -1), ("bfa_verify_tree", "VerifyArgs", VERIFY, dict(batch=0), 0),
+    ("bfa_verify_tree", "VerifyArgs", VERIFY, dict(dtype=-1), -3),
+    ("bfa_cache_append", "AppendArgs", APPEND, dict(page_size=0), -1), ("bfa_cache_append", "AppendArgs", APPEND, dict(), -1),
+    ("bfa_cache_append", "AppendArgs", APPEND, dict(head_dim=300), -3), ("bfa_cache_append", "AppendArgs", APPEND, dict(batch=0), 0),
+    ("bfa_rope", "RopeArgs", ROPE, dict(rotary_dim=7), -1), ("bfa_rope", "RopeArgs", ROPE, dict(rotary_dim=66), -2),
+    ("bfa_rope", "RopeArgs", ROPE, dict(interleaved=2), -1), ("bfa_rope", "RopeArgs", ROPE, dict(dtype=3), -3),
+    ("bfa_rope", "RopeArgs", ROPE, dict(), -1), ("bfa_rope", "RopeArgs", ROPE, dict(seqlen=0), 0)])
+def test_entry_points_check_their_arguments(name, cls, base, kw, code):
+    lib = bfa_lib.load()
+    assert getattr(lib, name)(block(getattr(bfa_lib, cls), **dict(base, **kw)), None) == code
+    assert getattr(lib, name)(None, None) == -1
+
+
+def test_status_has_a_message():
+    assert "index" in bfa_lib.load().bfa_strerror(bfa_lib.ERR_INDEX).decode()
+
+
+def test_workspace_bytes_of_invalid_problems():
+    lib = bfa_lib.load()
+    assert lib.bfa_tree_workspace_bytes(None) == 0
+    assert lib.bfa_tree_workspace_bytes(block(bfa_lib.TreeArgs, **dict(TREE, heads_q=3))) == 0
+    assert lib.bfa_tree_workspace_bytes(block(bfa_lib.TreeArgs, **dict(TREE, batch=0))) == 0
+    assert lib.bfa_tree_workspace_bytes(block(bfa_lib.TreeArgs, **TREE)) > 0
+
+
+def test_depths():
+    t = torch.tensor([[-1, 0, 0, 1, 3, 2], [-1, 0, 1, 2, 3, 4], [5, -1, 0, 1, -1, 2]], dtype=torch.int32)
+    d = td.tree_depths(t)
+    assert d.dtype == torch.int32 and d[0].tolist() == [0, 1, 1, 2, 3, 2] and d[1].tolist() == [0, 1, 2, 3, 4, 5]
+    assert d[2, 0] == 0 and d[2, 2] == 1 and d[2, 5] == 2
+    assert td.tree_depths(t[0]).tolist() == d[0].tolist() and td.tree_depths(torch.tensor([-1])).tolist() == [0]
+
+
+def test_cpu_tensors_are_refused():
+    q, k = torch.randn(1, 2, 3, 64), torch.randn(1, 1, 3, 64)
+    cache = td.PagedKVCache(torch.zeros(1, 1, 16, 64), torch.zeros(1, 1, 16, 64), torch.zeros(1, 1, dtype=torch.int32),
+                            torch.zeros(1, dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        td.tree_attention(q, k, k, cache)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        td.cache_append(cache, k, k)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        td.verify_tree(torch.ones(1, 3, 4), torch.zeros(1, 3, dtype=torch.int64), None, torch.rand(1, 3), torch.ones(1, 4))
