@@ -7,6 +7,7 @@ implementation: if the library is missing, every call raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import struct
 import threading
@@ -97,6 +98,8 @@ TreeArgs, pack_tree = _wide("TreeArgs", [
     ("q", Tensor), ("k", Tensor), ("v", Tensor), ("o", Tensor), ("lse", _ptr), ("k_pages", Tensor), ("v_pages", Tensor),
     ("page_table", _ptr), ("page_table_stride", _i64), ("lens", _ptr), ("parents", _ptr), ("parents_stride", _i64),
     ("status", _ptr), ("workspace", _ptr), ("workspace_bytes", _i64)])
+
+_TREE_VALUES = sum(5 if t is Tensor else 1 for _, t in TreeArgs._fields_)
 
 VerifyArgs, pack_verify = _wide("VerifyArgs", [
     ("batch", _i64), ("nodes", _i64), ("vocab", _i64), ("dtype", _i64), ("target", _ptr), ("target_stride", _i64 * 2),
@@ -212,37 +215,48 @@ def require_cuda(what: str, tensors, device=None) -> None:
             raise RuntimeError(f"{what}: tensors on {device} and {t.device}; they must share a device")
 
 
-class on_device:
-    """torch.cuda.device for a device that is nearly always the current one:
-    it is entered only where it is not."""
-    __slots__ = ("guard",)
-
-    def __init__(self, device: torch.device):
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-
-
 CHECK_STATUS = os.environ.get("BFA_CHECK_STATUS", "0") == "1"
+_functions = {}
 
 
 def launch(name: str, packed: bytes, device: torch.device) -> None:
     """One entry point that takes a packed argument block, on the device's
-    current stream."""
-    with on_device(device):
-        check(getattr(load(), name)(packed, stream_ptr(device)))
+    current stream. The tensors exist, so CUDA is initialised and the raw
+    calls (current device, current stream's handle) need no guard of torch's;
+    a decoding step makes a few such calls per layer, and their host time is
+    what it waits for."""
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(load(), name)
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(packed, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(packed, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc)
     if CHECK_STATUS:
         check(read_and_clear_status(device))
 
 
-def tree_workspace_bytes(packed: bytes) -> int:
-    return load().bfa_tree_workspace_bytes(packed)
+_status_at = {}
+
+
+def status_ptr(device: torch.device) -> int:
+    """Address of the device's status word."""
+    at = _status_at.get(device.index)
+    if at is None:
+        at = _status_at[device.index] = status_word(device).data_ptr()
+    return at
+
+
+@functools.lru_cache(maxsize=4096)
+def tree_workspace_bytes(index: int, *sizes) -> int:
+    """bfa_tree_workspace_bytes of a device and the sizes that open a
+    bfa_tree_args block (batch ... soft_cap); it depends on nothing else."""
+    with torch.cuda.device(index):
+        return load().bfa_tree_workspace_bytes(pack_tree(*sizes, *[0] * (_TREE_VALUES - len(sizes))))
 
 
 def stream_ptr(device: torch.device) -> int:

@@ -3,6 +3,8 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "bfa_common.cuh"
 
 namespace bfa {
@@ -51,6 +53,23 @@ int launch_status(const char* what);
 // Bytes of one element of a bfa_dtype (0 when invalid).
 inline int dtype_bytes(int dt) {
   return dt == BFA_DTYPE_F32 ? 4 : (dt == BFA_DTYPE_F16 || dt == BFA_DTYPE_BF16) ? 2 : 0;
+}
+
+// Lets `kernel` use `bytes` of dynamic shared memory on the current device;
+// asked of the runtime once per kernel and device (`done`: one bit a device,
+// owned by the call site).
+template <typename K>
+inline int allow_shared(K kernel, int bytes, std::atomic<uint64_t>& done, const char* what) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && dev < 64 && ((done.load(std::memory_order_relaxed) >> dev) & 1)) return BFA_OK;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return cuda_fail(what, e);
+  }
+  if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return BFA_OK;
 }
 
 // Whether 16-byte vectors can address every row of a tensor (unit innermost

@@ -96,16 +96,17 @@ struct Plan {
 Plan make_plan(const bfa_tree_args* a) {
   Plan pl{};
   const int64_t rows = a->heads_q / a->heads_kv * a->nodes;
-  pl.rb = kTreeSimtRows;
-  pl.chunk = kTreeSimtChunk;
-  int per_sm = kTreeSimtPerSm;
+  const TreeTile tile = a->dtype == BFA_DTYPE_F32 ? TreeTile{kTreeSimtRows, kTreeSimtChunk, a->head_dim > 128 ? 1 : 2}
+                                                  : tree_mma_tile(rows, (int)a->head_dim);
+  pl.rb = tile.rb;
+  pl.chunk = tile.chunk;
   pl.n_rb = (int)((rows + pl.rb - 1) / pl.rb);
   pl.tree_chunks = (int)((a->nodes + pl.chunk - 1) / pl.chunk);
   // At most one stretch per chunk that the tables could hold.
   int64_t seen = a->max_pages * a->page_size;
   if (a->sliding_window > 0) seen = std::min(seen, a->sliding_window);
   const int64_t chunks = ((seen + pl.chunk - 1) / pl.chunk + pl.tree_chunks) * a->batch * a->heads_kv * pl.n_rb;
-  pl.grid = (int)std::min<int64_t>(chunks, (int64_t)sm_count() * per_sm);
+  pl.grid = (int)std::min<int64_t>(chunks, (int64_t)sm_count() * tile.per_sm);
   const size_t rows_ws = (size_t)pl.grid * 2 * pl.rb;
   pl.lse_at = (rows_ws * a->head_dim * 4 + 255) / 256 * 256;
   pl.bytes = pl.lse_at + (rows_ws * 4 + 255) / 256 * 256;
@@ -167,7 +168,7 @@ extern "C" int bfa_tree_fwd(const bfa_tree_args* a, void* stream) {
   p.part_o = static_cast<float*>(a->workspace);
   p.part_lse = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + pl.lse_at);
   cudaStream_t st = (cudaStream_t)stream;
-  int rc = tree_simt(p, (int)a->dtype, st);
+  const int rc = a->dtype == BFA_DTYPE_F32 ? tree_simt(p, st) : tree_mma(p, (int)a->dtype, st);
   if (rc) return rc;
   switch (a->dtype) {
     case BFA_DTYPE_F32: return launch_merge<float>(p, st);

@@ -120,16 +120,17 @@ struct TreeCursor {
   }
 };
 
-// The rows of K and V that key j of a chunk lies in (byte addresses; 0 reads
-// as zeros). Reports a bad page or length.
+// The rows of K and V that key j of a chunk lies in (null reads as zeros).
+// Reports a bad page. Rows of absent nodes are read like the others: their
+// logits are masked, and the kernels keep values that a row does not see out
+// of its sum even where they are not finite.
 template <int kBytes>
-__device__ __forceinline__ void tree_key_rows(const TreeParams& p, const TreeCursor& cur, int j, uint64_t present, const char** kr,
-                                              const char** vr) {
+__device__ __forceinline__ void tree_key_rows(const TreeParams& p, const TreeCursor& cur, int j, const char** kr, const char** vr) {
   *kr = *vr = nullptr;
   const int hkv = cur.item / p.n_rb;
   const int key = cur.key0(p) + j;
   if (cur.in_tree(p)) {
-    if (key >= p.N || !((present >> key) & 1)) return;
+    if (key >= p.N) return;
     *kr = static_cast<const char*>(p.k) + (cur.b * p.sk[0] + hkv * p.sk[1] + key * p.sk[2]) * kBytes;
     *vr = static_cast<const char*>(p.v) + (cur.b * p.sv[0] + hkv * p.sv[1] + key * p.sv[2]) * kBytes;
     return;
@@ -152,7 +153,6 @@ struct TreeMasks {
   uint64_t anc[kTreeNodes];
   int32_t depth[kTreeNodes];
   int32_t up[kTreeNodes];
-  uint64_t present;
 };
 __device__ __forceinline__ void tree_masks(const TreeParams& p, int b, TreeMasks& m) {
   const int lane = threadIdx.x & 31;
@@ -193,15 +193,12 @@ __device__ __forceinline__ void tree_masks(const TreeParams& p, int b, TreeMasks
     }
     __syncwarp();
   }
-  unsigned there[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int n = lane + 32 * h;
     if (!(m.anc[n] & 1)) m.anc[n] = 0;  // does not hang under the root
     m.depth[n] = max(0, __popcll(m.anc[n]) - 1);
-    there[h] = __ballot_sync(0xffffffffu, m.anc[n] != 0);
   }
-  if (lane == 0) m.present = there[0] | ((uint64_t)there[1] << 32);
   __syncwarp();
 }
 
@@ -231,8 +228,18 @@ __device__ __forceinline__ float tree_row_shift(const TreeParams& p, int hq, int
   return slope * (float)(pos - tree_alibi_ref(p, slope, pos));
 }
 
-// tree_simt.cu: CUDA-core kernel, every dtype and layout.
-int tree_simt(const TreeParams& p, int dtype, cudaStream_t st);
-constexpr int kTreeSimtRows = 32, kTreeSimtChunk = 32, kTreeSimtPerSm = 1;
+// How a kernel cuts a problem: rows per block, keys per chunk, resident blocks
+// per SM.
+struct TreeTile {
+  int rb, chunk, per_sm;
+};
+
+// tree_simt.cu: CUDA cores, the fp32 path.
+int tree_simt(const TreeParams& p, cudaStream_t st);
+constexpr int kTreeSimtRows = 32, kTreeSimtChunk = 32;
+
+// tree_mma.cu: bf16 / fp16 on mma.sync.
+TreeTile tree_mma_tile(int64_t rows, int D);
+int tree_mma(const TreeParams& p, int dtype, cudaStream_t st);
 
 }  // namespace bfa

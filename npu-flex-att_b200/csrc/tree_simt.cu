@@ -80,23 +80,8 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const TreeParams p,
 
   auto lookup = [&](int buf) {  // fills the row addresses of chunk `ahead`
     if (tid < kKeys) {
-      uint64_t present = ~0ull;
-      if (ahead.in_tree(p)) {
-        // The masks in shared memory may be another sequence's: walk up from
-        // the node, which is present when it reaches the root.
-        int n = ahead.key0(p) + tid;
-        present = 0;
-        if (n < p.N) {
-          const int me = n;
-          while (n > 0) {
-            const int up = p.parents ? p.parents[ahead.b * p.parents_stride + n] : n - 1;
-            n = (up < 0 || up >= n) ? -1 : up;
-          }
-          if (n == 0) present = 1ull << me;
-        }
-      }
       const char *kr, *vr;
-      tree_key_rows<(int)sizeof(T)>(p, ahead, tid, present, &kr, &vr);
+      tree_key_rows<(int)sizeof(T)>(p, ahead, tid, &kr, &vr);
       sh.krow[buf][tid] = kr;
       sh.vrow[buf][tid] = vr;
     }
@@ -289,8 +274,9 @@ template <typename T, int D>
 int launch(const TreeParams& p, cudaStream_t st) {
   const int bytes = (int)(sizeof(SimtShared) + 15) / 16 * 16 + (kRows + 4 * kKeys) * (D + 4) * 4;
   auto kernel = tree_simt_kernel<T, D>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) return cuda_fail("tree_simt shared memory", e);
+  static std::atomic<uint64_t> done;
+  const int rc = allow_shared(kernel, bytes, done, "tree attention shared memory");
+  if (rc) return rc;
   auto rows = [](const void* d, const int64_t* s) {
     return ((uintptr_t)d & 15u) == 0 && s[0] % 4 == 0 && s[1] % 4 == 0 && s[2] % 4 == 0;
   };
@@ -300,21 +286,12 @@ int launch(const TreeParams& p, cudaStream_t st) {
   return launch_status("tree attention launch");
 }
 
-template <typename T>
-int launch_d(const TreeParams& p, cudaStream_t st) {
-  if (p.D <= 64) return launch<T, 64>(p, st);
-  if (p.D <= 128) return launch<T, 128>(p, st);
-  return launch<T, 256>(p, st);
-}
-
 }  // namespace
 
-int tree_simt(const TreeParams& p, int dtype, cudaStream_t st) {
-  switch (dtype) {
-    case BFA_DTYPE_F32: return launch_d<float>(p, st);
-    case BFA_DTYPE_F16: return launch_d<__half>(p, st);
-    default: return launch_d<__nv_bfloat16>(p, st);
-  }
+int tree_simt(const TreeParams& p, cudaStream_t st) {
+  if (p.D <= 64) return launch<float, 64>(p, st);
+  if (p.D <= 128) return launch<float, 128>(p, st);
+  return launch<float, 256>(p, st);
 }
 
 }  // namespace bfa

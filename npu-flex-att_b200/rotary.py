@@ -88,7 +88,7 @@ def _launch(q, k, cos, sin, positions, offsets, interleaved, inverse, out=None):
         _bfa.bfa_dtype(some.dtype), 1 if interleaved else 0, 1 if inverse else 0,
         *(_bfa.flat(q)), *(_bfa.flat(k)), *(_bfa.flat(qo)), *(_bfa.flat(ko)),
         cos.data_ptr(), sin.data_ptr(), cos.shape[0], cos.stride(0), pos, pos_bytes, pos_b, pos_s, off, off_bytes,
-        _bfa.status_word(dev).data_ptr())
+        _bfa.status_ptr(dev))
     _bfa.launch("bfa_rope", packed, dev)
     return qo, ko
 

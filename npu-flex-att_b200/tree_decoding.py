@@ -132,16 +132,16 @@ def tree_attention(query, key, value, cache, parents=None, *, scale=None, slidin
     q, k, v = _rows(query), _rows(key), _rows(value)
     o = torch.empty((B, Hq, N, D), dtype=dt, device=dev)
     lse = torch.empty((B, Hq, N), dtype=torch.float32, device=dev) if return_lse else None
-    head = (B, Hq, Hkv, N, D, _bfa.bfa_dtype(dt), kp.shape[0], kp.shape[2], table.shape[1], int(sliding_window),
-            float(scale) if scale is not None else 1.0 / math.sqrt(D), float(soft_cap),
-            slopes.data_ptr() if slopes is not None else 0,
-            *_bfa.flat(q), *_bfa.flat(k), *_bfa.flat(v), *_bfa.flat(o), lse.data_ptr() if return_lse else 0,
-            *_bfa.flat(kp), *_bfa.flat(vp), table.data_ptr(), table.stride(0), lens.data_ptr(), up, up_stride,
-            _bfa.status_word(dev).data_ptr())
-    with _bfa.on_device(dev):
-        nbytes = _bfa.tree_workspace_bytes(_bfa.pack_tree(*head, 0, 0))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        _bfa.launch("bfa_tree_fwd", _bfa.pack_tree(*head, ws.data_ptr() if nbytes else 0, nbytes), dev)
+    sizes = (B, Hq, Hkv, N, D, _bfa.bfa_dtype(dt), kp.shape[0], kp.shape[2], table.shape[1], int(sliding_window),
+             float(scale) if scale is not None else 1.0 / math.sqrt(D), float(soft_cap))
+    # Scratch of the partial results, from torch's caching allocator: the library allocates nothing.
+    nbytes = _bfa.tree_workspace_bytes(dev.index, *sizes)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _bfa.launch("bfa_tree_fwd", _bfa.pack_tree(
+        *sizes, slopes.data_ptr() if slopes is not None else 0,
+        *_bfa.flat(q), *_bfa.flat(k), *_bfa.flat(v), *_bfa.flat(o), lse.data_ptr() if return_lse else 0,
+        *_bfa.flat(kp), *_bfa.flat(vp), table.data_ptr(), table.stride(0), lens.data_ptr(), up, up_stride,
+        _bfa.status_ptr(dev), ws.data_ptr(), nbytes), dev)
     return (o, lse) if return_lse else o
 
 
@@ -195,7 +195,7 @@ def verify_tree(target_probs, draft_tokens, parents, uniforms, noise, *, draft_p
     packed = _bfa.pack_verify(
         B, N, V, _bfa.bfa_dtype(p.dtype), p.data_ptr(), p.stride(0), p.stride(1), law, law_b, law_n,
         tokens.data_ptr(), tokens.element_size(), tokens.stride(0), up, up_stride, u.data_ptr(), u.stride(0),
-        e.data_ptr(), e.stride(0), at, at + 4 * B * N, at + 4 * B * (N + 1), _bfa.status_word(dev).data_ptr())
+        e.data_ptr(), e.stride(0), at, at + 4 * B * N, at + 4 * B * (N + 1), _bfa.status_ptr(dev))
     _bfa.launch("bfa_verify_tree", packed, dev)
     return path, count, token
 
@@ -232,6 +232,6 @@ def cache_append(cache, key, value, *, take=None, count=None):
         B, Hkv, S, D, _bfa.bfa_dtype(dt), kp.shape[0], kp.shape[2], table.shape[1], *_bfa.flat(key.detach()),
         *_bfa.flat(value.detach()), *_bfa.flat(kp), *_bfa.flat(vp), table.data_ptr(), table.stride(0), lens.data_ptr(),
         take.data_ptr() if take is not None else 0, take.stride(0) if take is not None else 0,
-        count.data_ptr() if count is not None else 0, out.data_ptr(), _bfa.status_word(dev).data_ptr())
+        count.data_ptr() if count is not None else 0, out.data_ptr(), _bfa.status_ptr(dev))
     _bfa.launch("bfa_cache_append", packed, dev)
     return out
