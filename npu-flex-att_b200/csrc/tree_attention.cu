@@ -4,22 +4,30 @@
 
 #include <algorithm>
 #include <climits>
+#include <cstdlib>
 
 #include "tree_common.cuh"
 
 namespace bfa {
 namespace {
 
-// Joins the partial (O, LSE) of items that several blocks worked on, one warp
-// per row, partials in the order of their keys:
+// Joins the partial (O, LSE) of items that several blocks worked on, partials
+// in the order of their keys:
 //   lse = log2 sum_i 2^lse_i,  O = sum_i O_i·2^(lse_i - lse).
-// Rows of an item that one block did whole are already final.
-template <typename T>
+// Rows of an item that one block did whole are already final. kWarps warps
+// take a row: each sums every kWarps-th partial, eight loads in flight, and
+// the first adds the warps' sums in order. One warp where an item has few
+// partials (many items), four where a few items are spread over the GPU.
+// kVec: columns per lane and load (4 where D allows it, else 1).
+template <typename T, int kWarps, int kVec>
 __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeParams p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  constexpr int kRowsPer = 4 / kWarps;
+  constexpr int kLoads = kVec == 4 ? 2 : 8;  // of 32·kVec columns: 256
+  __shared__ float part[4][kVec * kLoads * 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % kWarps;
+  const int64_t row = (int64_t)blockIdx.x * kRowsPer + warp / kWarps;
   const int GN = p.G * p.N;
-  if (row >= (int64_t)p.B * p.Hkv * GN) return;
+  if (row >= (int64_t)p.B * p.Hkv * GN) return;  // whole blocks where kWarps is 4
   const int r_all = (int)(row % GN), hkv = (int)(row / GN % p.Hkv), b = (int)(row / GN / p.Hkv);
   const int rbk = r_all / p.rb, r = r_all - rbk * p.rb;
   const int64_t T_all = tree_chunks_before(p, p.B);
@@ -33,27 +41,61 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeParams p) {
   for (int i = i0 + lane; i <= i1; i += 32) m = fmaxf(m, p.part_lse[slot(i)]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  float total = 0.f, acc[kLoads][kVec];
+#pragma unroll
+  for (int c = 0; c < kLoads; ++c)
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) acc[c][e] = 0.f;
+  if (m != neg_inf()) {
+    for (int j0 = i0; j0 <= i1; j0 += 32) {
+      const float w = j0 + lane <= i1 ? exp2f(p.part_lse[slot(j0 + lane)] - m) : 0.f;
+      float sum = w;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      total += sum;
+      const int n = min(32, i1 - j0 + 1);
+#pragma unroll 8
+      for (int j = sub; j < n; j += kWarps) {
+        const float wj = __shfl_sync(0xffffffffu, w, j);
+        const float* po = p.part_o + slot(j0 + j) * p.D;
+#pragma unroll
+        for (int c = 0; c < kLoads; ++c) {
+          const int d = (lane + 32 * c) * kVec;
+          if (d >= p.D) continue;
+          float f[kVec];
+          if constexpr (kVec == 4) *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(po + d);
+          else f[0] = po[d];
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) acc[c][e] = fmaf(wj, f[e], acc[c][e]);
+        }
+      }
+    }
+  }
+  if constexpr (kWarps > 1) {
+#pragma unroll
+    for (int c = 0; c < kLoads; ++c)
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) part[warp][(c * kVec + e) * 32 + lane] = acc[c][e];
+    __syncthreads();
+    if (sub != 0) return;
+#pragma unroll
+    for (int c = 0; c < kLoads; ++c)
+#pragma unroll
+      for (int e = 0; e < kVec; ++e)
+#pragma unroll
+        for (int k = 1; k < kWarps; ++k) acc[c][e] += part[warp + k][(c * kVec + e) * 32 + lane];
+  }
   int hq, n;
   tree_row(p, hkv, r_all, &hq, &n);
   T* out = static_cast<T*>(p.o) + b * p.so[0] + hq * p.so[1] + n * p.so[2];
-  float total = 0.f, acc[8];
-#pragma unroll
-  for (int c = 0; c < 8; ++c) acc[c] = 0.f;
-  if (m != neg_inf()) {
-    for (int i = i0; i <= i1; ++i) {
-      const int64_t at = slot(i);
-      const float w = exp2f(p.part_lse[at] - m);
-      total += w;
-      const float* po = p.part_o + at * p.D;
-#pragma unroll
-      for (int c = 0; c < 8; ++c)
-        if (lane + 32 * c < p.D) acc[c] = fmaf(w, po[lane + 32 * c], acc[c]);
-    }
-  }
   const float inv = total > 0.f ? 1.f / total : 0.f;
 #pragma unroll
-  for (int c = 0; c < 8; ++c)
-    if (lane + 32 * c < p.D) out[lane + 32 * c] = from_f32<T>(acc[c] * inv);
+  for (int c = 0; c < kLoads; ++c)
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      const int d = (lane + 32 * c) * kVec + e;
+      if (d < p.D) out[d] = from_f32<T>(acc[c][e] * inv);
+    }
   if (lane == 0 && p.lse) {
     float l = neg_inf();
     if (total > 0.f) {
@@ -87,24 +129,22 @@ int check_tree(const bfa_tree_args* a) {
   return BFA_OK;
 }
 
+// Row block, chunk and grid of a problem.
 struct Plan {
   int rb, n_rb, chunk, tree_chunks, grid;
   size_t lse_at, bytes;
 };
 
-// Row block, chunk and grid of a problem: a function of sizes and type alone.
-Plan make_plan(const bfa_tree_args* a) {
+Plan make_plan(const bfa_tree_args* a, const TreeTile& tile) {
   Plan pl{};
   const int64_t rows = a->heads_q / a->heads_kv * a->nodes;
-  const TreeTile tile = a->dtype == BFA_DTYPE_F32 ? TreeTile{kTreeSimtRows, kTreeSimtChunk, a->head_dim > 128 ? 1 : 2}
-                                                  : tree_mma_tile(rows, (int)a->head_dim);
   pl.rb = tile.rb;
   pl.chunk = tile.chunk;
   pl.n_rb = (int)((rows + pl.rb - 1) / pl.rb);
   pl.tree_chunks = (int)((a->nodes + pl.chunk - 1) / pl.chunk);
   // At most one stretch per chunk that the tables could hold.
   int64_t seen = a->max_pages * a->page_size;
-  if (a->sliding_window > 0) seen = std::min(seen, a->sliding_window);
+  if (a->sliding_window > 0) seen = std::min(seen, a->sliding_window + pl.chunk);
   const int64_t chunks = ((seen + pl.chunk - 1) / pl.chunk + pl.tree_chunks) * a->batch * a->heads_kv * pl.n_rb;
   pl.grid = (int)std::min<int64_t>(chunks, (int64_t)sm_count() * tile.per_sm);
   const size_t rows_ws = (size_t)pl.grid * 2 * pl.rb;
@@ -113,10 +153,41 @@ Plan make_plan(const bfa_tree_args* a) {
   return pl;
 }
 
+TreeTile simt_tile(const bfa_tree_args* a) { return {kTreeSimtRows, kTreeSimtChunk, a->head_dim > 128 ? 1 : 2}; }
+
+// Rows per KV head from which the tcgen05 kernel is taken, where the layouts allow it.
+constexpr int64_t kTcgen05Rows = 33;
+
+bool tcgen05_on() {  // BFA_TREE_TCGEN05=0 keeps bf16/fp16 on the mma.sync kernel, =1 on tcgen05 at any row count
+  const char* e = std::getenv("BFA_TREE_TCGEN05");
+  return !(e && e[0] == '0');
+}
+bool tcgen05_always() {
+  const char* e = std::getenv("BFA_TREE_TCGEN05");
+  return e && e[0] == '1';
+}
+
+// Workspace for either 16-bit kernel: which one runs depends on the layouts,
+// the workspace on the sizes alone.
+size_t workspace_bytes(const bfa_tree_args* a) {
+  if (a->dtype == BFA_DTYPE_F32) return make_plan(a, simt_tile(a)).bytes;
+  const int64_t rows = a->heads_q / a->heads_kv * a->nodes;
+  return std::max(make_plan(a, tree_mma_tile(rows, (int)a->head_dim)).bytes, make_plan(a, tree_sm100_tile(rows, (int)a->head_dim)).bytes);
+}
+
 template <typename T>
 int launch_merge(const TreeParams& p, cudaStream_t st) {
   const int64_t rows = (int64_t)p.B * p.Hkv * p.G * p.N;
-  tree_merge_kernel<T><<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(p);
+  // Four warps per row where an item is spread over at least four blocks on average.
+  const bool wide = p.grid >= 4 * (int64_t)p.B * p.Hkv * p.n_rb;
+  const unsigned blocks = (unsigned)(wide ? rows : (rows + 3) / 4);
+  if (p.D % 4 == 0) {
+    if (wide) tree_merge_kernel<T, 4, 4><<<blocks, 128, 0, st>>>(p);
+    else tree_merge_kernel<T, 1, 4><<<blocks, 128, 0, st>>>(p);
+  } else {
+    if (wide) tree_merge_kernel<T, 4, 1><<<blocks, 128, 0, st>>>(p);
+    else tree_merge_kernel<T, 1, 1><<<blocks, 128, 0, st>>>(p);
+  }
   note_launch();
   return launch_status("tree merge launch");
 }
@@ -127,7 +198,7 @@ int launch_merge(const TreeParams& p, cudaStream_t st) {
 extern "C" size_t bfa_tree_workspace_bytes(const bfa_tree_args* a) {
   using namespace bfa;
   if (check_tree(a) || a->batch * a->heads_q == 0) return 0;
-  return make_plan(a).bytes;
+  return workspace_bytes(a);
 }
 
 extern "C" int bfa_tree_fwd(const bfa_tree_args* a, void* stream) {
@@ -141,9 +212,12 @@ extern "C" int bfa_tree_fwd(const bfa_tree_args* a, void* stream) {
   const bfa_tensor* unit[] = {&a->q, &a->k, &a->v, &a->o, &a->k_pages, &a->v_pages};
   for (const bfa_tensor* t : unit)
     if (t->data && a->head_dim > 1 && t->stride[3] != 1) return BFA_ERR_UNSUPPORTED;
-  const Plan pl = make_plan(a);
-  if (!a->workspace || a->workspace_bytes < (int64_t)pl.bytes || ((uintptr_t)a->workspace & 255u) != 0)
+  if (!a->workspace || a->workspace_bytes < (int64_t)workspace_bytes(a) || ((uintptr_t)a->workspace & 255u) != 0)
     return BFA_ERR_WORKSPACE;
+  const int64_t rows = a->heads_q / a->heads_kv * a->nodes;
+  const bool f32 = a->dtype == BFA_DTYPE_F32;
+  const bool tc = !f32 && tcgen05_on() && (rows >= kTcgen05Rows || tcgen05_always()) && tree_sm100_layout(a);
+  const Plan pl = make_plan(a, f32 ? simt_tile(a) : tc ? tree_sm100_tile(rows, (int)a->head_dim) : tree_mma_tile(rows, (int)a->head_dim));
   TreeParams p{};
   p.q = a->q.data; p.k = a->k.data; p.v = a->v.data; p.o = a->o.data;
   p.lse = a->lse;
@@ -168,7 +242,7 @@ extern "C" int bfa_tree_fwd(const bfa_tree_args* a, void* stream) {
   p.part_o = static_cast<float*>(a->workspace);
   p.part_lse = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + pl.lse_at);
   cudaStream_t st = (cudaStream_t)stream;
-  const int rc = a->dtype == BFA_DTYPE_F32 ? tree_simt(p, st) : tree_mma(p, (int)a->dtype, st);
+  const int rc = f32 ? tree_simt(p, st) : tc ? tree_sm100(p, (int)a->dtype, st) : tree_mma(p, (int)a->dtype, st);
   if (rc) return rc;
   switch (a->dtype) {
     case BFA_DTYPE_F32: return launch_merge<float>(p, st);

@@ -41,9 +41,12 @@ struct TreeParams {
 __device__ __forceinline__ int tree_len(const TreeParams& p, int b) {
   return min(max(p.lens[b], 0), p.cap_tokens);
 }
-// First visible cached token: with a window the root, at position len, sees
-// keys j >= len - W; deeper nodes see less.
-__device__ __forceinline__ int tree_lo(const TreeParams& p, int len) { return p.window > 0 ? max(0, len - p.window) : 0; }
+// First cached token that is read: with a window the root, at position len,
+// sees keys j >= len - W (deeper nodes see less), rounded down to a whole
+// chunk, so that chunks start at multiples of their length.
+__device__ __forceinline__ int tree_lo(const TreeParams& p, int len) {
+  return p.window > 0 ? max(0, len - p.window) / p.chunk * p.chunk : 0;
+}
 __device__ __forceinline__ int tree_chunks_of(const TreeParams& p, int len) {
   return (len - tree_lo(p, len) + p.chunk - 1) / p.chunk + p.tree_chunks;
 }
@@ -105,8 +108,10 @@ struct TreeCursor {
     item = (int)(in / n);
     c = (int)(in - (int64_t)item * n);
   }
-  __device__ __forceinline__ void next(const TreeParams& p) {
-    if (++c < n) return;
+  // On by k chunks of the same item (k >= 1; past its end: to the next item).
+  __device__ __forceinline__ void next(const TreeParams& p, int k = 1) {
+    c += k;
+    if (c < n) return;
     c = 0;
     if (++item < p.Hkv * p.n_rb) return;
     item = 0;
@@ -241,5 +246,11 @@ constexpr int kTreeSimtRows = 32, kTreeSimtChunk = 32;
 // tree_mma.cu: bf16 / fp16 on mma.sync.
 TreeTile tree_mma_tile(int64_t rows, int D);
 int tree_mma(const TreeParams& p, int dtype, cudaStream_t st);
+
+// tree_sm100.cu: bf16 / fp16 on tcgen05, pages by TMA.
+TreeTile tree_sm100_tile(int64_t rows, int D);
+// Whether its layouts allow it (the sizes are the caller's rule).
+bool tree_sm100_layout(const bfa_tree_args* a);
+int tree_sm100(const TreeParams& p, int dtype, cudaStream_t st);
 
 }  // namespace bfa

@@ -463,6 +463,7 @@ __global__ void __launch_bounds__(32 * RW * KW, (Tile<D, RW, KW>::kPerSm)) tree_
     const bool whole = seg_c0 == 0 && last;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
+      if (anc[h] == 0) l[h] = 0.f;  // an absent node: chunks that are not masked were summed for it too
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
     }

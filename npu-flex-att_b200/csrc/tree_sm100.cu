@@ -1,0 +1,655 @@
+// tree_sm100.cu -- attention of a tree of drafted tokens over a paged cache in
+// bf16 / fp16 on tcgen05, K/V pages by TMA.
+//
+// Mathematics: the online softmax of the other forwards (base 2; P rounded to
+// the input type and kept in TMEM as the A operand of P·V; O rescaled only when
+// a row's maximum grows by more than 2^8). The rows r = g·N + n of one KV head
+// are stacked into tiles of 128, so its K/V cross HBM once per block of rows.
+//
+// Bound: HBM (K/V read once) up to about 256 rows per KV head, the tensor cores
+// above; mma.sync falls behind HBM from about 64 rows.
+//
+// Split. Persistent blocks, one per SM, each with an equal stretch of the list
+// of chunks (tree_common.cuh). Warp roles:
+//   warp 0      producer: looks the chunk's pages up (a lane per box) and loads
+//               K and V by TMA into a ring that runs on across items
+//   warp 1      MMA issuer
+//   warp 2      TMEM allocator
+//   warps 4..   softmax, a thread per row (TMEM lane): 4 warps per 128-row tile
+// With two tiles (NT = 2) one tile's softmax runs under the other's products:
+// S_0(j), S_1(j), then PV_0(j), S_0(j+1), PV_1(j), S_1(j+1). With one tile S is
+// double-buffered: S(j+1) is formed before PV(j).
+//
+// A box is gcd(page_size, chunk) tokens of one page, so any page size that is a
+// multiple of 8 works (8 rows of 128 bytes are the swizzle's atom). Tokens past
+// a sequence's end, and nodes past N, arrive as whatever the page holds: their
+// logits are masked, and in such chunks the softmax warps clear those rows of
+// V before the product may read them.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <climits>
+#include <numeric>
+
+#include "sm100_host.h"
+#include "sm100_ptx.cuh"
+#include "tree_common.cuh"
+
+namespace bfa {
+namespace {
+
+using namespace sm100;
+
+constexpr int kBM = 128;
+constexpr float kRescaleThreshold = 8.0f;
+
+// CH keys per chunk: 128, or 64 at D = 256 (64 KB of K and V either way).
+template <int D, int NT>
+struct TreeLayout {
+  static constexpr int kCH = D == 256 ? 64 : 128;
+  static constexpr int kSub = D / 64;
+  static constexpr uint32_t kQTile = kBM * D * 2;
+  static constexpr uint32_t kKV = kCH * D * 2;
+  static constexpr uint32_t kMisc = 2048;
+  static constexpr int kFit = (int)((232448u - 1024u - kMisc - NT * kQTile) / kKV);
+  static constexpr int kStages = kFit < 8 ? kFit : 8;
+  static constexpr uint32_t kOffKV = NT * kQTile;
+  static constexpr uint32_t kOffMisc = kOffKV + kStages * kKV;
+  static constexpr uint32_t kBytes = kOffMisc + kMisc + 1024;  // 1024: alignment of the tiles
+  static constexpr uint32_t kTmemO = 2 * kCH;
+  static constexpr int kThreads = 128 + 128 * NT;
+  static_assert(kStages >= 4, "K and V of two chunks");
+  static_assert(kTmemO + NT * D <= 512, "TMEM");
+  static_assert(kBytes <= 232448, "shared memory");
+};
+
+struct TreeMisc {
+  uint64_t bar[40];
+  uint32_t tmem;
+  int abort;
+  unsigned long long bad[2][2];  // by the chunk's parity: its keys whose values are not finite
+  TreeMasks masks;
+};
+static_assert(sizeof(TreeMisc) <= 2048, "misc");
+
+// One column (32 bits per lane) of TMEM.
+__device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr) {
+  uint32_t r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
+  return r;
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  return BF16 ? pack_bf16(a, b) : pack_f16(a, b);
+}
+template <bool BF16>
+__device__ __forceinline__ float half_of(uint32_t w, int hi) {
+  const uint32_t h = hi ? w >> 16 : w & 0xffffu;
+  return BF16 ? __uint_as_float(h << 16) : __half2float(__ushort_as_half((unsigned short)h));
+}
+template <bool BF16>
+__device__ __forceinline__ bool any_not_finite(uint32_t w) {
+  constexpr uint32_t e = BF16 ? 0x7f80u : 0x7c00u;
+  return (w & e) == e || ((w >> 16) & e) == e;
+}
+
+template <int D, int NT, bool BF16, bool PLAIN>
+__global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
+    tree_kernel(const __grid_constant__ CUtensorMap tmKp, const __grid_constant__ CUtensorMap tmVp,
+                const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeParams p, int box,
+                uint64_t timeout_ns) {
+  using L = TreeLayout<D, NT>;
+  constexpr int CH = L::kCH, NS = L::kStages;
+  enum {
+    kQFull = 0,
+    kKVFull = 1,
+    kKVEmpty = kKVFull + NS,
+    kSFull = kKVEmpty + NS,  // NT = 2: S_t formed; NT = 1: the S buffer of that parity
+    kPHalf = kSFull + 2,     // P of the first half of the keys (and a final O) in TMEM
+    kPFull = kPHalf + NT,
+    kODone = kPFull + NT,
+    kDrain = kODone + NT,
+    kNumBars = kDrain + 1
+  };
+  static_assert(kNumBars <= 40, "barriers");
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
+  const uint32_t sbase = smem_u32(smem);
+  TreeMisc& mi = *reinterpret_cast<TreeMisc*>(smem + L::kOffMisc);
+  auto bar = [&](int i) -> uint32_t { return sbase + L::kOffMisc + 8u * (uint32_t)i; };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  const int64_t T_all = tree_chunks_before(p, p.B);
+  const int blocks = tree_blocks(p, T_all);
+  if ((int)blockIdx.x >= blocks) return;
+  const int64_t x0 = tree_start(T_all, blocks, blockIdx.x);
+  const int n_x = (int)(tree_start(T_all, blocks, blockIdx.x + 1) - x0);
+  TreeCursor cur;
+  cur.seek(p, x0);
+
+  WaitCtl ctl{(volatile int*)&mi.abort, p.status, timeout_ns};
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kNumBars; ++i)
+      mbar_init(bar(i), i == kQFull ? 4u * NT : (i >= kPHalf && i < kODone) ? 4u : 1u);
+    mi.abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == 2) {
+    tmem_alloc(smem_u32(&mi.tmem), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = mi.tmem;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      tma_prefetch_desc(&tmKp);
+      tma_prefetch_desc(&tmVp);
+      tma_prefetch_desc(&tmK);
+      tma_prefetch_desc(&tmV);
+    }
+    bool ok = true;
+    int n = 0;
+    for (int x = 0; x < n_x && ok; ++x) {
+      const bool tree = cur.in_tree(p);
+      const int key0 = cur.key0(p), hkv = cur.item / p.n_rb;
+      // Lane i: box i of the chunk, tokens [key0 + i·box, + box) of one page.
+      const int t0 = key0 + lane * box;
+      const bool mine = tree ? lane == 0 : (lane < CH / box && t0 < cur.len);
+      int page = 0, slot = 0;
+      if (mine && !tree) {
+        const int pg = t0 / p.page;
+        slot = t0 - pg * p.page;
+        page = p.table[cur.b * p.table_stride + pg];
+        if (page < 0 || page >= p.num_pages) {
+          page = (int)p.num_pages;  // outside the tensor: reads as zeros
+          if (p.status) *p.status = BFA_ERR_INDEX;
+        }
+      }
+      const uint32_t bytes = tree ? 64u * 128u * L::kSub : (uint32_t)__popc(__ballot_sync(0xffffffffu, mine)) * box * 128u * L::kSub;
+      for (int kv = 0; kv < 2; ++kv, ++n) {
+        const int st = n % NS;
+        if (n >= NS) {
+          int w = 1;
+          if (lane == 0) w = mbar_wait(bar(kKVEmpty + st), ((n / NS) & 1) ^ 1, ctl, BFA_ERR_DEVICE_TIMEOUT) ? 1 : 0;
+          ok = __shfl_sync(0xffffffffu, w, 0) != 0;
+          if (!ok) break;
+        }
+        if (lane == 0) mbar_arrive_expect_tx(bar(kKVFull + st), bytes);
+        __syncwarp();
+        if (mine) {
+          const uint32_t dst = sbase + L::kOffKV + st * L::kKV;
+          for (int s = 0; s < L::kSub; ++s) {
+            if (tree) tma_load_4d(dst + s * (CH * 128), kv ? &tmV : &tmK, bar(kKVFull + st), s * 64, 0, hkv, cur.b);
+            else
+              tma_load_4d(dst + s * (CH * 128) + lane * box * 128, kv ? &tmVp : &tmKp, bar(kKVFull + st), s * 64, slot, hkv, page);
+          }
+        }
+        __syncwarp();
+      }
+      cur.next(p);
+    }
+    if (lane == 0)
+      for (int i = (n > NS ? n - NS : 0); i < n; ++i) drain_wait(bar(kKVFull + i % NS), (i / NS) & 1, timeout_ns);
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t idS = idesc_f16(kBM, CH, BF16, false);
+      constexpr uint32_t idO = idesc_f16(kBM, D, BF16, true);
+      auto kv_addr = [&](int idx) -> uint32_t { return sbase + L::kOffKV + (uint32_t)(idx % NS) * L::kKV; };
+      auto issue_s = [&](int t, int buf, int idx) {
+        const uint64_t dq = desc_kmajor(sbase + t * L::kQTile);
+        const uint64_t dk = desc_kmajor(kv_addr(idx));
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t offq = (kk >> 2) * (kBM * 128) + (kk & 3) * 32;
+          const uint32_t offk = (kk >> 2) * (CH * 128) + (kk & 3) * 32;
+          mma_ss(tmem + buf * CH, dq + (offq >> 4), dk + (offk >> 4), idS, kk > 0 ? 1u : 0u);
+        }
+        mma_commit(bar(kSFull + buf));
+      };
+      // P·V in two halves of the keys; O is zeroed by the softmax warps at an
+      // item's start, so every product accumulates.
+      auto issue_pv = [&](int t, int buf, int idx, int half) {
+        const uint64_t dv = desc_mnmajor(kv_addr(idx), CH * 128);
+#pragma unroll
+        for (int k4 = 0; k4 < CH / 32; ++k4) {
+          const int kk = half * (CH / 32) + k4;
+          mma_ts(tmem + L::kTmemO + t * D, tmem + buf * CH + kk * 8, dv + ((kk * 16 * 128) >> 4), idO, 1u);
+        }
+        if (half == 1) mma_commit(bar(kODone + t));
+      };
+      auto wait = [&](int i, int parity) {
+        if (!mbar_wait(bar(i), (uint32_t)parity, ctl, BFA_ERR_DEVICE_TIMEOUT)) return false;
+        tc_fence_after();
+        return true;
+      };
+      auto wait_load = [&](int idx) { return wait(kKVFull + idx % NS, (idx / NS) & 1); };
+      auto pv = [&](int t, int buf, int x) {
+        if (!wait(kPHalf + t, x & 1)) return false;
+        issue_pv(t, buf, 2 * x + 1, 0);
+        if (!wait(kPFull + t, x & 1)) return false;
+        issue_pv(t, buf, 2 * x + 1, 1);
+        return true;
+      };
+      bool ok = true;
+      int seg = 0;
+      for (int x = 0; x < n_x && ok; ++seg) {
+        const int count = min(cur.n - cur.c, n_x - x);  // chunks of this segment
+        const int end = x + count;
+        ok = wait(kQFull, seg & 1) && wait_load(2 * x);
+        if (!ok) break;
+        if constexpr (NT == 2) {
+          issue_s(0, 0, 2 * x);
+          issue_s(1, 1, 2 * x);
+          mma_commit(bar(kKVEmpty + (2 * x) % NS));
+        } else {
+          issue_s(0, x & 1, 2 * x);
+          mma_commit(bar(kKVEmpty + (2 * x) % NS));
+        }
+        for (; x < end; ++x) {
+          const int iv = 2 * x + 1, ik = 2 * x + 2;
+          const bool more = x + 1 < end;
+          if constexpr (NT == 2) {
+            if (!(ok = wait_load(iv) && pv(0, 0, x))) break;
+            if (more) {
+              if (!(ok = wait_load(ik))) break;
+              issue_s(0, 0, ik);
+            }
+            if (!(ok = pv(1, 1, x))) break;
+            mma_commit(bar(kKVEmpty + iv % NS));
+            if (more) {
+              issue_s(1, 1, ik);
+              mma_commit(bar(kKVEmpty + ik % NS));
+            }
+          } else {
+            if (more) {
+              if (!(ok = wait_load(ik))) break;
+              issue_s(0, (x + 1) & 1, ik);
+              mma_commit(bar(kKVEmpty + ik % NS));
+            }
+            if (!(ok = wait_load(iv) && pv(0, x & 1, x))) break;
+            mma_commit(bar(kKVEmpty + iv % NS));
+          }
+        }
+        cur.next(p, count);
+      }
+      mma_commit(bar(kDrain));
+      drain_wait(bar(kDrain), 0, timeout_ns);
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ softmax
+    const int t = (warp - 4) >> 2, wq = warp & 3;
+    const int row = t * kBM + wq * 32 + lane;  // of the row block
+    const int sid = threadIdx.x - 128;         // among the softmax threads
+    constexpr int kSoft = 128 * NT;
+    const uint32_t lane_base = (uint32_t)(wq * 32) << 16;
+    const uint32_t tO = tmem + lane_base + L::kTmemO + t * D;
+    const float sl2 = p.scale * kLog2e;
+    const bool cap = !PLAIN && p.soft_cap > 0.f;
+    const float cap_in = cap ? p.scale / p.soft_cap : 0.f, cap_out = cap ? p.soft_cap * kLog2e : 0.f;
+    bool ok = true;  // false: this block gave up on a wait; the flow goes on without waiting
+    int x = 0;
+    while (x < n_x) {
+      // ---------------------------------------------------- an item begins
+      // (`cur` stands at its first chunk of this block's; little else is kept
+      // over the loop, whose S row fills the registers: what only the masked
+      // chunks and the end need is formed again there.)
+      const int count = min(cur.n - cur.c, n_x - x);
+      const int rows = p.G * p.N - (cur.item % p.n_rb) * (NT * kBM);
+      const bool live_row = row < rows;  // rows past them are zeros, worked on like the others and not stored
+      auto where = [&](int* hq, int* node) {  // the row's head and node
+        int item = cur.item;  // opaque: each use forms its values anew, none stay in registers between
+        asm volatile("" : "+r"(item));
+        *hq = item / p.n_rb * p.G;
+        *node = 0;
+        if (live_row) tree_row(p, item / p.n_rb, (item % p.n_rb) * (NT * kBM) + row, hq, node);
+      };
+      {
+        // q's row into the swizzled tile (its readers, the last item's S
+        // products, are done: their barrier was waited for).
+        int hq, node;
+        where(&hq, &node);
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + cur.b * p.sq[0] + hq * p.sq[1] + node * p.sq[2]);
+        uint8_t* dst = smem + t * L::kQTile;
+#pragma unroll 4
+        for (int c = 0; c < D / 8; ++c) {
+          uint4 w = make_uint4(0u, 0u, 0u, 0u);
+          if (live_row && c * 8 < p.D) w = src[c];
+          *reinterpret_cast<uint4*>(dst + (c >> 3) * (kBM * 128) + sw128_offset(wq * 32 + lane, c & 7)) = w;
+        }
+        fence_async_shared();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kQFull));
+      {
+        uint32_t z[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) z[i] = 0u;
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) tmem_st16(tO + 16 * c, z);
+        tmem_st_wait();
+      }
+      named_sync(1, kSoft);  // the last item's masks are no longer read
+      if (warp == 4) tree_masks(p, cur.b, mi.masks);
+      if (sid == 0 && p.status && p.lens[cur.b] != cur.len) *p.status = BFA_ERR_INDEX;
+      named_sync(1, kSoft);
+      const int all_from = p.window > 0 ? cur.len + p.N - 1 - p.window : 0;
+      float m = neg_inf(), l = 0.f;
+
+      for (int it = 0; it < count; ++it, ++x) {
+        const int c = cur.c + it;
+        const bool tree = c >= cur.n - p.tree_chunks;
+        const int key0 = tree ? 0 : cur.lo + c * CH;
+        const int valid = tree ? p.N : min(CH, cur.len - key0);  // rows of the chunk that hold keys
+        const bool masked = tree || valid < CH || key0 < all_from;
+        const int buf = NT == 2 ? t : x & 1;
+        const uint32_t tS = tmem + lane_base + buf * CH;
+        ok = ok && warp_wait(bar(kSFull + buf), (uint32_t)(NT == 2 ? x & 1 : (x >> 1) & 1), ctl);
+        tc_fence_after();
+
+        // V rows that no key holds are cleared; where rows differ in what they
+        // see, values that are not finite are looked for (0·inf must not
+        // reach a row that does not see the key).
+        bool hold = false;
+        if (masked) {
+          ok = ok && warp_wait(bar(kKVFull + (2 * x + 1) % NS), (uint32_t)(((2 * x + 1) / NS) & 1), ctl);
+          uint8_t* vt = smem + L::kOffKV + ((2 * x + 1) % NS) * L::kKV;
+          const bool differ = tree || key0 < all_from;
+          unsigned long long* bad = mi.bad[x & 1];  // the other one may still be read by a slower warp
+          if (sid < 2) bad[sid] = 0ull;
+          named_sync(1, kSoft);
+          // Piece i: 16 bytes of row i % CH of a 64-column sub-tile.
+          for (int i = sid; i < CH * (D / 8); i += kSoft) {
+            const int r = (i >> 3) % CH, sub = (i >> 3) / CH;
+            uint4* at = reinterpret_cast<uint4*>(vt + sub * (CH * 128) + r * 128 + (i & 7) * 16);
+            if (r >= valid) {
+              *at = make_uint4(0u, 0u, 0u, 0u);
+            } else if (differ) {
+              const uint4 w = *at;
+              if (any_not_finite<BF16>(w.x) || any_not_finite<BF16>(w.y) || any_not_finite<BF16>(w.z) || any_not_finite<BF16>(w.w))
+                atomicOr(&bad[r >> 6], 1ull << (r & 63));
+            }
+          }
+          fence_async_shared();
+          named_sync(1, kSoft);
+          hold = (bad[0] | bad[1]) != 0;
+        }
+
+        float alpha = 1.f;
+        bool rescale = false;
+        uint32_t r[CH / 32][32];
+        float m_use = 0.f;
+        const bool formed = !PLAIN || masked || !(sl2 > 0.f);  // logits in r, else raw products
+        {
+          float mx = neg_inf();
+          if (formed) {
+            // Logits in base 2, masked, formed 32 columns at a time in place in
+            // TMEM: the rarer chunks stay out of the registers and the code of
+            // the plain ones. Kept columns: [lo, hi) of cached tokens, or the
+            // seen nodes.
+            int hq, node;
+            where(&hq, &node);
+            const int depth = mi.masks.depth[node], pos = cur.len + depth;
+            uint64_t seen = live_row ? mi.masks.anc[node] : 0ull;
+            const int lo = p.window > 0 ? max(0, pos - p.window - key0) : 0;
+            const int hi = seen ? valid : 0;
+            if (tree && p.window > 0 && p.window < p.N)
+              for (int i = 0; i < p.N; ++i)
+                if (depth - mi.masks.depth[i] > p.window) seen &= ~(1ull << i);
+            float slope2 = 0.f;
+            int ref = 0;
+            if (!PLAIN && p.alibi) {
+              slope2 = p.alibi[hq] * kLog2e;
+              ref = tree_alibi_ref(p, slope2, pos);
+            }
+#pragma unroll 1
+            for (int ch = 0; ch < CH / 32; ++ch) {
+              uint32_t u[32];
+              tmem_ld32(tS + 32 * ch, u);
+              tmem_ld_wait();
+              uint32_t keep = 0;  // bit e: column 32·ch + e
+              if (tree) {
+                keep = ch < 2 ? (uint32_t)(seen >> (32 * ch)) : 0u;
+              } else {
+                const int from = min(max(lo - 32 * ch, 0), 32), to = min(max(hi - 32 * ch, 0), 32);
+                if (to > from) keep = (0xffffffffu >> (32 - (to - from))) << from;
+              }
+              const float abase = slope2 * (float)(ref - key0 - 32 * ch);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                float y = __uint_as_float(u[e]);
+                if (PLAIN) {
+                  y *= sl2;
+                } else {
+                  y = cap ? cap_out * tanh_any(y * cap_in) : y * sl2;
+                  if (p.alibi) {
+                    if (tree) y += slope2 * (float)(ref - cur.len - mi.masks.depth[(32 * ch + e) & (kTreeNodes - 1)]);
+                    else y += fmaf(-slope2, (float)e, abase);
+                  }
+                }
+                y = (keep >> e) & 1u ? y : neg_inf();
+                mx = fmaxf(mx, y);
+                u[e] = __float_as_uint(y);
+              }
+              tmem_st32(tS + 32 * ch, u);
+            }
+            tmem_st_wait();
+          }
+#pragma unroll
+          for (int ch = 0; ch < CH / 32; ++ch) tmem_ld32(tS + 32 * ch, r[ch]);
+          tmem_ld_wait();
+          if (!formed) {
+            float m4[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
+#pragma unroll
+            for (int ch = 0; ch < CH / 32; ++ch)
+#pragma unroll
+              for (int e = 0; e < 32; e += 2)
+                m4[(e >> 1) & 3] = fmax3(m4[(e >> 1) & 3], __uint_as_float(r[ch][e]), __uint_as_float(r[ch][e + 1]));
+            mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sl2;
+          }
+          const bool grow = (mx > m + kRescaleThreshold) || (m == neg_inf() && mx != neg_inf());
+          float m_new = m;
+          if (__any_sync(0xffffffffu, grow)) {
+            m_new = fmaxf(m, mx);
+            rescale = it > 0;
+          }
+          m_use = m_new == neg_inf() ? 0.f : m_new;
+          alpha = ex2(m - m_use);
+          m = m_new;
+        }
+        // O stands still: the last P·V is done.
+        if (it > 0) {
+          ok = ok && warp_wait(bar(kODone + t), (uint32_t)((x - 1) & 1), ctl);
+          tc_fence_after();
+        }
+        {
+          if (rescale) {
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o16[16];
+              tmem_ld16(tO + 16 * c, o16);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o16[i] = __float_as_uint(__uint_as_float(o16[i]) * alpha);
+              tmem_st16(tO + 16 * c, o16);
+            }
+          }
+          float2 s2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          const float2 xs2 = make_float2(formed ? 1.f : sl2, formed ? 1.f : sl2), nm2 = make_float2(-m_use, -m_use);
+#pragma unroll
+          for (int ch = 0; ch < CH / 32; ++ch) {
+            if (ch == CH / 64 && !hold) {  // the first half of P is stored
+              tmem_st_wait();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(bar(kPHalf + t));
+            }
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float2 y = __ffma2_rn(make_float2(__uint_as_float(r[ch][e]), __uint_as_float(r[ch][e + 1])), xs2, nm2);
+              const float p0 = ex2(y.x), p1 = ex2(y.y);
+              s2[(e >> 1) & 1] = __fadd2_rn(s2[(e >> 1) & 1], make_float2(p0, p1));
+              pk[e / 2] = pack2<BF16>(p0, p1);
+            }
+            tmem_st16(tS + 16 * ch, pk);
+          }
+          l = l * alpha + ((s2[0].x + s2[0].y) + (s2[1].x + s2[1].y));
+          tmem_st_wait();
+        }
+        if (hold) {
+          // Values that are not finite: O += p·v by hand for the rows that see
+          // them, then the rows of V are cleared for the product.
+          uint8_t* vt = smem + L::kOffKV + ((2 * x + 1) % NS) * L::kKV;
+          {
+#pragma unroll 1
+            for (int n = 0; n < valid; ++n) {
+              if (!((mi.bad[x & 1][n >> 6] >> (n & 63)) & 1)) continue;
+              const uint32_t w = tmem_ld1(tS + (n >> 1));
+              tmem_ld_wait();
+              const float pr = half_of<BF16>(w, n & 1);
+#pragma unroll 1
+              for (int c = 0; c < D / 16; ++c) {
+                uint32_t o16[16];
+                tmem_ld16(tO + 16 * c, o16);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  const uint4 v = *reinterpret_cast<const uint4*>(vt + (c >> 2) * (CH * 128) + sw128_offset(n, (c & 3) * 2 + i));
+                  const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                  for (int e = 0; e < 8; ++e)
+                    if (pr != 0.f)
+                      o16[8 * i + e] = __float_as_uint(__uint_as_float(o16[8 * i + e]) + pr * half_of<BF16>(vw[e >> 1], e & 1));
+                }
+                tmem_st16(tO + 16 * c, o16);
+                tmem_st_wait();
+              }
+            }
+          }
+          named_sync(1, kSoft);
+          for (int i = sid; i < CH * (D / 8); i += kSoft) {
+            const int rr = (i >> 3) % CH, sub = (i >> 3) / CH;
+            if ((mi.bad[x & 1][rr >> 6] >> (rr & 63)) & 1)
+              *reinterpret_cast<uint4*>(vt + sub * (CH * 128) + rr * 128 + (i & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_async_shared();
+          named_sync(1, kSoft);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (hold) mbar_arrive(bar(kPHalf + t));
+          mbar_arrive(bar(kPFull + t));
+        }
+      }
+
+      // ------------------------------------------------------ the item ends
+      ok = ok && warp_wait(bar(kODone + t), (uint32_t)((x - 1) & 1), ctl);
+      tc_fence_after();
+      if (ok) {
+        const bool whole = cur.c == 0 && count == cur.n;
+        int hq, node;
+        where(&hq, &node);
+        if (mi.masks.anc[node] == 0) l = 0.f;  // absent: chunks that are not masked were summed for it too
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        const int64_t prow = ((int64_t)blockIdx.x * 2 + (cur.c > 0 ? 0 : 1)) * p.rb + row;
+        uint16_t* og = static_cast<uint16_t*>(p.o) + cur.b * p.so[0] + hq * p.so[1] + node * p.so[2];
+        float* pg = p.part_o + prow * p.D;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t r[32];
+          tmem_ld32(tO + 32 * c, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int d = 32 * c + 8 * q;
+            if (!live_row || d >= p.D) continue;
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = inv > 0.f ? __uint_as_float(r[8 * q + e]) * inv : 0.f;
+            if (whole) {
+              *reinterpret_cast<uint4*>(og + d) =
+                  make_uint4(pack2<BF16>(f[0], f[1]), pack2<BF16>(f[2], f[3]), pack2<BF16>(f[4], f[5]), pack2<BF16>(f[6], f[7]));
+            } else {
+              *reinterpret_cast<float4*>(pg + d) = make_float4(f[0], f[1], f[2], f[3]);
+              *reinterpret_cast<float4*>(pg + d + 4) = make_float4(f[4], f[5], f[6], f[7]);
+            }
+          }
+          __syncwarp();
+        }
+        if (live_row) {
+          const float l2 = l > 0.f ? m + lg2(l) : neg_inf();
+          if (!whole) p.part_lse[prow] = l2;
+          else if (p.lse)
+            p.lse[((int64_t)cur.b * p.Hq + hq) * p.N + node] =
+                l2 == neg_inf() ? l2 : l2 * kLn2 + tree_row_shift(p, hq, cur.len + mi.masks.depth[node]);
+        }
+      }
+      cur.next(p, count);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+constexpr uint64_t kTimeoutNs = 1000000000ull;
+
+template <int D, int NT, bool BF16>
+int launch(const TreeParams& p, int dtype, cudaStream_t st) {
+  using L = TreeLayout<D, NT>;
+  const int box = std::gcd(p.page, L::kCH);
+  CUtensorMap tm[4];
+  if (!make_tmap_bhsd(&tm[0], p.kp, dtype, p.D, p.page, p.Hkv, (int)p.num_pages, p.skp, box) ||
+      !make_tmap_bhsd(&tm[1], p.vp, dtype, p.D, p.page, p.Hkv, (int)p.num_pages, p.svp, box) ||
+      !make_tmap_bhsd(&tm[2], p.k, dtype, p.D, p.N, p.Hkv, p.B, p.sk, 64) ||
+      !make_tmap_bhsd(&tm[3], p.v, dtype, p.D, p.N, p.Hkv, p.B, p.sv, 64))
+    return BFA_ERR_CUDA;
+  const bool plain = p.soft_cap == 0.f && !p.alibi;
+  auto kernel = plain ? tree_kernel<D, NT, BF16, true> : tree_kernel<D, NT, BF16, false>;
+  static std::atomic<uint64_t> done[2];
+  const int rc = allow_shared(kernel, (int)L::kBytes, done[plain], "tree attention shared memory");
+  if (rc) return rc;
+  kernel<<<p.grid, L::kThreads, L::kBytes, st>>>(tm[0], tm[1], tm[2], tm[3], p, box, kTimeoutNs);
+  note_launch();
+  return launch_status("tree attention launch");
+}
+
+template <bool BF16>
+int launch_d(const TreeParams& p, int dtype, cudaStream_t st) {
+  const bool two = p.rb == 2 * kBM;
+  if (p.D <= 64) return two ? launch<64, 2, BF16>(p, dtype, st) : launch<64, 1, BF16>(p, dtype, st);
+  if (p.D <= 128) return two ? launch<128, 2, BF16>(p, dtype, st) : launch<128, 1, BF16>(p, dtype, st);
+  return launch<256, 1, BF16>(p, dtype, st);
+}
+
+}  // namespace
+
+TreeTile tree_sm100_tile(int64_t rows, int D) {
+  return {rows > kBM && D <= 128 ? 2 * kBM : kBM, D > 128 ? 64 : 128, 1};
+}
+
+bool tree_sm100_layout(const bfa_tree_args* a) {
+  return device_is_sm100() && a->head_dim % 8 == 0 && a->page_size % 8 == 0 && a->num_pages > 0 && a->num_pages < INT32_MAX &&
+         a->max_pages > 0 && vector_rows(a->q, 2) && vector_rows(a->o, 2) && tma_layout_ok(a->k.data, a->k.stride, 2) &&
+         tma_layout_ok(a->v.data, a->v.stride, 2) && tma_layout_ok(a->k_pages.data, a->k_pages.stride, 2) &&
+         tma_layout_ok(a->v_pages.data, a->v_pages.stride, 2);
+}
+
+int tree_sm100(const TreeParams& p, int dtype, cudaStream_t st) {
+  return dtype == BFA_DTYPE_BF16 ? launch_d<true>(p, dtype, st) : launch_d<false>(p, dtype, st);
+}
+
+}  // namespace bfa

@@ -17,6 +17,19 @@ import tree_decoding as td
 from tree_reference import attention, dense, page_cache, verify
 
 DEV = "cuda:0"
+
+
+@pytest.fixture(params=["", "0", "1"], ids=["rule", "mma", "tcgen05"], autouse=True)
+def kernel(request, monkeypatch):
+    """Attention tests run by the library's own choice of kernel and on either
+    16-bit kernel at every size that its layouts allow."""
+    name = request.node.name
+    if request.param and ("verify" in name or "append" in name or "refusals" in name):
+        pytest.skip("one kernel")
+    if request.param:
+        monkeypatch.setenv("BFA_TREE_TCGEN05", request.param)
+
+
 U = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
 
 
@@ -100,6 +113,8 @@ def test_absent_nodes_give_empty_rows(dtype, N):
     ref = attention(q, k, v, cache, parents)
     gone = ref[1] == -math.inf
     assert gone[0, 0, 3] and gone[0, 0, 7] and gone[1, 0, 1:].all()
+    up = torch.tensor(parents, dtype=torch.int32, device=DEV)
+    compare(*td.tree_attention(q, k, v, cache, up, return_lse=True), *ref)
     for t in (k, v):
         t.masked_fill_(gone[:, :1, :, None], float("nan"))
     q.masked_fill_(gone[:, :, :, None], float("inf"))
