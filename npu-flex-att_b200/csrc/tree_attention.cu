@@ -11,106 +11,119 @@
 namespace bfa {
 namespace {
 
+// Rows of an item per merge block: one where four warps share a row (few
+// items: all their rows at once), else 16.
+constexpr int merge_rows(int warps) { return warps == 4 ? 1 : 16; }
+
 // Joins the partial (O, LSE) of items that several blocks worked on, partials
 // in the order of their keys:
 //   lse = log2 sum_i 2^lse_i,  O = sum_i O_i·2^(lse_i - lse).
-// Rows of an item that one block did whole are already final. kWarps warps
-// take a row: each sums every kWarps-th partial, eight loads in flight, and
-// the first adds the warps' sums in order. One warp where an item has few
-// partials (many items), four where a few items are spread over the GPU.
-// kVec: columns per lane and load (4 where D allows it, else 1).
+// An item that one block did whole is already final, and its merge blocks
+// leave at once. kWarps warps take a row: each sums every kWarps-th partial,
+// eight loads in flight, and the first adds the warps' sums in order. One warp
+// where an item has few partials (many items), four where a few items are
+// spread over the GPU. kVec: columns per lane and load (4 where D allows it,
+// else 1). Launched to start under the attention kernel's tail: what it needs
+// of the inputs alone comes before it waits for the partials.
 template <typename T, int kWarps, int kVec>
 __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeParams p) {
-  constexpr int kRowsPer = 4 / kWarps;
+  constexpr int kMergeRows = merge_rows(kWarps);
   constexpr int kLoads = kVec == 4 ? 2 : 8;  // of 32·kVec columns: 256
   __shared__ float part[4][kVec * kLoads * 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % kWarps;
-  const int64_t row = (int64_t)blockIdx.x * kRowsPer + warp / kWarps;
   const int GN = p.G * p.N;
-  if (row >= (int64_t)p.B * p.Hkv * GN) return;  // whole blocks where kWarps is 4
-  const int r_all = (int)(row % GN), hkv = (int)(row / GN % p.Hkv), b = (int)(row / GN / p.Hkv);
-  const int rbk = r_all / p.rb, r = r_all - rbk * p.rb;
-  const int64_t T_all = tree_chunks_before(p, p.B);
+  const int per_item = (min(p.rb, GN) + kMergeRows - 1) / kMergeRows;
+  const int item_all = blockIdx.x / per_item, row0 = (blockIdx.x - item_all * per_item) * kMergeRows;
+  const int b = item_all / (p.Hkv * p.n_rb), item = item_all - b * p.Hkv * p.n_rb;
+  const int hkv = item / p.n_rb, rb0 = (item - hkv * p.n_rb) * p.rb;
+  int64_t s0;
+  const int64_t total_chunks = tree_total(p, b, &s0);
   const int len = tree_len(p, b), n_chunks = tree_chunks_of(p, len);
-  const int64_t s0 = tree_chunks_before(p, b) + (int64_t)(hkv * p.n_rb + rbk) * n_chunks;
-  const int blocks = tree_blocks(p, T_all);
-  const int i0 = tree_owner(T_all, blocks, s0), i1 = tree_owner(T_all, blocks, s0 + n_chunks - 1);
+  s0 += (int64_t)item * n_chunks;
+  const int blocks = tree_blocks(p, total_chunks);
+  const int i0 = tree_owner(total_chunks, blocks, s0), i1 = tree_owner(total_chunks, blocks, s0 + n_chunks - 1);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (i0 == i1) return;
-  auto slot = [&](int i) { return ((int64_t)i * 2 + (i == i0 ? 1 : 0)) * p.rb + r; };
-  float m = neg_inf();
-  for (int i = i0 + lane; i <= i1; i += 32) m = fmaxf(m, p.part_lse[slot(i)]);
+  for (int rr = warp / kWarps; rr < kMergeRows; rr += 4 / kWarps) {
+    const int r = row0 + rr;
+    if (r >= p.rb || rb0 + r >= GN) break;  // alike for the warps of a row
+    auto slot = [&](int i) { return ((int64_t)i * 2 + (i == i0 ? 1 : 0)) * p.rb + r; };
+    float m = neg_inf();
+    for (int i = i0 + lane; i <= i1; i += 32) m = fmaxf(m, p.part_lse[slot(i)]);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  float total = 0.f, acc[kLoads][kVec];
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float total = 0.f, acc[kLoads][kVec];
 #pragma unroll
-  for (int c = 0; c < kLoads; ++c)
+    for (int c = 0; c < kLoads; ++c)
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) acc[c][e] = 0.f;
-  if (m != neg_inf()) {
-    for (int j0 = i0; j0 <= i1; j0 += 32) {
-      const float w = j0 + lane <= i1 ? exp2f(p.part_lse[slot(j0 + lane)] - m) : 0.f;
-      float sum = w;
+      for (int e = 0; e < kVec; ++e) acc[c][e] = 0.f;
+    if (m != neg_inf()) {
+      for (int j0 = i0; j0 <= i1; j0 += 32) {
+        const float w = j0 + lane <= i1 ? exp2f(p.part_lse[slot(j0 + lane)] - m) : 0.f;
+        float sum = w;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      total += sum;
-      const int n = min(32, i1 - j0 + 1);
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        total += sum;
+        const int n = min(32, i1 - j0 + 1);
 #pragma unroll 8
-      for (int j = sub; j < n; j += kWarps) {
-        const float wj = __shfl_sync(0xffffffffu, w, j);
-        const float* po = p.part_o + slot(j0 + j) * p.D;
+        for (int j = sub; j < n; j += kWarps) {
+          const float wj = __shfl_sync(0xffffffffu, w, j);
+          const float* po = p.part_o + slot(j0 + j) * p.D;
 #pragma unroll
-        for (int c = 0; c < kLoads; ++c) {
-          const int d = (lane + 32 * c) * kVec;
-          if (d >= p.D) continue;
-          float f[kVec];
-          if constexpr (kVec == 4) *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(po + d);
-          else f[0] = po[d];
+          for (int c = 0; c < kLoads; ++c) {
+            const int d = (lane + 32 * c) * kVec;
+            if (d >= p.D) continue;
+            float f[kVec];
+            if constexpr (kVec == 4) *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(po + d);
+            else f[0] = po[d];
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) acc[c][e] = fmaf(wj, f[e], acc[c][e]);
+            for (int e = 0; e < kVec; ++e) acc[c][e] = fmaf(wj, f[e], acc[c][e]);
+          }
         }
       }
     }
-  }
-  if constexpr (kWarps > 1) {
+    if constexpr (kWarps > 1) {
+      __syncthreads();  // the last row's sums have been read
 #pragma unroll
-    for (int c = 0; c < kLoads; ++c)
+      for (int c = 0; c < kLoads; ++c)
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) part[warp][(c * kVec + e) * 32 + lane] = acc[c][e];
-    __syncthreads();
-    if (sub != 0) return;
+        for (int e = 0; e < kVec; ++e) part[warp][(c * kVec + e) * 32 + lane] = acc[c][e];
+      __syncthreads();
+      if (sub != 0) continue;
 #pragma unroll
-    for (int c = 0; c < kLoads; ++c)
+      for (int c = 0; c < kLoads; ++c)
 #pragma unroll
-      for (int e = 0; e < kVec; ++e)
+        for (int e = 0; e < kVec; ++e)
 #pragma unroll
-        for (int k = 1; k < kWarps; ++k) acc[c][e] += part[warp + k][(c * kVec + e) * 32 + lane];
-  }
-  int hq, n;
-  tree_row(p, hkv, r_all, &hq, &n);
-  T* out = static_cast<T*>(p.o) + b * p.so[0] + hq * p.so[1] + n * p.so[2];
-  const float inv = total > 0.f ? 1.f / total : 0.f;
-#pragma unroll
-  for (int c = 0; c < kLoads; ++c)
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      const int d = (lane + 32 * c) * kVec + e;
-      if (d < p.D) out[d] = from_f32<T>(acc[c][e] * inv);
+          for (int k = 1; k < kWarps; ++k) acc[c][e] += part[warp + k][(c * kVec + e) * 32 + lane];
     }
-  if (lane == 0 && p.lse) {
-    float l = neg_inf();
-    if (total > 0.f) {
-      l = (m + log2f(total)) * kLn2;
-      if (p.alibi) {  // the row's depth, by the way up to the root
-        int depth = 0;
-        for (int x = n; x > 0; ++depth) {
-          const int up = p.parents ? p.parents[b * p.parents_stride + x] : x - 1;
-          if (up < 0 || up >= x) break;
-          x = up;
-        }
-        l += tree_row_shift(p, hq, len + depth);
+    int hq, n;
+    tree_row(p, hkv, rb0 + r, &hq, &n);
+    T* out = static_cast<T*>(p.o) + b * p.so[0] + hq * p.so[1] + n * p.so[2];
+    const float inv = total > 0.f ? 1.f / total : 0.f;
+#pragma unroll
+    for (int c = 0; c < kLoads; ++c)
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        const int d = (lane + 32 * c) * kVec + e;
+        if (d < p.D) out[d] = from_f32<T>(acc[c][e] * inv);
       }
+    if (lane == 0 && p.lse) {
+      float l = neg_inf();
+      if (total > 0.f) {
+        l = (m + log2f(total)) * kLn2;
+        if (p.alibi) {  // the row's depth, by the way up to the root
+          int depth = 0;
+          for (int x = n; x > 0; ++depth) {
+            const int up = p.parents ? p.parents[b * p.parents_stride + x] : x - 1;
+            if (up < 0 || up >= x) break;
+            x = up;
+          }
+          l += tree_row_shift(p, hq, len + depth);
+        }
+      }
+      p.lse[((int64_t)b * p.Hq + hq) * p.N + n] = l;
     }
-    p.lse[((int64_t)b * p.Hq + hq) * p.N + n] = l;
   }
 }
 
@@ -122,9 +135,11 @@ int check_tree(const bfa_tree_args* a) {
   if (a->head_dim < 1 || a->head_dim > 256 || a->nodes > kTreeNodes || a->dtype != (int)a->dtype ||
       dtype_bytes((int)a->dtype) == 0)
     return BFA_ERR_UNSUPPORTED;
-  // Positions, rows per KV head and items are counted in 32 bits.
+  // Positions, rows per KV head, items, and the chunks of a sequence's items
+  // are counted in 32 bits.
   if (a->batch > (1 << 24) || a->heads_q > (1 << 20) || a->page_size > INT32_MAX / 2 ||
-      a->max_pages > (INT32_MAX / 2 - 128) / a->page_size || a->batch * a->heads_q > INT32_MAX / kTreeNodes)
+      a->max_pages > (INT32_MAX / 2 - 128) / a->page_size || a->batch * a->heads_q > INT32_MAX / kTreeNodes ||
+      a->heads_q * ((a->max_pages * a->page_size + 64) / 32 + 4) > INT32_MAX / 4)
     return BFA_ERR_UNSUPPORTED;
   return BFA_OK;
 }
@@ -156,7 +171,7 @@ Plan make_plan(const bfa_tree_args* a, const TreeTile& tile) {
 TreeTile simt_tile(const bfa_tree_args* a) { return {kTreeSimtRows, kTreeSimtChunk, a->head_dim > 128 ? 1 : 2}; }
 
 // Rows per KV head from which the tcgen05 kernel is taken, where the layouts allow it.
-constexpr int64_t kTcgen05Rows = 33;
+constexpr int64_t kTcgen05Rows = 1;
 
 bool tcgen05_on() {  // BFA_TREE_TCGEN05=0 keeps bf16/fp16 on the mma.sync kernel, =1 on tcgen05 at any row count
   const char* e = std::getenv("BFA_TREE_TCGEN05");
@@ -177,19 +192,28 @@ size_t workspace_bytes(const bfa_tree_args* a) {
 
 template <typename T>
 int launch_merge(const TreeParams& p, cudaStream_t st) {
-  const int64_t rows = (int64_t)p.B * p.Hkv * p.G * p.N;
+  const int64_t items = (int64_t)p.B * p.Hkv * p.n_rb;
   // Four warps per row where an item is spread over at least four blocks on average.
-  const bool wide = p.grid >= 4 * (int64_t)p.B * p.Hkv * p.n_rb;
-  const unsigned blocks = (unsigned)(wide ? rows : (rows + 3) / 4);
-  if (p.D % 4 == 0) {
-    if (wide) tree_merge_kernel<T, 4, 4><<<blocks, 128, 0, st>>>(p);
-    else tree_merge_kernel<T, 1, 4><<<blocks, 128, 0, st>>>(p);
-  } else {
-    if (wide) tree_merge_kernel<T, 4, 1><<<blocks, 128, 0, st>>>(p);
-    else tree_merge_kernel<T, 1, 1><<<blocks, 128, 0, st>>>(p);
+  const bool wide = p.grid >= 4 * items;
+  cudaLaunchConfig_t cfg{};
+  const int rows = merge_rows(wide ? 4 : 1);
+  cfg.gridDim = dim3((unsigned)(items * ((std::min(p.rb, p.G * p.N) + rows - 1) / rows)));
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  auto kernel = p.D % 4 == 0 ? (wide ? tree_merge_kernel<T, 4, 4> : tree_merge_kernel<T, 1, 4>)
+                             : (wide ? tree_merge_kernel<T, 4, 1> : tree_merge_kernel<T, 1, 1>);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return cuda_fail("tree merge launch", e);
   }
   note_launch();
-  return launch_status("tree merge launch");
+  return BFA_OK;
 }
 
 }  // namespace

@@ -51,16 +51,6 @@ __device__ __forceinline__ int tree_chunks_of(const TreeParams& p, int len) {
   return (len - tree_lo(p, len) + p.chunk - 1) / p.chunk + p.tree_chunks;
 }
 
-// Chunks before sequence b (all heads and row blocks), and of all sequences
-// for b = B; every lane of a warp calls it.
-__device__ __forceinline__ int64_t tree_chunks_before(const TreeParams& p, int b) {
-  int64_t n = 0;
-  for (int i = threadIdx.x & 31; i < b; i += 32) n += tree_chunks_of(p, tree_len(p, i));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-  return n * p.Hkv * p.n_rb;
-}
-
 // Of `grid` blocks, those that have work: every one of them at least a chunk.
 __device__ __forceinline__ int tree_blocks(const TreeParams& p, int64_t T) { return (int)(T < p.grid ? T : p.grid); }
 // Where block i's stretch of T chunks begins, and which block holds chunk x.
@@ -78,36 +68,6 @@ struct TreeCursor {
       n = tree_chunks_of(p, len);
     }
   }
-  // Positions the cursor at chunk x of the list (all lanes of a warp).
-  __device__ __forceinline__ void seek(const TreeParams& p, int64_t x) {
-    const int lane = threadIdx.x & 31;
-    const int per = p.Hkv * p.n_rb;
-    int64_t before = 0;
-    b = 0;
-    // 32 sequences at a time: a prefix sum over the warp finds x's sequence.
-    for (int b0 = 0; b0 < p.B; b0 += 32) {
-      const int64_t mine = b0 + lane < p.B ? (int64_t)tree_chunks_of(p, tree_len(p, b0 + lane)) * per : 0;
-      int64_t sum = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += y;
-      }
-      const unsigned m = __ballot_sync(0xffffffffu, before + sum > x);
-      if (m) {
-        const int l = __ffs(m) - 1;
-        b = b0 + l;
-        before += __shfl_sync(0xffffffffu, sum - mine, l);
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, sum, 31);
-      b = b0 + 32;
-    }
-    load(p);
-    const int64_t in = x - before;
-    item = (int)(in / n);
-    c = (int)(in - (int64_t)item * n);
-  }
   // On by k chunks of the same item (k >= 1; past its end: to the next item).
   __device__ __forceinline__ void next(const TreeParams& p, int k = 1) {
     c += k;
@@ -124,6 +84,71 @@ struct TreeCursor {
     return in_tree(p) ? (c - (n - p.tree_chunks)) * p.chunk : lo + c * p.chunk;
   }
 };
+
+// Chunks of all sequences' items, and of those before sequence b (b < 0: not
+// asked for); every lane of a warp calls it.
+__device__ __forceinline__ int64_t tree_total(const TreeParams& p, int b, int64_t* before) {
+  int64_t n = 0, m = 0;
+  for (int i = threadIdx.x & 31; i < p.B; i += 32) {
+    const int c = tree_chunks_of(p, tree_len(p, i));
+    n += c;
+    if (i < b) m += c;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    n += __shfl_xor_sync(0xffffffffu, n, o);
+    m += __shfl_xor_sync(0xffffffffu, m, o);
+  }
+  *before = m * p.Hkv * p.n_rb;
+  return n * p.Hkv * p.n_rb;
+}
+
+// This block's stretch: `cur` at its first chunk, returns its number of chunks
+// (0: none). Every lane of a warp calls it; one pass over the lengths where a
+// lane each holds them.
+__device__ __forceinline__ int tree_stretch(const TreeParams& p, TreeCursor& cur) {
+  const int lane = threadIdx.x & 31;
+  const int per = p.Hkv * p.n_rb;
+  int64_t T = 0, before = 0, x = 0, end = 0;
+  for (int pass = p.B > 32 ? 0 : 1; pass < 2; ++pass) {
+    // Pass 0 (more than 32 sequences): the total. Pass 1: 32 sequences at a
+    // time, a prefix sum over the warp finds the sequence of chunk x.
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+      const int64_t mine = b0 + lane < p.B ? (int64_t)tree_chunks_of(p, tree_len(p, b0 + lane)) * per : 0;
+      int64_t sum = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += y;
+      }
+      const int64_t all = __shfl_sync(0xffffffffu, sum, 31);
+      if (pass == 0) {
+        T += all;
+        continue;
+      }
+      if (b0 == 0) {
+        if (p.B <= 32) T = all;
+        const int blocks = tree_blocks(p, T);
+        if ((int)blockIdx.x >= blocks) return 0;
+        x = tree_start(T, blocks, blockIdx.x);
+        end = tree_start(T, blocks, blockIdx.x + 1);
+      }
+      const unsigned m = __ballot_sync(0xffffffffu, before + sum > x);
+      if (m) {
+        const int l = __ffs(m) - 1;
+        cur.b = b0 + l;
+        before += __shfl_sync(0xffffffffu, sum - mine, l);
+        break;
+      }
+      before += all;
+    }
+  }
+  cur.load(p);
+  const int in = (int)(x - before);  // within one sequence: fits 32 bits (checked by the host)
+  cur.item = in / cur.n;
+  cur.c = in - cur.item * cur.n;
+  return (int)(end - x);
+}
 
 // The rows of K and V that key j of a chunk lies in (null reads as zeros).
 // Reports a bad page. Rows of absent nodes are read like the others: their

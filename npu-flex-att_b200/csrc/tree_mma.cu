@@ -130,13 +130,10 @@ __global__ void __launch_bounds__(32 * RW * KW, (Tile<D, RW, KW>::kPerSm)) tree_
   const int rw = warp % RW, kw = warp / RW;
   const int g = lane >> 2, t = lane & 3;
 
-  const int64_t T_all = tree_chunks_before(p, p.B);
-  const int blocks = tree_blocks(p, T_all);
-  if ((int)blockIdx.x >= blocks) return;
-  const int64_t x0 = tree_start(T_all, blocks, blockIdx.x);
-  const int n_x = (int)(tree_start(T_all, blocks, blockIdx.x + 1) - x0);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   TreeCursor cur;
-  cur.seek(p, x0);
+  const int n_x = tree_stretch(p, cur);
+  if (n_x == 0) return;
   TreeCursor ahead = cur;  // the next chunk to look up
 
   // Columns past the head dim are never loaded.

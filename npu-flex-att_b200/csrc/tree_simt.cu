@@ -56,12 +56,10 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const TreeParams p,
   float* vs = ks + 2 * kKeys * kPitch;    // [2][kKeys][kPitch]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
-  const int64_t T_all = tree_chunks_before(p, p.B);
-  const int blocks = tree_blocks(p, T_all);
-  if ((int)blockIdx.x >= blocks) return;
-  const int64_t x0 = tree_start(T_all, blocks, blockIdx.x), x1 = tree_start(T_all, blocks, blockIdx.x + 1);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   TreeCursor cur;
-  cur.seek(p, x0);
+  const int n_x = tree_stretch(p, cur);
+  if (n_x == 0) return;
   if (tid == 0) {  // a clamped length is an error of the caller's
     if (p.status && p.lens[cur.b] != cur.len) *p.status = BFA_ERR_INDEX;
   }
@@ -98,14 +96,14 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const TreeParams p,
   lookup(0);
   __syncthreads();
   load(0);
-  if (x0 + 1 < x1) lookup(1);
+  if (n_x > 1) lookup(1);
 
-  for (int64_t x = x0; x < x1; ++x) {
-    const int buf = (int)((x - x0) & 1);
+  for (int x = 0; x < n_x; ++x) {
+    const int buf = x & 1;
     const int hkv = cur.item / p.n_rb, rb0 = (cur.item - hkv * p.n_rb) * kRows;
     const int R = min(kRows, p.G * p.N - rb0);
     __syncthreads();  // the other buffer's readers and this chunk's addresses are done
-    if (x + 1 < x1) load(buf ^ 1);
+    if (x + 1 < n_x) load(buf ^ 1);
     if (fresh) {
       fresh = false;
       seg_c0 = cur.c;
@@ -142,10 +140,10 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const TreeParams p,
 #pragma unroll
           for (int c = 0; c < kC; ++c) acc[a][i][c] = 0.f;
     }
-    if (x + 1 < x1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    if (x + 1 < n_x) asm volatile("cp.async.wait_group 1;" ::: "memory");
     else asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
-    if (x + 2 < x1) lookup(buf);  // this chunk's own addresses have been used
+    if (x + 2 < n_x) lookup(buf);  // this chunk's own addresses have been used
 
     {  // S and softmax: rows 4·warp + i, key = lane
       const float* kr = ks + (buf * kKeys + lane) * kPitch;
@@ -221,7 +219,7 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const TreeParams p,
     }
     const TreeCursor done = cur;
     cur.next(p);
-    if (cur.c != 0 && x + 1 < x1) continue;
+    if (cur.c != 0 && x + 1 < n_x) continue;
 
     // The item, or this block's stretch of it, ends.
     fresh = true;

@@ -11,25 +11,31 @@
 //
 // Split. Persistent blocks, one per SM, each with an equal stretch of the list
 // of chunks (tree_common.cuh). Warp roles:
-//   warp 0      producer: looks the chunk's pages up (a lane per box) and loads
-//               K and V by TMA into a ring that runs on across items
+//   warp 0      producer: looks a chunk's pages up one chunk ahead and loads K
+//               and V by TMA, a lane per box, into a ring that runs on across
+//               items
 //   warp 1      MMA issuer
 //   warp 2      TMEM allocator
-//   warps 4..   softmax, a thread per row (TMEM lane): 4 warps per 128-row tile
+//   warp 3      the tree's ancestor sets, one item ahead
+//   warps 4..   softmax, 8 warps per 128-row tile: two threads share a row (TMEM
+//               lane), each with half of the chunk's keys and of O's columns;
+//               they agree on the row's maximum through shared memory
 // With two tiles (NT = 2) one tile's softmax runs under the other's products:
 // S_0(j), S_1(j), then PV_0(j), S_0(j+1), PV_1(j), S_1(j+1). With one tile S is
-// double-buffered: S(j+1) is formed before PV(j).
+// double-buffered: S(j+1) is formed before PV(j). P·V goes out in two halves
+// of the keys, the first when the first half's threads have stored P.
 //
 // A box is gcd(page_size, chunk) tokens of one page, so any page size that is a
 // multiple of 8 works (8 rows of 128 bytes are the swizzle's atom). Tokens past
-// a sequence's end, and nodes past N, arrive as whatever the page holds: their
-// logits are masked, and in such chunks the softmax warps clear those rows of
-// V before the product may read them.
+// a sequence's end arrive as whatever the page holds: their logits are masked,
+// P·V stops at the last 16 keys that hold one, and the softmax warps clear the
+// rest of those 16 in V before the product may read it.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <climits>
 #include <numeric>
+#include <type_traits>
 
 #include "sm100_host.h"
 #include "sm100_ptx.cuh"
@@ -42,6 +48,7 @@ using namespace sm100;
 
 constexpr int kBM = 128;
 constexpr float kRescaleThreshold = 8.0f;
+constexpr int kPolyEvery = 8;
 
 // CH keys per chunk: 128, or 64 at D = 256 (64 KB of K and V either way).
 template <int D, int NT>
@@ -50,14 +57,14 @@ struct TreeLayout {
   static constexpr int kSub = D / 64;
   static constexpr uint32_t kQTile = kBM * D * 2;
   static constexpr uint32_t kKV = kCH * D * 2;
-  static constexpr uint32_t kMisc = 2048;
+  static constexpr uint32_t kMisc = 10240;
   static constexpr int kFit = (int)((232448u - 1024u - kMisc - NT * kQTile) / kKV);
   static constexpr int kStages = kFit < 8 ? kFit : 8;
   static constexpr uint32_t kOffKV = NT * kQTile;
   static constexpr uint32_t kOffMisc = kOffKV + kStages * kKV;
   static constexpr uint32_t kBytes = kOffMisc + kMisc + 1024;  // 1024: alignment of the tiles
   static constexpr uint32_t kTmemO = 2 * kCH;
-  static constexpr int kThreads = 128 + 128 * NT;
+  static constexpr int kThreads = 128 + 256 * NT;
   static_assert(kStages >= 4, "K and V of two chunks");
   static_assert(kTmemO + NT * D <= 512, "TMEM");
   static_assert(kBytes <= 232448, "shared memory");
@@ -68,9 +75,11 @@ struct TreeMisc {
   uint32_t tmem;
   int abort;
   unsigned long long bad[2][2];  // by the chunk's parity: its keys whose values are not finite
-  TreeMasks masks;
+  float top[2][2][2][kBM];       // row maxima: chunk's parity, tile, half of the keys, row
+  float sum[2][2][kBM];          // row sums at an item's end: tile, half, row
+  TreeMasks masks[2];            // by the item's parity
 };
-static_assert(sizeof(TreeMisc) <= 2048, "misc");
+static_assert(sizeof(TreeMisc) <= 10240, "misc");
 
 // One column (32 bits per lane) of TMEM.
 __device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr) {
@@ -94,20 +103,23 @@ __device__ __forceinline__ bool any_not_finite(uint32_t w) {
   return (w & e) == e || ((w >> 16) & e) == e;
 }
 
-template <int D, int NT, bool BF16, bool PLAIN>
+template <int D, int NT, bool BF16, bool CAP, bool ALIBI>
 __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
     tree_kernel(const __grid_constant__ CUtensorMap tmKp, const __grid_constant__ CUtensorMap tmVp,
                 const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeParams p, int box,
                 uint64_t timeout_ns) {
   using L = TreeLayout<D, NT>;
   constexpr int CH = L::kCH, NS = L::kStages;
+  constexpr int HC = CH / 2;  // keys of a softmax thread per chunk
   enum {
     kQFull = 0,
     kKVFull = 1,
     kKVEmpty = kKVFull + NS,
-    kSFull = kKVEmpty + NS,  // NT = 2: S_t formed; NT = 1: the S buffer of that parity
-    kPHalf = kSFull + 2,     // P of the first half of the keys (and a final O) in TMEM
-    kPFull = kPHalf + NT,
+    kMask = kKVEmpty + NS,   // the item's ancestor sets, by its parity
+    kMaskFree = kMask + 2,   // an item's softmax is done with them
+    kSFull = kMaskFree + 2,  // NT = 2: S_t formed; NT = 1: the S buffer of that parity
+    kPHalf = kSFull + 2,     // P of the first half of the keys, and a final O, in TMEM
+    kPFull = kPHalf + NT,    // P of the second half
     kODone = kPFull + NT,
     kDrain = kODone + NT,
     kNumBars = kDrain + 1
@@ -121,18 +133,17 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
   auto bar = [&](int i) -> uint32_t { return sbase + L::kOffMisc + 8u * (uint32_t)i; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  const int64_t T_all = tree_chunks_before(p, p.B);
-  const int blocks = tree_blocks(p, T_all);
-  if ((int)blockIdx.x >= blocks) return;
-  const int64_t x0 = tree_start(T_all, blocks, blockIdx.x);
-  const int n_x = (int)(tree_start(T_all, blocks, blockIdx.x + 1) - x0);
-  TreeCursor cur;
-  cur.seek(p, x0);
-
-  WaitCtl ctl{(volatile int*)&mi.abort, p.status, timeout_ns};
-  if (threadIdx.x == 0) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (threadIdx.x == 32) {
+    tma_prefetch_desc(&tmKp);
+    tma_prefetch_desc(&tmVp);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
     for (int i = 0; i < kNumBars; ++i)
-      mbar_init(bar(i), i == kQFull ? 4u * NT : (i >= kPHalf && i < kODone) ? 4u : 1u);
+      mbar_init(bar(i), i == kQFull || i == kMaskFree || i == kMaskFree + 1 ? 8u * NT
+                        : i >= kPHalf && i < kPFull                         ? 8u
+                        : i >= kPFull && i < kODone                         ? 4u
+                                                                            : 1u);
     mi.abort = 0;
     fence_barrier_init();
   }
@@ -140,6 +151,9 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
     tmem_alloc(smem_u32(&mi.tmem), 512);
     tmem_relinquish();
   }
+  TreeCursor cur;
+  const int n_x = tree_stretch(p, cur);  // 0 in a block without work: it only passes through
+  WaitCtl ctl{(volatile int*)&mi.abort, p.status, timeout_ns};
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -147,31 +161,44 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
-    if (lane == 0) {
-      tma_prefetch_desc(&tmKp);
-      tma_prefetch_desc(&tmVp);
-      tma_prefetch_desc(&tmK);
-      tma_prefetch_desc(&tmV);
-    }
+    // Lane i·kSub + s: columns [64s, 64s + 64) of box i, tokens [key0 + i·box,
+    // + box) of one page (the tree's chunk: one box of 64 nodes).
+    const int my_box = lane / L::kSub, my_sub = lane % L::kSub;
+    struct Box {
+      int page, slot;
+      bool mine;
+    };
+    auto lookup = [&](const TreeCursor& at) -> Box {
+      Box r{0, 0, false};
+      if (at.in_tree(p)) {
+        r.mine = my_box == 0;
+        return r;
+      }
+      const int t0 = at.key0(p) + my_box * box;
+      r.mine = my_box < CH / box && t0 < at.len;
+      if (r.mine) {
+        const int pg = t0 / p.page;
+        r.slot = t0 - pg * p.page;
+        r.page = p.table[at.b * p.table_stride + pg];
+      }
+      return r;
+    };
     bool ok = true;
     int n = 0;
+    Box next{0, 0, false};
+    if (n_x > 0) next = lookup(cur);
     for (int x = 0; x < n_x && ok; ++x) {
-      const bool tree = cur.in_tree(p);
-      const int key0 = cur.key0(p), hkv = cur.item / p.n_rb;
-      // Lane i: box i of the chunk, tokens [key0 + i·box, + box) of one page.
-      const int t0 = key0 + lane * box;
-      const bool mine = tree ? lane == 0 : (lane < CH / box && t0 < cur.len);
-      int page = 0, slot = 0;
-      if (mine && !tree) {
-        const int pg = t0 / p.page;
-        slot = t0 - pg * p.page;
-        page = p.table[cur.b * p.table_stride + pg];
-        if (page < 0 || page >= p.num_pages) {
-          page = (int)p.num_pages;  // outside the tensor: reads as zeros
-          if (p.status) *p.status = BFA_ERR_INDEX;
-        }
+      Box me = next;
+      const TreeCursor here = cur;
+      cur.next(p);
+      if (x + 1 < n_x) next = lookup(cur);  // in flight while this chunk's slots are waited for
+      const bool tree = here.in_tree(p);
+      const int hkv = here.item / p.n_rb;
+      if (!tree && me.mine && (me.page < 0 || me.page >= p.num_pages)) {
+        me.page = (int)p.num_pages;  // outside the tensor: reads as zeros
+        if (p.status) *p.status = BFA_ERR_INDEX;
       }
-      const uint32_t bytes = tree ? 64u * 128u * L::kSub : (uint32_t)__popc(__ballot_sync(0xffffffffu, mine)) * box * 128u * L::kSub;
+      const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xffffffffu, me.mine)) * (tree ? 64 : box) * 128u;
       for (int kv = 0; kv < 2; ++kv, ++n) {
         const int st = n % NS;
         if (n >= NS) {
@@ -182,17 +209,13 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
         }
         if (lane == 0) mbar_arrive_expect_tx(bar(kKVFull + st), bytes);
         __syncwarp();
-        if (mine) {
-          const uint32_t dst = sbase + L::kOffKV + st * L::kKV;
-          for (int s = 0; s < L::kSub; ++s) {
-            if (tree) tma_load_4d(dst + s * (CH * 128), kv ? &tmV : &tmK, bar(kKVFull + st), s * 64, 0, hkv, cur.b);
-            else
-              tma_load_4d(dst + s * (CH * 128) + lane * box * 128, kv ? &tmVp : &tmKp, bar(kKVFull + st), s * 64, slot, hkv, page);
-          }
+        if (me.mine) {
+          const uint32_t dst = sbase + L::kOffKV + st * L::kKV + my_sub * (CH * 128) + my_box * box * 128;
+          if (tree) tma_load_4d(dst, kv ? &tmV : &tmK, bar(kKVFull + st), my_sub * 64, 0, hkv, here.b);
+          else tma_load_4d(dst, kv ? &tmVp : &tmKp, bar(kKVFull + st), my_sub * 64, me.slot, hkv, me.page);
         }
         __syncwarp();
       }
-      cur.next(p);
     }
     if (lane == 0)
       for (int i = (n > NS ? n - NS : 0); i < n; ++i) drain_wait(bar(kKVFull + i % NS), (i / NS) & 1, timeout_ns);
@@ -214,55 +237,51 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
         }
         mma_commit(bar(kSFull + buf));
       };
-      // P·V in two halves of the keys; O is zeroed by the softmax warps at an
-      // item's start, so every product accumulates.
-      auto issue_pv = [&](int t, int buf, int idx, int half) {
-        const uint64_t dv = desc_mnmajor(kv_addr(idx), CH * 128);
-#pragma unroll
-        for (int k4 = 0; k4 < CH / 32; ++k4) {
-          const int kk = half * (CH / 32) + k4;
-          mma_ts(tmem + L::kTmemO + t * D, tmem + buf * CH + kk * 8, dv + ((kk * 16 * 128) >> 4), idO, 1u);
-        }
-        if (half == 1) mma_commit(bar(kODone + t));
-      };
       auto wait = [&](int i, int parity) {
         if (!mbar_wait(bar(i), (uint32_t)parity, ctl, BFA_ERR_DEVICE_TIMEOUT)) return false;
         tc_fence_after();
         return true;
       };
       auto wait_load = [&](int idx) { return wait(kKVFull + idx % NS, (idx / NS) & 1); };
-      auto pv = [&](int t, int buf, int x) {
-        if (!wait(kPHalf + t, x & 1)) return false;
-        issue_pv(t, buf, 2 * x + 1, 0);
-        if (!wait(kPFull + t, x & 1)) return false;
-        issue_pv(t, buf, 2 * x + 1, 1);
+      // P·V of chunk x over its first `steps`·16 keys, in two halves. O is
+      // zeroed by the softmax warps at an item's start: every product adds.
+      auto pv = [&](int t, int buf, int x, int steps) {
+        const uint64_t dv = desc_mnmajor(kv_addr(2 * x + 1), CH * 128);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          if (!wait(half ? kPFull + t : kPHalf + t, x & 1)) return false;
+#pragma unroll
+          for (int k4 = 0; k4 < CH / 32; ++k4) {
+            const int kk = half * (CH / 32) + k4;
+            if (kk < steps)
+              mma_ts(tmem + L::kTmemO + t * D, tmem + buf * CH + kk * 8, dv + ((kk * 16 * 128) >> 4), idO, 1u);
+          }
+        }
+        mma_commit(bar(kODone + t));
         return true;
       };
       bool ok = true;
       int seg = 0;
       for (int x = 0; x < n_x && ok; ++seg) {
-        const int count = min(cur.n - cur.c, n_x - x);  // chunks of this segment
-        const int end = x + count;
+        const int count = min(cur.n - cur.c, n_x - x);  // chunks of this item that are this block's
         ok = wait(kQFull, seg & 1) && wait_load(2 * x);
         if (!ok) break;
-        if constexpr (NT == 2) {
-          issue_s(0, 0, 2 * x);
-          issue_s(1, 1, 2 * x);
-          mma_commit(bar(kKVEmpty + (2 * x) % NS));
-        } else {
-          issue_s(0, x & 1, 2 * x);
-          mma_commit(bar(kKVEmpty + (2 * x) % NS));
-        }
-        for (; x < end; ++x) {
+        issue_s(0, NT == 2 ? 0 : x & 1, 2 * x);
+        if constexpr (NT == 2) issue_s(1, 1, 2 * x);
+        mma_commit(bar(kKVEmpty + (2 * x) % NS));
+        for (int it = 0; it < count; ++it, ++x) {
           const int iv = 2 * x + 1, ik = 2 * x + 2;
-          const bool more = x + 1 < end;
+          const bool more = it + 1 < count;
+          const int c = cur.c + it;
+          const int keys = c >= cur.n - p.tree_chunks ? p.N : min(CH, cur.len - (cur.lo + c * CH));
+          const int steps = (keys + 15) / 16;
           if constexpr (NT == 2) {
-            if (!(ok = wait_load(iv) && pv(0, 0, x))) break;
+            if (!(ok = wait_load(iv) && pv(0, 0, x, steps))) break;
             if (more) {
               if (!(ok = wait_load(ik))) break;
               issue_s(0, 0, ik);
             }
-            if (!(ok = pv(1, 1, x))) break;
+            if (!(ok = pv(1, 1, x, steps))) break;
             mma_commit(bar(kKVEmpty + iv % NS));
             if (more) {
               issue_s(1, 1, ik);
@@ -274,7 +293,7 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
               issue_s(0, (x + 1) & 1, ik);
               mma_commit(bar(kKVEmpty + ik % NS));
             }
-            if (!(ok = wait_load(iv) && pv(0, x & 1, x))) break;
+            if (!(ok = wait_load(iv) && pv(0, x & 1, x, steps))) break;
             mma_commit(bar(kKVEmpty + iv % NS));
           }
         }
@@ -283,65 +302,76 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
       mma_commit(bar(kDrain));
       drain_wait(bar(kDrain), 0, timeout_ns);
     }
+  } else if (warp == 3) {
+    // ------------------------------------------------------------ ancestor sets
+    bool ok = true;
+    int seg = 0;
+    for (int x = 0; x < n_x && ok; ++seg) {
+      const int count = min(cur.n - cur.c, n_x - x);
+      if (seg > 1) ok = warp_wait(bar(kMaskFree + (seg & 1)), (uint32_t)(((seg >> 1) - 1) & 1), ctl);
+      tree_masks(p, cur.b, mi.masks[seg & 1]);
+      if (lane == 0) {
+        if (p.status && p.lens[cur.b] != cur.len) *p.status = BFA_ERR_INDEX;
+        mbar_arrive(bar(kMask + (seg & 1)));
+      }
+      x += count;
+      cur.next(p, count);
+    }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ softmax
-    const int t = (warp - 4) >> 2, wq = warp & 3;
-    const int row = t * kBM + wq * 32 + lane;  // of the row block
-    const int sid = threadIdx.x - 128;         // among the softmax threads
-    constexpr int kSoft = 128 * NT;
+    const int t = NT == 2 ? (warp - 4) >> 3 : 0, h = ((warp - 4) >> 2) & 1, wq = warp & 3;
+    const int row = wq * 32 + lane;     // of the tile
+    const int sid = threadIdx.x - 128;  // among the softmax threads
+    constexpr int kSoft = 256 * NT;
     const uint32_t lane_base = (uint32_t)(wq * 32) << 16;
-    const uint32_t tO = tmem + lane_base + L::kTmemO + t * D;
+    const uint32_t tO = tmem + lane_base + L::kTmemO + t * D + h * (D / 2);  // this thread's half of O
     const float sl2 = p.scale * kLog2e;
-    const bool cap = !PLAIN && p.soft_cap > 0.f;
-    const float cap_in = cap ? p.scale / p.soft_cap : 0.f, cap_out = cap ? p.soft_cap * kLog2e : 0.f;
+    const float cap_in = CAP ? p.scale / p.soft_cap : 0.f, cap_out = CAP ? p.soft_cap * kLog2e : 0.f;
     bool ok = true;  // false: this block gave up on a wait; the flow goes on without waiting
-    int x = 0;
-    while (x < n_x) {
+    int seg = 0;
+    for (int x = 0; x < n_x; ++seg) {
       // ---------------------------------------------------- an item begins
-      // (`cur` stands at its first chunk of this block's; little else is kept
-      // over the loop, whose S row fills the registers: what only the masked
-      // chunks and the end need is formed again there.)
+      // (`cur` stands at its first chunk of this block's. Little else is kept
+      // over the loop: what only masked chunks and the end need is formed
+      // again there, from values made opaque so that none stays in registers.)
       const int count = min(cur.n - cur.c, n_x - x);
-      const int rows = p.G * p.N - (cur.item % p.n_rb) * (NT * kBM);
-      const bool live_row = row < rows;  // rows past them are zeros, worked on like the others and not stored
-      auto where = [&](int* hq, int* node) {  // the row's head and node
-        int item = cur.item;  // opaque: each use forms its values anew, none stay in registers between
+      auto where = [&](int* hq, int* node) -> bool {  // the row's head and node; false past the rows
+        int item = cur.item;
         asm volatile("" : "+r"(item));
-        *hq = item / p.n_rb * p.G;
-        *node = 0;
-        if (live_row) tree_row(p, item / p.n_rb, (item % p.n_rb) * (NT * kBM) + row, hq, node);
+        const int hkv = item / p.n_rb, r = (item - hkv * p.n_rb) * (NT * kBM) + t * kBM + row;
+        const bool live = r < p.G * p.N;
+        tree_row(p, hkv, live ? r : 0, hq, node);
+        return live;
       };
       {
-        // q's row into the swizzled tile (its readers, the last item's S
-        // products, are done: their barrier was waited for).
+        // Half of q's row into the swizzled tile (its readers, the last item's
+        // S products, are done: their barrier was waited for).
         int hq, node;
-        where(&hq, &node);
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + cur.b * p.sq[0] + hq * p.sq[1] + node * p.sq[2]);
+        const bool live = where(&hq, &node);
+        const uint4* src =
+            reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + cur.b * p.sq[0] + hq * p.sq[1] + node * p.sq[2]);
         uint8_t* dst = smem + t * L::kQTile;
-#pragma unroll 4
-        for (int c = 0; c < D / 8; ++c) {
+#pragma unroll 8
+        for (int i = 0; i < D / 16; ++i) {
+          const int c = h * (D / 16) + i;
           uint4 w = make_uint4(0u, 0u, 0u, 0u);
-          if (live_row && c * 8 < p.D) w = src[c];
-          *reinterpret_cast<uint4*>(dst + (c >> 3) * (kBM * 128) + sw128_offset(wq * 32 + lane, c & 7)) = w;
+          if (live && c * 8 < p.D) w = src[c];
+          *reinterpret_cast<uint4*>(dst + (c >> 3) * (kBM * 128) + sw128_offset(row, c & 7)) = w;
         }
         fence_async_shared();
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kQFull));
-      {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kQFull));
         uint32_t z[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) z[i] = 0u;
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) tmem_st16(tO + 16 * c, z);
+        for (int c = 0; c < D / 32; ++c) tmem_st16(tO + 16 * c, z);
         tmem_st_wait();
       }
-      named_sync(1, kSoft);  // the last item's masks are no longer read
-      if (warp == 4) tree_masks(p, cur.b, mi.masks);
-      if (sid == 0 && p.status && p.lens[cur.b] != cur.len) *p.status = BFA_ERR_INDEX;
-      named_sync(1, kSoft);
+      TreeMasks& masks = mi.masks[seg & 1];
+      ok = ok && warp_wait(bar(kMask + (seg & 1)), (uint32_t)((seg >> 1) & 1), ctl);
       const int all_from = p.window > 0 ? cur.len + p.N - 1 - p.window : 0;
-      float m = neg_inf(), l = 0.f;
+      float m = neg_inf(), l = 0.f;  // l: of this thread's keys
 
       for (int it = 0; it < count; ++it, ++x) {
         const int c = cur.c + it;
@@ -351,156 +381,192 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
         const bool masked = tree || valid < CH || key0 < all_from;
         const int buf = NT == 2 ? t : x & 1;
         const uint32_t tS = tmem + lane_base + buf * CH;
-        ok = ok && warp_wait(bar(kSFull + buf), (uint32_t)(NT == 2 ? x & 1 : (x >> 1) & 1), ctl);
-        tc_fence_after();
 
-        // V rows that no key holds are cleared; where rows differ in what they
-        // see, values that are not finite are looked for (0·inf must not
-        // reach a row that does not see the key).
+        // The last P·V's rows of V that no key holds are cleared (the tree's
+        // come as zeros); where rows differ in what they see, values that are
+        // not finite are looked for: 0·inf must not reach a row that does not
+        // see the key.
         bool hold = false;
-        if (masked) {
+        const bool differ = (tree && p.N > 1) || key0 < all_from;
+        if (differ || (!tree && (valid & 15))) {
           ok = ok && warp_wait(bar(kKVFull + (2 * x + 1) % NS), (uint32_t)(((2 * x + 1) / NS) & 1), ctl);
           uint8_t* vt = smem + L::kOffKV + ((2 * x + 1) % NS) * L::kKV;
-          const bool differ = tree || key0 < all_from;
           unsigned long long* bad = mi.bad[x & 1];  // the other one may still be read by a slower warp
           if (sid < 2) bad[sid] = 0ull;
-          named_sync(1, kSoft);
-          // Piece i: 16 bytes of row i % CH of a 64-column sub-tile.
-          for (int i = sid; i < CH * (D / 8); i += kSoft) {
-            const int r = (i >> 3) % CH, sub = (i >> 3) / CH;
-            uint4* at = reinterpret_cast<uint4*>(vt + sub * (CH * 128) + r * 128 + (i & 7) * 16);
-            if (r >= valid) {
-              *at = make_uint4(0u, 0u, 0u, 0u);
-            } else if (differ) {
-              const uint4 w = *at;
-              if (any_not_finite<BF16>(w.x) || any_not_finite<BF16>(w.y) || any_not_finite<BF16>(w.z) || any_not_finite<BF16>(w.w))
-                atomicOr(&bad[r >> 6], 1ull << (r & 63));
+          named_sync(3, kSoft);
+          // Piece i: 16 bytes of row i / 8 of a 64-column sub-tile.
+          const int upto = (valid + 15) / 16 * 16;
+          for (int i = (differ ? 0 : valid * 8) + sid; i < upto * 8; i += kSoft) {
+            const int r = i >> 3;
+#pragma unroll
+            for (int sub = 0; sub < L::kSub; ++sub) {
+              uint4* at = reinterpret_cast<uint4*>(vt + sub * (CH * 128) + r * 128 + (i & 7) * 16);
+              if (r >= valid) {
+                *at = make_uint4(0u, 0u, 0u, 0u);
+              } else {
+                const uint4 w = *at;
+                if (any_not_finite<BF16>(w.x) || any_not_finite<BF16>(w.y) || any_not_finite<BF16>(w.z) || any_not_finite<BF16>(w.w))
+                  atomicOr(&bad[r >> 6], 1ull << (r & 63));
+              }
             }
           }
           fence_async_shared();
-          named_sync(1, kSoft);
+          named_sync(3, kSoft);
           hold = (bad[0] | bad[1]) != 0;
         }
 
-        float alpha = 1.f;
-        bool rescale = false;
-        uint32_t r[CH / 32][32];
-        float m_use = 0.f;
-        const bool formed = !PLAIN || masked || !(sl2 > 0.f);  // logits in r, else raw products
-        {
-          float mx = neg_inf();
-          if (formed) {
-            // Logits in base 2, masked, formed 32 columns at a time in place in
-            // TMEM: the rarer chunks stay out of the registers and the code of
-            // the plain ones. Kept columns: [lo, hi) of cached tokens, or the
-            // seen nodes.
+        ok = ok && warp_wait(bar(kSFull + buf), (uint32_t)(NT == 2 ? x & 1 : (x >> 1) & 1), ctl);
+        tc_fence_after();
+        uint32_t r[HC / 32][32];
+#pragma unroll
+        for (int ch = 0; ch < HC / 32; ++ch) tmem_ld32(tS + h * HC + 32 * ch, r[ch]);
+        tmem_ld_wait();
+        const bool formed = CAP || ALIBI || masked || !(sl2 > 0.f);  // logits in r, else raw products
+        float mx;
+        if (formed) {
+          // Logits in base 2 (cap's tanh: the series on the FMA pipe where
+          // every |s/cap| of the warp is small, else the closed form).
+          float slope2 = 0.f;
+          int ref = 0, depth = 0, pos = 0;
+          uint64_t seen = 0;
+          if (ALIBI || masked) {
             int hq, node;
-            where(&hq, &node);
-            const int depth = mi.masks.depth[node], pos = cur.len + depth;
-            uint64_t seen = live_row ? mi.masks.anc[node] : 0ull;
+            const bool live = where(&hq, &node);
+            depth = masks.depth[node];
+            pos = cur.len + depth;
+            seen = live ? masks.anc[node] : 0ull;
+            if (ALIBI) {
+              slope2 = p.alibi[hq] * kLog2e;
+              ref = tree_alibi_ref(p, slope2, pos);
+            }
+          }
+          auto form = [&](auto tier_tag) {
+            constexpr int TIER = decltype(tier_tag)::value;
+            const float abase = ALIBI ? slope2 * (float)(ref - key0 - h * HC) : 0.f;
+#pragma unroll
+            for (int ch = 0; ch < HC / 32; ++ch)
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) {
+                const float2 raw = make_float2(__uint_as_float(r[ch][e]), __uint_as_float(r[ch][e + 1]));
+                float2 y;
+                if (CAP) {
+                  float2 th;
+                  y = cap_logit2x2<TIER>(raw, cap_in, cap_out, &th);
+                } else {
+                  y = __fmul2_rn(raw, make_float2(sl2, sl2));
+                }
+                if (ALIBI) {
+                  const int k = 32 * ch + e;
+                  if (tree) {
+                    y.x += slope2 * (float)(ref - cur.len - masks.depth[(h * HC + k) & (kTreeNodes - 1)]);
+                    y.y += slope2 * (float)(ref - cur.len - masks.depth[(h * HC + k + 1) & (kTreeNodes - 1)]);
+                  } else {
+                    y.x += fmaf(-slope2, (float)k, abase);
+                    y.y += fmaf(-slope2, (float)(k + 1), abase);
+                  }
+                }
+                r[ch][e] = __float_as_uint(y.x);
+                r[ch][e + 1] = __float_as_uint(y.y);
+              }
+          };
+          const int tier = CAP ? cap_tier<HC>(&r[0][0], cap_in) : 0;
+          if (CAP && tier == 2) form(std::integral_constant<int, 2>{});
+          else if (CAP && tier == 1) form(std::integral_constant<int, 1>{});
+          else form(std::integral_constant<int, 0>{});
+          if (masked) {
+            // Kept columns: [lo, hi) of cached tokens, or the seen nodes.
             const int lo = p.window > 0 ? max(0, pos - p.window - key0) : 0;
             const int hi = seen ? valid : 0;
             if (tree && p.window > 0 && p.window < p.N)
               for (int i = 0; i < p.N; ++i)
-                if (depth - mi.masks.depth[i] > p.window) seen &= ~(1ull << i);
-            float slope2 = 0.f;
-            int ref = 0;
-            if (!PLAIN && p.alibi) {
-              slope2 = p.alibi[hq] * kLog2e;
-              ref = tree_alibi_ref(p, slope2, pos);
-            }
-#pragma unroll 1
-            for (int ch = 0; ch < CH / 32; ++ch) {
-              uint32_t u[32];
-              tmem_ld32(tS + 32 * ch, u);
-              tmem_ld_wait();
-              uint32_t keep = 0;  // bit e: column 32·ch + e
+                if (depth - masks.depth[i] > p.window) seen &= ~(1ull << i);
+#pragma unroll
+            for (int ch = 0; ch < HC / 32; ++ch) {
+              const int k0 = h * HC + 32 * ch;
+              uint32_t keep = 0;  // bit e: column k0 + e
               if (tree) {
-                keep = ch < 2 ? (uint32_t)(seen >> (32 * ch)) : 0u;
+                keep = k0 < kTreeNodes ? (uint32_t)(seen >> (k0 & 63)) : 0u;
               } else {
-                const int from = min(max(lo - 32 * ch, 0), 32), to = min(max(hi - 32 * ch, 0), 32);
+                const int from = min(max(lo - k0, 0), 32), to = min(max(hi - k0, 0), 32);
                 if (to > from) keep = (0xffffffffu >> (32 - (to - from))) << from;
               }
-              const float abase = slope2 * (float)(ref - key0 - 32 * ch);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                float y = __uint_as_float(u[e]);
-                if (PLAIN) {
-                  y *= sl2;
-                } else {
-                  y = cap ? cap_out * tanh_any(y * cap_in) : y * sl2;
-                  if (p.alibi) {
-                    if (tree) y += slope2 * (float)(ref - cur.len - mi.masks.depth[(32 * ch + e) & (kTreeNodes - 1)]);
-                    else y += fmaf(-slope2, (float)e, abase);
-                  }
-                }
-                y = (keep >> e) & 1u ? y : neg_inf();
-                mx = fmaxf(mx, y);
-                u[e] = __float_as_uint(y);
-              }
-              tmem_st32(tS + 32 * ch, u);
+              for (int e = 0; e < 32; ++e) r[ch][e] = (keep >> e) & 1u ? r[ch][e] : 0xff800000u;
             }
-            tmem_st_wait();
           }
-#pragma unroll
-          for (int ch = 0; ch < CH / 32; ++ch) tmem_ld32(tS + 32 * ch, r[ch]);
-          tmem_ld_wait();
-          if (!formed) {
-            float m4[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
-#pragma unroll
-            for (int ch = 0; ch < CH / 32; ++ch)
-#pragma unroll
-              for (int e = 0; e < 32; e += 2)
-                m4[(e >> 1) & 3] = fmax3(m4[(e >> 1) & 3], __uint_as_float(r[ch][e]), __uint_as_float(r[ch][e + 1]));
-            mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sl2;
-          }
-          const bool grow = (mx > m + kRescaleThreshold) || (m == neg_inf() && mx != neg_inf());
-          float m_new = m;
-          if (__any_sync(0xffffffffu, grow)) {
-            m_new = fmaxf(m, mx);
-            rescale = it > 0;
-          }
-          m_use = m_new == neg_inf() ? 0.f : m_new;
-          alpha = ex2(m - m_use);
-          m = m_new;
         }
+        {
+          float m4[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
+#pragma unroll
+          for (int ch = 0; ch < HC / 32; ++ch)
+#pragma unroll
+            for (int e = 0; e < 32; e += 2)
+              m4[(e >> 1) & 3] = fmax3(m4[(e >> 1) & 3], __uint_as_float(r[ch][e]), __uint_as_float(r[ch][e + 1]));
+          mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+          if (!formed) mx *= sl2;
+        }
+        // The row's maximum over both halves. The barrier also lets the second
+        // half store P over columns of S that the first half has read by now.
+        mi.top[x & 1][t][h][row] = mx;
+        tc_fence_before();
+        named_sync(1 + t, 256);
+        tc_fence_after();
+        mx = fmaxf(mx, mi.top[x & 1][t][h ^ 1][row]);
+        const bool grow = (mx > m + kRescaleThreshold) || (m == neg_inf() && mx != neg_inf());
+        float m_new = m;
+        bool rescale = false;
+        if (__any_sync(0xffffffffu, grow)) {  // alike in both halves: the same rows and maxima
+          m_new = fmaxf(m, mx);
+          rescale = it > 0;
+        }
+        const float m_use = m_new == neg_inf() ? 0.f : m_new;
+        const float alpha = ex2(m - m_use);
+        m = m_new;
         // O stands still: the last P·V is done.
         if (it > 0) {
           ok = ok && warp_wait(bar(kODone + t), (uint32_t)((x - 1) & 1), ctl);
           tc_fence_after();
         }
-        {
-          if (rescale) {
+        if (rescale) {
 #pragma unroll 1
-            for (int c = 0; c < D / 16; ++c) {
-              uint32_t o16[16];
-              tmem_ld16(tO + 16 * c, o16);
-              tmem_ld_wait();
+          for (int i = 0; i < D / 32; ++i) {
+            uint32_t o16[16];
+            tmem_ld16(tO + 16 * i, o16);
+            tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) o16[i] = __float_as_uint(__uint_as_float(o16[i]) * alpha);
-              tmem_st16(tO + 16 * c, o16);
-            }
+            for (int e = 0; e < 16; ++e) o16[e] = __float_as_uint(__uint_as_float(o16[e]) * alpha);
+            tmem_st16(tO + 16 * i, o16);
           }
+          tmem_st_wait();
+        }
+        if (h == 1 && !hold) {  // this half of O is final before the first P·V half
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(kPHalf + t));
+        }
+        {
           float2 s2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
           const float2 xs2 = make_float2(formed ? 1.f : sl2, formed ? 1.f : sl2), nm2 = make_float2(-m_use, -m_use);
+          // On chunks that every row keeps whole, every kPolyEvery-th
+          // exponential runs on the FMA pipe.
+          auto exps = [&](auto split_tag) {
+            constexpr bool SPLIT = decltype(split_tag)::value;
 #pragma unroll
-          for (int ch = 0; ch < CH / 32; ++ch) {
-            if (ch == CH / 64 && !hold) {  // the first half of P is stored
-              tmem_st_wait();
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(bar(kPHalf + t));
-            }
-            uint32_t pk[16];
+            for (int ch = 0; ch < HC / 32; ++ch) {
+              uint32_t pk[16];
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float2 y = __ffma2_rn(make_float2(__uint_as_float(r[ch][e]), __uint_as_float(r[ch][e + 1])), xs2, nm2);
-              const float p0 = ex2(y.x), p1 = ex2(y.y);
-              s2[(e >> 1) & 1] = __fadd2_rn(s2[(e >> 1) & 1], make_float2(p0, p1));
-              pk[e / 2] = pack2<BF16>(p0, p1);
+              for (int e = 0; e < 32; e += 2) {
+                const float2 y = __ffma2_rn(make_float2(__uint_as_float(r[ch][e]), __uint_as_float(r[ch][e + 1])), xs2, nm2);
+                const float p0 = ex2(y.x);
+                const float p1 = (SPLIT && e % kPolyEvery == kPolyEvery - 2) ? ex2_poly(y.y) : ex2(y.y);
+                s2[(e >> 1) & 1] = __fadd2_rn(s2[(e >> 1) & 1], make_float2(p0, p1));
+                pk[e / 2] = pack2<BF16>(p0, p1);
+              }
+              tmem_st16(tS + h * (HC / 2) + 16 * ch, pk);
             }
-            tmem_st16(tS + 16 * ch, pk);
-          }
+          };
+          if (masked) exps(std::false_type{});
+          else exps(std::true_type{});
           l = l * alpha + ((s2[0].x + s2[0].y) + (s2[1].x + s2[1].y));
           tmem_st_wait();
         }
@@ -508,70 +574,76 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
           // Values that are not finite: O += p·v by hand for the rows that see
           // them, then the rows of V are cleared for the product.
           uint8_t* vt = smem + L::kOffKV + ((2 * x + 1) % NS) * L::kKV;
-          {
+          tc_fence_before();
+          named_sync(3, kSoft);  // all of P is stored
+          tc_fence_after();
 #pragma unroll 1
-            for (int n = 0; n < valid; ++n) {
-              if (!((mi.bad[x & 1][n >> 6] >> (n & 63)) & 1)) continue;
-              const uint32_t w = tmem_ld1(tS + (n >> 1));
+          for (int n = 0; n < valid; ++n) {
+            if (!((mi.bad[x & 1][n >> 6] >> (n & 63)) & 1)) continue;
+            const uint32_t w = tmem_ld1(tS + (n >> 1));
+            tmem_ld_wait();
+            const float pr = half_of<BF16>(w, n & 1);
+#pragma unroll 1
+            for (int i = 0; i < D / 32; ++i) {
+              const int col = h * (D / 2) + 16 * i;
+              uint32_t o16[16];
+              tmem_ld16(tO + 16 * i, o16);
               tmem_ld_wait();
-              const float pr = half_of<BF16>(w, n & 1);
-#pragma unroll 1
-              for (int c = 0; c < D / 16; ++c) {
-                uint32_t o16[16];
-                tmem_ld16(tO + 16 * c, o16);
-                tmem_ld_wait();
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                  const uint4 v = *reinterpret_cast<const uint4*>(vt + (c >> 2) * (CH * 128) + sw128_offset(n, (c & 3) * 2 + i));
-                  const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
+              for (int e8 = 0; e8 < 2; ++e8) {
+                const uint4 v = *reinterpret_cast<const uint4*>(vt + (col >> 6) * (CH * 128) + sw128_offset(n, ((col & 63) >> 3) + e8));
+                const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                  for (int e = 0; e < 8; ++e)
-                    if (pr != 0.f)
-                      o16[8 * i + e] = __float_as_uint(__uint_as_float(o16[8 * i + e]) + pr * half_of<BF16>(vw[e >> 1], e & 1));
-                }
-                tmem_st16(tO + 16 * c, o16);
-                tmem_st_wait();
+                for (int e = 0; e < 8; ++e)
+                  if (pr != 0.f)
+                    o16[8 * e8 + e] = __float_as_uint(__uint_as_float(o16[8 * e8 + e]) + pr * half_of<BF16>(vw[e >> 1], e & 1));
               }
+              tmem_st16(tO + 16 * i, o16);
+              tmem_st_wait();
             }
           }
-          named_sync(1, kSoft);
-          for (int i = sid; i < CH * (D / 8); i += kSoft) {
-            const int rr = (i >> 3) % CH, sub = (i >> 3) / CH;
-            if ((mi.bad[x & 1][rr >> 6] >> (rr & 63)) & 1)
-              *reinterpret_cast<uint4*>(vt + sub * (CH * 128) + rr * 128 + (i & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-          }
+          named_sync(3, kSoft);
+          for (int i = sid; i < valid * 8; i += kSoft)
+            if ((mi.bad[x & 1][i >> 9] >> ((i >> 3) & 63)) & 1)
+#pragma unroll
+              for (int sub = 0; sub < L::kSub; ++sub)
+                *reinterpret_cast<uint4*>(vt + sub * (CH * 128) + (i >> 3) * 128 + (i & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
           fence_async_shared();
-          named_sync(1, kSoft);
+          named_sync(3, kSoft);
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          if (hold) mbar_arrive(bar(kPHalf + t));
-          mbar_arrive(bar(kPFull + t));
+          if (h == 0 || hold) mbar_arrive(bar(kPHalf + t));
+          if (h == 1) mbar_arrive(bar(kPFull + t));
         }
       }
 
       // ------------------------------------------------------ the item ends
+      mi.sum[t][h][row] = l;
+      named_sync(1 + t, 256);
+      l = mi.sum[t][0][row] + mi.sum[t][1][row];
       ok = ok && warp_wait(bar(kODone + t), (uint32_t)((x - 1) & 1), ctl);
       tc_fence_after();
       if (ok) {
         const bool whole = cur.c == 0 && count == cur.n;
         int hq, node;
-        where(&hq, &node);
-        if (mi.masks.anc[node] == 0) l = 0.f;  // absent: chunks that are not masked were summed for it too
+        const bool live = where(&hq, &node);
+        if (masks.anc[node] == 0) l = 0.f;  // absent: chunks that are not masked were summed for it too
         const float inv = l > 0.f ? 1.f / l : 0.f;
-        const int64_t prow = ((int64_t)blockIdx.x * 2 + (cur.c > 0 ? 0 : 1)) * p.rb + row;
-        uint16_t* og = static_cast<uint16_t*>(p.o) + cur.b * p.so[0] + hq * p.so[1] + node * p.so[2];
-        float* pg = p.part_o + prow * p.D;
+        const int64_t prow = ((int64_t)blockIdx.x * 2 + (cur.c > 0 ? 0 : 1)) * p.rb + t * kBM + row;
+        uint16_t* og = static_cast<uint16_t*>(p.o) + cur.b * p.so[0] + hq * p.so[1] + node * p.so[2] + h * (D / 2);
+        float* pg = p.part_o + prow * p.D + h * (D / 2);
+        const int d_end = live ? p.D - h * (D / 2) : 0;
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
+        for (int c = 0; c < D / 64; ++c) {
           uint32_t r[32];
           tmem_ld32(tO + 32 * c, r);
           tmem_ld_wait();
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const int d = 32 * c + 8 * q;
-            if (!live_row || d >= p.D) continue;
+            if (d >= d_end) continue;
             float f[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] = inv > 0.f ? __uint_as_float(r[8 * q + e]) * inv : 0.f;
@@ -585,14 +657,16 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
           }
           __syncwarp();
         }
-        if (live_row) {
+        if (live && h == 0) {
           const float l2 = l > 0.f ? m + lg2(l) : neg_inf();
           if (!whole) p.part_lse[prow] = l2;
           else if (p.lse)
             p.lse[((int64_t)cur.b * p.Hq + hq) * p.N + node] =
-                l2 == neg_inf() ? l2 : l2 * kLn2 + tree_row_shift(p, hq, cur.len + mi.masks.depth[node]);
+                l2 == neg_inf() ? l2 : l2 * kLn2 + tree_row_shift(p, hq, cur.len + masks.depth[node]);
         }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kMaskFree + (seg & 1)));
       cur.next(p, count);
     }
   }
@@ -617,10 +691,11 @@ int launch(const TreeParams& p, int dtype, cudaStream_t st) {
       !make_tmap_bhsd(&tm[2], p.k, dtype, p.D, p.N, p.Hkv, p.B, p.sk, 64) ||
       !make_tmap_bhsd(&tm[3], p.v, dtype, p.D, p.N, p.Hkv, p.B, p.sv, 64))
     return BFA_ERR_CUDA;
-  const bool plain = p.soft_cap == 0.f && !p.alibi;
-  auto kernel = plain ? tree_kernel<D, NT, BF16, true> : tree_kernel<D, NT, BF16, false>;
-  static std::atomic<uint64_t> done[2];
-  const int rc = allow_shared(kernel, (int)L::kBytes, done[plain], "tree attention shared memory");
+  const bool cap = p.soft_cap > 0.f, alibi = p.alibi != nullptr;
+  auto kernel = cap ? (alibi ? tree_kernel<D, NT, BF16, true, true> : tree_kernel<D, NT, BF16, true, false>)
+                    : (alibi ? tree_kernel<D, NT, BF16, false, true> : tree_kernel<D, NT, BF16, false, false>);
+  static std::atomic<uint64_t> done[4];
+  const int rc = allow_shared(kernel, (int)L::kBytes, done[2 * cap + alibi], "tree attention shared memory");
   if (rc) return rc;
   kernel<<<p.grid, L::kThreads, L::kBytes, st>>>(tm[0], tm[1], tm[2], tm[3], p, box, kTimeoutNs);
   note_launch();
