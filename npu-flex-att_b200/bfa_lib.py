@@ -7,9 +7,7 @@ implementation: if the library is missing, every call raises.
 from __future__ import annotations
 
 import ctypes
-import functools
 import os
-import struct
 import threading
 
 import torch
@@ -67,51 +65,41 @@ class BwdArgs(ctypes.Structure):
                 ("phases", ctypes.c_uint32), ("accumulate", ctypes.c_uint32)]
 
 
-def _wide(name, fields):
-    """A ctypes mirror of a structure whose fields are all 8 bytes wide, and
-    the struct.Struct that packs its fields in order, a tensor as its pointer
-    and four strides: one pack() call fills an argument block several times
-    faster than attribute by attribute, which is what a decoding step's calls
-    spend most of their host time on."""
-    cls = type(name, (ctypes.Structure,), {"_fields_": fields})
-    code = ""
-    for _, t in fields:
-        code += {Tensor: "5q", ctypes.c_int64: "q", ctypes.c_int64 * 2: "2q", ctypes.c_void_p: "q", ctypes.c_double: "d"}[t]
-    pack = struct.Struct("@" + code)
-    assert pack.size == ctypes.sizeof(cls)
-    return cls, pack.pack
-
-
 _i64, _ptr = ctypes.c_int64, ctypes.c_void_p
 
-RopeArgs, pack_rope = _wide("RopeArgs", [
-    ("batch", _i64), ("heads_q", _i64), ("heads_k", _i64), ("seqlen", _i64), ("head_dim", _i64),
-    ("rotary_dim", _i64), ("dtype", _i64), ("interleaved", _i64), ("inverse", _i64),
-    ("q", Tensor), ("k", Tensor), ("q_out", Tensor), ("k_out", Tensor), ("cos", _ptr), ("sin", _ptr),
-    ("table_rows", _i64), ("table_stride", _i64), ("positions", _ptr), ("positions_bytes", _i64),
-    ("positions_stride", _i64 * 2), ("offsets", _ptr), ("offsets_bytes", _i64), ("status", _ptr)])
 
-TreeArgs, pack_tree = _wide("TreeArgs", [
-    ("batch", _i64), ("heads_q", _i64), ("heads_kv", _i64), ("nodes", _i64), ("head_dim", _i64), ("dtype", _i64),
-    ("num_pages", _i64), ("page_size", _i64), ("max_pages", _i64), ("sliding_window", _i64),
-    ("scale", ctypes.c_double), ("soft_cap", ctypes.c_double), ("alibi_slopes", _ptr),
-    ("q", Tensor), ("k", Tensor), ("v", Tensor), ("o", Tensor), ("lse", _ptr), ("k_pages", Tensor), ("v_pages", Tensor),
-    ("page_table", _ptr), ("page_table_stride", _i64), ("lens", _ptr), ("parents", _ptr), ("parents_stride", _i64),
-    ("status", _ptr), ("workspace", _ptr), ("workspace_bytes", _i64)])
+class RopeArgs(ctypes.Structure):
+    _fields_ = [("batch", _i64), ("heads_q", _i64), ("heads_k", _i64), ("seqlen", _i64), ("head_dim", _i64),
+                ("rotary_dim", _i64), ("dtype", _i64), ("interleaved", _i64), ("inverse", _i64),
+                ("q", Tensor), ("k", Tensor), ("q_out", Tensor), ("k_out", Tensor), ("cos", _ptr), ("sin", _ptr),
+                ("table_rows", _i64), ("table_stride", _i64), ("positions", _ptr), ("positions_bytes", _i64),
+                ("positions_stride", _i64 * 2), ("offsets", _ptr), ("offsets_bytes", _i64), ("status", _ptr)]
 
-_TREE_VALUES = sum(5 if t is Tensor else 1 for _, t in TreeArgs._fields_)
 
-VerifyArgs, pack_verify = _wide("VerifyArgs", [
-    ("batch", _i64), ("nodes", _i64), ("vocab", _i64), ("dtype", _i64), ("target", _ptr), ("target_stride", _i64 * 2),
-    ("draft", _ptr), ("draft_stride", _i64 * 2), ("tokens", _ptr), ("tokens_bytes", _i64), ("tokens_stride", _i64),
-    ("parents", _ptr), ("parents_stride", _i64), ("uniforms", _ptr), ("uniforms_stride", _i64), ("noise", _ptr),
-    ("noise_stride", _i64), ("path", _ptr), ("count", _ptr), ("next_token", _ptr), ("status", _ptr)])
+class TreeArgs(ctypes.Structure):
+    _fields_ = [("batch", _i64), ("heads_q", _i64), ("heads_kv", _i64), ("nodes", _i64), ("head_dim", _i64),
+                ("dtype", _i64), ("num_pages", _i64), ("page_size", _i64), ("max_pages", _i64), ("sliding_window", _i64),
+                ("scale", ctypes.c_double), ("soft_cap", ctypes.c_double), ("alibi_slopes", _ptr),
+                ("q", Tensor), ("k", Tensor), ("v", Tensor), ("o", Tensor), ("lse", _ptr),
+                ("k_pages", Tensor), ("v_pages", Tensor), ("page_table", _ptr), ("page_table_stride", _i64),
+                ("lens", _ptr), ("parents", _ptr), ("parents_stride", _i64), ("status", _ptr), ("workspace", _ptr),
+                ("workspace_bytes", _i64)]
 
-AppendArgs, pack_append = _wide("AppendArgs", [
-    ("batch", _i64), ("heads_kv", _i64), ("tokens", _i64), ("head_dim", _i64), ("dtype", _i64), ("num_pages", _i64),
-    ("page_size", _i64), ("max_pages", _i64), ("k", Tensor), ("v", Tensor), ("k_pages", Tensor), ("v_pages", Tensor),
-    ("page_table", _ptr), ("page_table_stride", _i64), ("lens", _ptr), ("take", _ptr), ("take_stride", _i64),
-    ("count", _ptr), ("lens_out", _ptr), ("status", _ptr)])
+
+class VerifyArgs(ctypes.Structure):
+    _fields_ = [("batch", _i64), ("nodes", _i64), ("vocab", _i64), ("dtype", _i64), ("target", _ptr),
+                ("target_stride", _i64 * 2), ("draft", _ptr), ("draft_stride", _i64 * 2), ("tokens", _ptr),
+                ("tokens_bytes", _i64), ("tokens_stride", _i64), ("parents", _ptr), ("parents_stride", _i64),
+                ("uniforms", _ptr), ("uniforms_stride", _i64), ("noise", _ptr), ("noise_stride", _i64), ("path", _ptr),
+                ("count", _ptr), ("next_token", _ptr), ("status", _ptr)]
+
+
+class AppendArgs(ctypes.Structure):
+    _fields_ = [("batch", _i64), ("heads_kv", _i64), ("tokens", _i64), ("head_dim", _i64), ("dtype", _i64),
+                ("num_pages", _i64), ("page_size", _i64), ("max_pages", _i64), ("k", Tensor), ("v", Tensor),
+                ("k_pages", Tensor), ("v_pages", Tensor), ("page_table", _ptr), ("page_table_stride", _i64),
+                ("lens", _ptr), ("take", _ptr), ("take_stride", _i64), ("count", _ptr), ("lens_out", _ptr),
+                ("status", _ptr)]
 
 
 _lib = None
@@ -156,12 +144,12 @@ def load() -> ctypes.CDLL:
         lib.bfa_merge_partial.argtypes = [ctypes.c_int32] * 4 + [
             Tensor, ctypes.c_int32, ctypes.c_void_p, Tensor, ctypes.c_int32, ctypes.c_void_p,
             ctypes.c_void_p]
-        # Packed argument blocks travel as bytes objects (a read-only pointer to them).
-        for name in ("bfa_rope", "bfa_tree_fwd", "bfa_verify_tree", "bfa_cache_append"):
+        for name, args in (("bfa_rope", RopeArgs), ("bfa_tree_fwd", TreeArgs), ("bfa_verify_tree", VerifyArgs),
+                           ("bfa_cache_append", AppendArgs)):
             fn = getattr(lib, name)
-            fn.restype, fn.argtypes = ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]
+            fn.restype, fn.argtypes = ctypes.c_int, [ctypes.POINTER(args), ctypes.c_void_p]
         lib.bfa_tree_workspace_bytes.restype = ctypes.c_size_t
-        lib.bfa_tree_workspace_bytes.argtypes = [ctypes.c_char_p]
+        lib.bfa_tree_workspace_bytes.argtypes = [ctypes.POINTER(TreeArgs)]
         ver = lib.bfa_abi_version()
         if ver != ABI_VERSION:
             raise RuntimeError(f"libbfa ABI version {ver}, expected {ABI_VERSION}")
@@ -199,66 +187,6 @@ def tensor(t: torch.Tensor | None) -> Tensor:
     return out
 
 
-def flat(t: torch.Tensor | None) -> tuple:
-    """A [B, H, S, D] tensor's pointer and strides, as the packers take them."""
-    return (0, 0, 0, 0, 0) if t is None else (t.data_ptr(), *t.stride())
-
-
-def require_cuda(what: str, tensors, device=None) -> None:
-    """Every tensor is on one CUDA device (`device`, or the first one's)."""
-    for t in tensors:
-        if not t.is_cuda:
-            raise RuntimeError(f"{what} (B200 build) needs CUDA tensors; there is no CPU path")
-        if device is None:
-            device = t.device
-        elif t.device != device:
-            raise RuntimeError(f"{what}: tensors on {device} and {t.device}; they must share a device")
-
-
-CHECK_STATUS = os.environ.get("BFA_CHECK_STATUS", "0") == "1"
-_functions = {}
-
-
-def launch(name: str, packed: bytes, device: torch.device) -> None:
-    """One entry point that takes a packed argument block, on the device's
-    current stream. The tensors exist, so CUDA is initialised and the raw
-    calls (current device, current stream's handle) need no guard of torch's;
-    a decoding step makes a few such calls per layer, and their host time is
-    what it waits for."""
-    fn = _functions.get(name)
-    if fn is None:
-        fn = _functions[name] = getattr(load(), name)
-    index = device.index
-    if torch._C._cuda_getDevice() == index:
-        rc = fn(packed, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(device):
-            rc = fn(packed, torch._C._cuda_getCurrentRawStream(index))
-    if rc:
-        check(rc)
-    if CHECK_STATUS:
-        check(read_and_clear_status(device))
-
-
-_status_at = {}
-
-
-def status_ptr(device: torch.device) -> int:
-    """Address of the device's status word."""
-    at = _status_at.get(device.index)
-    if at is None:
-        at = _status_at[device.index] = status_word(device).data_ptr()
-    return at
-
-
-@functools.lru_cache(maxsize=4096)
-def tree_workspace_bytes(index: int, *sizes) -> int:
-    """bfa_tree_workspace_bytes of a device and the sizes that open a
-    bfa_tree_args block (batch ... soft_cap); it depends on nothing else."""
-    with torch.cuda.device(index):
-        return load().bfa_tree_workspace_bytes(pack_tree(*sizes, *[0] * (_TREE_VALUES - len(sizes))))
-
-
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
@@ -280,3 +208,20 @@ def read_and_clear_status(device: torch.device) -> int:
     val = int(w.item())
     w.zero_()
     return val
+
+
+def status_ptr(index: int) -> int:
+    """Address of device `index`'s status word (for bfa_torch, which asks once)."""
+    return status_word(torch.device("cuda", index)).data_ptr()
+
+
+def binding():
+    """bfa_torch, the compiled PyTorch side of the rotary and tree-decoding
+    operators. Like the library itself it has no stand-in: without it, raise."""
+    load()
+    try:
+        import bfa_torch
+    except ImportError as e:
+        raise RuntimeError(f"{os.path.join(HERE, 'bfa_torch.so')} is missing or does not load ({e}); build it with "
+                           f"`python {HERE}/build.py`") from e
+    return bfa_torch

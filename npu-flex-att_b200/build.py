@@ -1,4 +1,6 @@
-"""Build libbfa.so (the C-ABI attention library) for sm_100a with nvcc.
+"""Build libbfa.so (the C-ABI attention library) for sm_100a with nvcc, and
+bfa_torch.so (the PyTorch side of the rotary and tree-decoding operators) with
+the host compiler.
 
 Usage: python build.py [--force] [--jobs N]
 
@@ -21,6 +23,9 @@ CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libbfa.so")
+BINDING = os.path.join(HERE, "bfa_torch.so")
+BINDING_SRC = os.path.join(CSRC, "torch_binding.cpp")
+CXX = "g++"  # the compiler nvcc calls too: its libstdc++ is the shared one that torch uses
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
@@ -32,7 +37,7 @@ def sources():
 
 
 def _deps_mtime():
-    paths = [os.path.join(CSRC, f) for f in os.listdir(CSRC)]
+    paths = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".h", ".cuh"))]
     paths += [os.path.join(INCLUDE, f) for f in os.listdir(INCLUDE)]
     return max(os.path.getmtime(p) for p in paths)
 
@@ -47,6 +52,32 @@ def compile_one(src: str, force: bool) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"nvcc failed for {src}:\n{r.stdout}\n{r.stderr}")
     return obj
+
+
+def build_binding(force: bool = False, verbose: bool = True) -> str:
+    """bfa_torch.so, a CPython module against this Python's torch and libbfa.so's
+    C ABI (found next to it)."""
+    deps = [BINDING_SRC, os.path.join(INCLUDE, "bfa.h")]
+    if not force and os.path.exists(BINDING) and os.path.getmtime(BINDING) >= max(map(os.path.getmtime, deps)):
+        return BINDING
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cuda = os.path.dirname(os.path.dirname(NVCC))
+    inc = [x for d in [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda, "include"), INCLUDE]
+           for x in ("-isystem" if d != INCLUDE else "-I", d)]
+    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=bfa_torch",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *inc,
+           BINDING_SRC, "-o", BINDING, "-L", HERE, "-lbfa", "-Wl,-rpath,$ORIGIN", "-L", lib, "-lc10", "-lc10_cuda",
+           "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python", f"-Wl,-rpath,{lib}",
+           "-L", os.path.join(cuda, "lib64"), "-lcudart"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{CXX} failed for {BINDING_SRC}:\n{r.stdout}\n{r.stderr}")
+    if verbose:
+        print("built", BINDING)
+    return BINDING
 
 
 def build(force: bool = False, jobs: int | None = None, verbose: bool = True) -> str:
@@ -64,6 +95,7 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = True) ->
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         if verbose:
             print("built", LIB)
+    build_binding(force, verbose)
     return LIB
 
 

@@ -11,23 +11,19 @@
 namespace bfa {
 namespace {
 
-// Rows of an item per merge block: one where four warps share a row (few
-// items: all their rows at once), else 16.
-constexpr int merge_rows(int warps) { return warps == 4 ? 1 : 16; }
 
 // Joins the partial (O, LSE) of items that several blocks worked on, partials
 // in the order of their keys:
 //   lse = log2 sum_i 2^lse_i,  O = sum_i O_i·2^(lse_i - lse).
 // An item that one block did whole is already final, and its merge blocks
-// leave at once. kWarps warps take a row: each sums every kWarps-th partial,
+// leave at once. A block has kMergeRows rows of an item, kWarps warps take a row: each sums every kWarps-th partial,
 // eight loads in flight, and the first adds the warps' sums in order. One warp
 // where an item has few partials (many items), four where a few items are
 // spread over the GPU. kVec: columns per lane and load (4 where D allows it,
 // else 1). Launched to start under the attention kernel's tail: what it needs
 // of the inputs alone comes before it waits for the partials.
-template <typename T, int kWarps, int kVec>
+template <typename T, int kWarps, int kVec, int kMergeRows>
 __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeParams p) {
-  constexpr int kMergeRows = merge_rows(kWarps);
   constexpr int kLoads = kVec == 4 ? 2 : 8;  // of 32·kVec columns: 256
   __shared__ float part[4][kVec * kLoads * 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % kWarps;
@@ -36,12 +32,19 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeParams p) {
   const int item_all = blockIdx.x / per_item, row0 = (blockIdx.x - item_all * per_item) * kMergeRows;
   const int b = item_all / (p.Hkv * p.n_rb), item = item_all - b * p.Hkv * p.n_rb;
   const int hkv = item / p.n_rb, rb0 = (item - hkv * p.n_rb) * p.rb;
-  int64_t s0;
-  const int64_t total_chunks = tree_total(p, b, &s0);
   const int len = tree_len(p, b), n_chunks = tree_chunks_of(p, len);
-  s0 += (int64_t)item * n_chunks;
-  const int blocks = tree_blocks(p, total_chunks);
-  const int i0 = tree_owner(total_chunks, blocks, s0), i1 = tree_owner(total_chunks, blocks, s0 + n_chunks - 1);
+  int i0, i1;
+  auto owners = [&](auto zero) {
+    using I = decltype(zero);
+    I s0;
+    const I T_all = tree_total<I>(p, b, &s0);
+    s0 += (I)item * n_chunks;
+    const I blocks = tree_blocks<I>(p, T_all);
+    i0 = tree_owner<I>(T_all, blocks, s0);
+    i1 = tree_owner<I>(T_all, blocks, s0 + n_chunks - 1);
+  };
+  if (p.small) owners(uint32_t{0});
+  else owners(int64_t{0});
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (i0 == i1) return;
   for (int rr = warp / kWarps; rr < kMergeRows; rr += 4 / kWarps) {
@@ -148,6 +151,7 @@ int check_tree(const bfa_tree_args* a) {
 struct Plan {
   int rb, n_rb, chunk, tree_chunks, grid;
   size_t lse_at, bytes;
+  bool small;
 };
 
 Plan make_plan(const bfa_tree_args* a, const TreeTile& tile) {
@@ -162,6 +166,7 @@ Plan make_plan(const bfa_tree_args* a, const TreeTile& tile) {
   if (a->sliding_window > 0) seen = std::min(seen, a->sliding_window + pl.chunk);
   const int64_t chunks = ((seen + pl.chunk - 1) / pl.chunk + pl.tree_chunks) * a->batch * a->heads_kv * pl.n_rb;
   pl.grid = (int)std::min<int64_t>(chunks, (int64_t)sm_count() * tile.per_sm);
+  pl.small = chunks < ((int64_t)1 << 31) / (pl.grid + 1);
   const size_t rows_ws = (size_t)pl.grid * 2 * pl.rb;
   pl.lse_at = (rows_ws * a->head_dim * 4 + 255) / 256 * 256;
   pl.bytes = pl.lse_at + (rows_ws * 4 + 255) / 256 * 256;
@@ -193,10 +198,12 @@ size_t workspace_bytes(const bfa_tree_args* a) {
 template <typename T>
 int launch_merge(const TreeParams& p, cudaStream_t st) {
   const int64_t items = (int64_t)p.B * p.Hkv * p.n_rb;
-  // Four warps per row where an item is spread over at least four blocks on average.
+  // Four warps per row where an item is spread over at least four blocks on
+  // average; a warp per row while all rows' warps fit the GPU at once (16
+  // blocks of 128 threads an SM), four rows a warp, one after another, above.
   const bool wide = p.grid >= 4 * items;
+  const int rows = wide ? 1 : items * std::min(p.rb, p.G * p.N) <= (int64_t)sm_count() * 64 ? 4 : 16;
   cudaLaunchConfig_t cfg{};
-  const int rows = merge_rows(wide ? 4 : 1);
   cfg.gridDim = dim3((unsigned)(items * ((std::min(p.rb, p.G * p.N) + rows - 1) / rows)));
   cfg.blockDim = dim3(128);
   cfg.stream = st;
@@ -205,8 +212,9 @@ int launch_merge(const TreeParams& p, cudaStream_t st) {
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  auto kernel = p.D % 4 == 0 ? (wide ? tree_merge_kernel<T, 4, 4> : tree_merge_kernel<T, 1, 4>)
-                             : (wide ? tree_merge_kernel<T, 4, 1> : tree_merge_kernel<T, 1, 1>);
+  auto kernel = p.D % 4 == 0
+                    ? (wide ? tree_merge_kernel<T, 4, 4, 1> : rows == 4 ? tree_merge_kernel<T, 1, 4, 4> : tree_merge_kernel<T, 1, 4, 16>)
+                    : (wide ? tree_merge_kernel<T, 4, 1, 1> : rows == 4 ? tree_merge_kernel<T, 1, 1, 4> : tree_merge_kernel<T, 1, 1, 16>);
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -263,6 +271,8 @@ extern "C" int bfa_tree_fwd(const bfa_tree_args* a, void* stream) {
   p.scale = (float)a->scale;
   p.soft_cap = (float)a->soft_cap;
   p.grid = pl.grid; p.rb = pl.rb; p.n_rb = pl.n_rb; p.chunk = pl.chunk; p.tree_chunks = pl.tree_chunks;
+  p.chunk_log2 = pl.chunk == 128 ? 7 : pl.chunk == 64 ? 6 : 5;
+  p.small = pl.small;
   p.part_o = static_cast<float*>(a->workspace);
   p.part_lse = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + pl.lse_at);
   cudaStream_t st = (cudaStream_t)stream;

@@ -33,7 +33,8 @@ struct TreeParams {
   int B, Hq, Hkv, G, N, D, page, cap_tokens;  // cap_tokens: max_pages·page_size
   int window;
   float scale, soft_cap;
-  int grid, rb, n_rb, chunk, tree_chunks;
+  int grid, rb, n_rb, chunk, chunk_log2, tree_chunks;
+  bool small;  // grid times the number of chunks fits 32 bits (a bound of the host's)
   float* part_o;    // [grid][2][rb][D]: slot 0 an item begun by an earlier block, slot 1 one left to a later
   float* part_lse;  // [grid][2][rb], base 2, without the ALiBi row constant
 };
@@ -45,17 +46,27 @@ __device__ __forceinline__ int tree_len(const TreeParams& p, int b) {
 // sees keys j >= len - W (deeper nodes see less), rounded down to a whole
 // chunk, so that chunks start at multiples of their length.
 __device__ __forceinline__ int tree_lo(const TreeParams& p, int len) {
-  return p.window > 0 ? max(0, len - p.window) / p.chunk * p.chunk : 0;
+  return p.window > 0 ? max(0, len - p.window) >> p.chunk_log2 << p.chunk_log2 : 0;
 }
 __device__ __forceinline__ int tree_chunks_of(const TreeParams& p, int len) {
-  return (len - tree_lo(p, len) + p.chunk - 1) / p.chunk + p.tree_chunks;
+  return ((len - tree_lo(p, len) + p.chunk - 1) >> p.chunk_log2) + p.tree_chunks;
 }
 
+// Counts of chunks: 32 bits (p.small) or 64.
 // Of `grid` blocks, those that have work: every one of them at least a chunk.
-__device__ __forceinline__ int tree_blocks(const TreeParams& p, int64_t T) { return (int)(T < p.grid ? T : p.grid); }
+template <typename I>
+__device__ __forceinline__ I tree_blocks(const TreeParams& p, I T) {
+  return T < (I)p.grid ? T : (I)p.grid;
+}
 // Where block i's stretch of T chunks begins, and which block holds chunk x.
-__device__ __forceinline__ int64_t tree_start(int64_t T, int grid, int64_t i) { return i * T / grid; }
-__device__ __forceinline__ int tree_owner(int64_t T, int grid, int64_t x) { return (int)(((x + 1) * grid - 1) / T); }
+template <typename I>
+__device__ __forceinline__ I tree_start(I T, I blocks, I i) {
+  return i * T / blocks;
+}
+template <typename I>
+__device__ __forceinline__ int tree_owner(I T, I blocks, I x) {
+  return (int)(((x + 1) * blocks - 1) / T);
+}
 
 // A position in the list of chunks.
 struct TreeCursor {
@@ -85,10 +96,11 @@ struct TreeCursor {
   }
 };
 
-// Chunks of all sequences' items, and of those before sequence b (b < 0: not
-// asked for); every lane of a warp calls it.
-__device__ __forceinline__ int64_t tree_total(const TreeParams& p, int b, int64_t* before) {
-  int64_t n = 0, m = 0;
+// Chunks of all sequences' items, and of those before sequence b; every lane
+// of a warp calls it.
+template <typename I>
+__device__ __forceinline__ I tree_total(const TreeParams& p, int b, I* before) {
+  I n = 0, m = 0;
   for (int i = threadIdx.x & 31; i < p.B; i += 32) {
     const int c = tree_chunks_of(p, tree_len(p, i));
     n += c;
@@ -99,55 +111,64 @@ __device__ __forceinline__ int64_t tree_total(const TreeParams& p, int b, int64_
     n += __shfl_xor_sync(0xffffffffu, n, o);
     m += __shfl_xor_sync(0xffffffffu, m, o);
   }
-  *before = m * p.Hkv * p.n_rb;
-  return n * p.Hkv * p.n_rb;
+  const I per = p.Hkv * p.n_rb;
+  *before = m * per;
+  return n * per;
 }
 
-// This block's stretch: `cur` at its first chunk, returns its number of chunks
-// (0: none). Every lane of a warp calls it; one pass over the lengths where a
-// lane each holds them.
-__device__ __forceinline__ int tree_stretch(const TreeParams& p, TreeCursor& cur) {
+template <typename I>
+__device__ __forceinline__ int tree_stretch_in(const TreeParams& p, TreeCursor& cur) {
   const int lane = threadIdx.x & 31;
-  const int per = p.Hkv * p.n_rb;
-  int64_t T = 0, before = 0, x = 0, end = 0;
+  const I per = p.Hkv * p.n_rb;
+  I T = 0, before = 0, x = 0, end = 0;
   for (int pass = p.B > 32 ? 0 : 1; pass < 2; ++pass) {
     // Pass 0 (more than 32 sequences): the total. Pass 1: 32 sequences at a
     // time, a prefix sum over the warp finds the sequence of chunk x.
     for (int b0 = 0; b0 < p.B; b0 += 32) {
-      const int64_t mine = b0 + lane < p.B ? (int64_t)tree_chunks_of(p, tree_len(p, b0 + lane)) * per : 0;
-      int64_t sum = mine;
+      const int len = b0 + lane < p.B ? tree_len(p, b0 + lane) : 0;
+      const I mine = b0 + lane < p.B ? (I)tree_chunks_of(p, len) * per : 0;
+      I sum = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, sum, o);
+        const I y = __shfl_up_sync(0xffffffffu, sum, o);
         if (lane >= o) sum += y;
       }
-      const int64_t all = __shfl_sync(0xffffffffu, sum, 31);
+      const I all = __shfl_sync(0xffffffffu, sum, 31);
       if (pass == 0) {
         T += all;
         continue;
       }
       if (b0 == 0) {
         if (p.B <= 32) T = all;
-        const int blocks = tree_blocks(p, T);
-        if ((int)blockIdx.x >= blocks) return 0;
-        x = tree_start(T, blocks, blockIdx.x);
-        end = tree_start(T, blocks, blockIdx.x + 1);
+        const I blocks = tree_blocks<I>(p, T);
+        if ((I)blockIdx.x >= blocks) return 0;
+        x = tree_start<I>(T, blocks, blockIdx.x);
+        end = tree_start<I>(T, blocks, blockIdx.x + 1);
       }
       const unsigned m = __ballot_sync(0xffffffffu, before + sum > x);
       if (m) {
         const int l = __ffs(m) - 1;
         cur.b = b0 + l;
+        cur.len = __shfl_sync(0xffffffffu, len, l);
         before += __shfl_sync(0xffffffffu, sum - mine, l);
         break;
       }
       before += all;
     }
   }
-  cur.load(p);
+  cur.lo = tree_lo(p, cur.len);
+  cur.n = tree_chunks_of(p, cur.len);
   const int in = (int)(x - before);  // within one sequence: fits 32 bits (checked by the host)
   cur.item = in / cur.n;
   cur.c = in - cur.item * cur.n;
   return (int)(end - x);
+}
+
+// This block's stretch: `cur` at its first chunk, returns its number of chunks
+// (0: none). Every lane of a warp calls it; one pass over the lengths where a
+// lane each holds them.
+__device__ __forceinline__ int tree_stretch(const TreeParams& p, TreeCursor& cur) {
+  return p.small ? tree_stretch_in<uint32_t>(p, cur) : tree_stretch_in<int64_t>(p, cur);
 }
 
 // The rows of K and V that key j of a chunk lies in (null reads as zeros).

@@ -164,11 +164,32 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
     // Lane i·kSub + s: columns [64s, 64s + 64) of box i, tokens [key0 + i·box,
     // + box) of one page (the tree's chunk: one box of 64 nodes).
     const int my_box = lane / L::kSub, my_sub = lane % L::kSub;
+    // The sequence's page table, 64 entries at a time: lane i holds entries
+    // wb + i and wb + 32 + i; the second half is loaded 32 pages before it is
+    // used.
+    int wb = 0, wseq = -1, w0 = 0, w1 = 0;
+    auto entry = [&](const TreeCursor& at, int pg) {
+      return (int64_t)pg * p.page < at.len ? p.table[at.b * p.table_stride + pg] : 0;
+    };
+    auto fill = [&](const TreeCursor& at) {
+      if (at.in_tree(p)) return;
+      const int pg = at.key0(p) / p.page;
+      if (at.b != wseq || pg < wb || pg >= wb + 64) {
+        wseq = at.b;
+        wb = pg;
+        w0 = entry(at, wb + lane);
+        w1 = entry(at, wb + 32 + lane);
+      } else if (pg >= wb + 32) {
+        w0 = w1;
+        wb += 32;
+        w1 = entry(at, wb + 32 + lane);
+      }
+    };
     struct Box {
       int page, slot;
       bool mine;
     };
-    auto lookup = [&](const TreeCursor& at) -> Box {
+    auto find = [&](const TreeCursor& at) -> Box {
       Box r{0, 0, false};
       if (at.in_tree(p)) {
         r.mine = my_box == 0;
@@ -176,22 +197,23 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
       }
       const int t0 = at.key0(p) + my_box * box;
       r.mine = my_box < CH / box && t0 < at.len;
-      if (r.mine) {
-        const int pg = t0 / p.page;
-        r.slot = t0 - pg * p.page;
-        r.page = p.table[at.b * p.table_stride + pg];
+      const int pg = r.mine ? t0 / p.page : wb;
+      r.slot = t0 - pg * p.page;
+      r.page = __shfl_sync(0xffffffffu, w0, pg - wb);  // the lane is taken modulo 32
+      if (__any_sync(0xffffffffu, pg - wb >= 32)) {
+        const int v = __shfl_sync(0xffffffffu, w1, pg - wb);
+        if (pg - wb >= 32) r.page = v;
       }
       return r;
     };
     bool ok = true;
     int n = 0;
-    Box next{0, 0, false};
-    if (n_x > 0) next = lookup(cur);
+    if (n_x > 0) fill(cur);
     for (int x = 0; x < n_x && ok; ++x) {
-      Box me = next;
+      Box me = find(cur);
       const TreeCursor here = cur;
       cur.next(p);
-      if (x + 1 < n_x) next = lookup(cur);  // in flight while this chunk's slots are waited for
+      if (x + 1 < n_x) fill(cur);  // in flight while this chunk's slots are waited for
       const bool tree = here.in_tree(p);
       const int hkv = here.item / p.n_rb;
       if (!tree && me.mine && (me.page < 0 || me.page >= p.num_pages)) {

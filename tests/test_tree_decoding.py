@@ -14,7 +14,7 @@ import tree_decoding as td
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
-def test_packed_blocks_match_header_layout(tmp_path):
+def test_argument_blocks_match_header_layout(tmp_path):
     if shutil.which("gcc") is None:
         pytest.skip("gcc not available")
     structs = {"bfa_rope_args": bfa_lib.RopeArgs, "bfa_tree_args": bfa_lib.TreeArgs, "bfa_verify_args": bfa_lib.VerifyArgs,
@@ -38,7 +38,7 @@ def block(cls, **kw):
     a = cls()
     for key, x in kw.items():
         setattr(a, key, x)
-    return bytes(a)
+    return a
 
 
 TREE = dict(batch=1, heads_q=4, heads_kv=2, nodes=3, head_dim=64, dtype=2, num_pages=1, page_size=16, max_pages=1)
