@@ -11,10 +11,10 @@
 //
 // Split. A unit is what one thread holds of a row: two 16-byte vectors that
 // make whole pairs (half layout), or one (interleaved, and the copied dims).
-// A thread keeps its unit's cos/sin in registers and goes over kHeads heads,
-// all loads before the first store, so that kHeads·2 vectors are in flight per
-// thread. kHeads is 4 where that still fills the GPU and 1 below (a decoding
-// step, where the launch's latency is all there is). Rows that 16-byte vectors
+// A thread keeps its unit's cos/sin in registers and goes over a span of heads,
+// kHeads at a time, all loads before the first store, so that kHeads·2 vectors
+// are in flight per thread. kHeads is 4 where that still fills the GPU and 1
+// below (a decoding step, where the launch's latency is all there is). Rows that 16-byte vectors
 // cannot address (strides, alignment, R/2 not a multiple of the vector) take
 // the element-wise form of the same kernel.
 #include <cuda_runtime.h>
@@ -36,6 +36,7 @@ struct RopeParams {
   int64_t pos_s[2];
   int pos_bytes, off_bytes;
   int B, Hq, Hk, S, D, R, units;
+  int span;  // heads of a thread
   float sign;  // of sin: -1 for the transposed rotation
   int32_t* status;
 };
@@ -62,6 +63,21 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& r) {
   else *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(r.x);
 }
 
+// kPairs consecutive table entries, in vectors where the rows allow it (V > 1).
+template <int V, int kPairs>
+__device__ __forceinline__ void load_table(float (&f)[kPairs], const float* p) {
+  if constexpr (V > 1 && kPairs % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < kPairs; i += 4) *reinterpret_cast<float4*>(f + i) = __ldg(reinterpret_cast<const float4*>(p + i));
+  } else if constexpr (V > 1 && kPairs % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < kPairs; i += 2) *reinterpret_cast<float2*>(f + i) = __ldg(reinterpret_cast<const float2*>(p + i));
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) f[i] = __ldg(p + i);
+  }
+}
+
 // V: elements per vector access (1: element-wise, any strides).
 template <typename T, bool IL, int V, int kHeads>
 __global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
@@ -79,55 +95,59 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
   const int d0 = !turn ? p.R + (u - n_turn) * V : IL ? u * kTurn : u * V;
   const int d1 = IL ? d0 + 1 : d0 + p.R / 2;
   const int H = p.Hq + p.Hk;
-  const int h0 = blockIdx.y * kHeads;
+  const int first = blockIdx.y * p.span, last = min(first + p.span, H);
 
   for (int b = blockIdx.z; b < p.B; b += gridDim.z) {
-    float c[kPairs], sn[kPairs];
+    alignas(16) float c[kPairs], sn[kPairs];
     if (turn) {
       int64_t t = p.pos ? load_index(p.pos, p.pos_bytes, b * p.pos_s[0] + s * p.pos_s[1]) : s;
       if (p.off) t += load_index(p.off, p.off_bytes, b);
       const bool ok = t >= 0 && t < p.rows;
       if (!ok && p.status) *p.status = BFA_ERR_INDEX;
       const int64_t at = (ok ? t : 0) * p.table_stride + u * kPairs;
+      load_table<V, kPairs>(c, p.cos + at);
+      load_table<V, kPairs>(sn, p.sin + at);
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) {
-        c[i] = ok ? p.cos[at + i] : __int_as_float(0x7fc00000);
-        sn[i] = ok ? p.sin[at + i] * p.sign : __int_as_float(0x7fc00000);
+        c[i] = ok ? c[i] : __int_as_float(0x7fc00000);
+        sn[i] = ok ? sn[i] * p.sign : __int_as_float(0x7fc00000);
       }
     }
-    Pack<T, V> x0[kHeads], x1[kHeads];
+    for (int h0 = first; h0 < last; h0 += kHeads) {
+      Pack<T, V> x0[kHeads], x1[kHeads];
 #pragma unroll
-    for (int j = 0; j < kHeads; ++j) {
-      const int h = h0 + j;
-      if (h < H) {
-        const bool isq = h < p.Hq;
-        const int64_t* st = isq ? p.sq : p.sk;
-        const T* base = static_cast<const T*>(isq ? p.q : p.k) + b * st[0] + (int64_t)(isq ? h : h - p.Hq) * st[1] + s * st[2];
-        const int64_t sd = V > 1 ? 1 : st[3];
-        x0[j] = load_pack<T, V>(base + d0 * sd);
-        if (kTwo && turn) x1[j] = load_pack<T, V>(base + d1 * sd);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < kHeads; ++j) {
-      const int h = h0 + j;
-      if (h < H) {
-        const bool isq = h < p.Hq;
-        const int64_t* st = isq ? p.sqo : p.sko;
-        T* base = static_cast<T*>(isq ? p.qo : p.ko) + b * st[0] + (int64_t)(isq ? h : h - p.Hq) * st[1] + s * st[2];
-        const int64_t sd = V > 1 ? 1 : st[3];
-        if (turn) {
-#pragma unroll
-          for (int i = 0; i < kPairs; ++i) {
-            T& ra = kTwo ? x0[j].x[i] : x0[j].x[(2 * i) % V];
-            T& rb = kTwo ? x1[j].x[i] : x0[j].x[(2 * i + 1) % V];
-            const float a = to_f32(ra), bb = to_f32(rb);
-            ra = from_f32<T>(a * c[i] - bb * sn[i]);
-            rb = from_f32<T>(a * sn[i] + bb * c[i]);
-          }
+      for (int j = 0; j < kHeads; ++j) {
+        const int h = h0 + j;
+        if (h < last) {
+          const bool isq = h < p.Hq;
+          const int64_t* st = isq ? p.sq : p.sk;
+          const T* base = static_cast<const T*>(isq ? p.q : p.k) + b * st[0] + (int64_t)(isq ? h : h - p.Hq) * st[1] + s * st[2];
+          const int64_t sd = V > 1 ? 1 : st[3];
+          x0[j] = load_pack<T, V>(base + d0 * sd);
+          if (kTwo && turn) x1[j] = load_pack<T, V>(base + d1 * sd);
         }
-        store_pack<T, V>(base + d0 * sd, x0[j]);
-        if (kTwo && turn) store_pack<T, V>(base + d1 * sd, x1[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < kHeads; ++j) {
+        const int h = h0 + j;
+        if (h < last) {
+          const bool isq = h < p.Hq;
+          const int64_t* st = isq ? p.sqo : p.sko;
+          T* base = static_cast<T*>(isq ? p.qo : p.ko) + b * st[0] + (int64_t)(isq ? h : h - p.Hq) * st[1] + s * st[2];
+          const int64_t sd = V > 1 ? 1 : st[3];
+          if (turn) {
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) {
+              T& ra = kTwo ? x0[j].x[i] : x0[j].x[(2 * i) % V];
+              T& rb = kTwo ? x1[j].x[i] : x0[j].x[(2 * i + 1) % V];
+              const float a = to_f32(ra), bb = to_f32(rb);
+              ra = from_f32<T>(a * c[i] - bb * sn[i]);
+              rb = from_f32<T>(a * sn[i] + bb * c[i]);
+            }
+          }
+          store_pack<T, V>(base + d0 * sd, x0[j]);
+          if (kTwo && turn) store_pack<T, V>(base + d1 * sd, x1[j]);
+        }
       }
     }
   }
@@ -147,10 +167,15 @@ int launch_rope(RopeParams& p, bool in_place, cudaStream_t st) {
   const int64_t per_head = (int64_t)p.S * p.units;
   if (per_head > INT32_MAX - 256) return BFA_ERR_UNSUPPORTED;
   const int H = p.Hq + p.Hk;
-  // Four heads per thread where that leaves at least two full waves of threads.
-  const bool four = per_head * p.B * ((H + 3) / 4) >= (int64_t)sm_count() * 2048 * 2;
+  // Four heads in flight per thread where that leaves a full wave of threads,
+  // and more of them, one group of four after another (the table's values stay
+  // in registers), while two waves remain.
+  const int64_t wave = (int64_t)sm_count() * 2048;
+  const bool four = per_head * p.B * ((H + 3) / 4) >= wave;
+  p.span = four ? 4 : 1;
+  while (four && p.span < H && per_head * p.B * ((H + 2 * p.span - 1) / (2 * p.span)) >= 2 * wave) p.span *= 2;
   const int threads = (int)std::min<int64_t>(256, (per_head + 31) / 32 * 32);
-  const int heads = four ? (H + 3) / 4 : H;
+  const int heads = (H + p.span - 1) / p.span;
   if (heads > 65535) return BFA_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)((per_head + threads - 1) / threads), (unsigned)heads, (unsigned)std::min(p.B, 65535));
   if (four) rope_kernel<T, IL, V, 4><<<grid, threads, 0, st>>>(p);
@@ -165,6 +190,7 @@ int launch_typed(RopeParams& p, const bfa_rope_args& a, cudaStream_t st) {
   const bool il = a.interleaved != 0;
   const bool in_place = same_place(a.q, a.q_out) && (a.heads_k == 0 || same_place(a.k, a.k_out));
   bool vec = p.R % (il ? E : 2 * E) == 0 && p.D % E == 0 && vector_rows(a.q, sizeof(T)) && vector_rows(a.q_out, sizeof(T));
+  vec = vec && (((uintptr_t)a.cos | (uintptr_t)a.sin) & 15u) == 0 && a.table_stride % 4 == 0;
   if (a.heads_k > 0) vec = vec && vector_rows(a.k, sizeof(T)) && vector_rows(a.k_out, sizeof(T));
   if (il) return vec ? launch_rope<T, true, E>(p, in_place, st) : launch_rope<T, true, 1>(p, in_place, st);
   return vec ? launch_rope<T, false, E>(p, in_place, st) : launch_rope<T, false, 1>(p, in_place, st);
@@ -185,7 +211,7 @@ extern "C" int bfa_rope(const bfa_rope_args* a, void* stream) {
     return BFA_ERR_UNSUPPORTED;
   const int64_t heads = a->heads_q + a->heads_k;
   if (a->batch == 0 || a->seqlen == 0 || heads == 0) return BFA_OK;
-  if (!a->cos || !a->sin || (a->heads_q > 0 && (!a->q.data || !a->q_out.data)) ||
+  if (!a->cos || !a->sin || a->table_rows < 1 || (a->heads_q > 0 && (!a->q.data || !a->q_out.data)) ||
       (a->heads_k > 0 && (!a->k.data || !a->k_out.data)))
     return BFA_ERR_INVALID_ARGUMENT;
   if ((a->positions && a->positions_bytes != 4 && a->positions_bytes != 8) ||

@@ -271,6 +271,9 @@ extern "C" int bfa_tree_fwd(const bfa_tree_args* a, void* stream) {
   p.scale = (float)a->scale;
   p.soft_cap = (float)a->soft_cap;
   p.grid = pl.grid; p.rb = pl.rb; p.n_rb = pl.n_rb; p.chunk = pl.chunk; p.tree_chunks = pl.tree_chunks;
+  p.page_log2 = -1;
+  for (int i = 0; i < 31; ++i)
+    if (p.page == 1 << i) p.page_log2 = i;
   p.chunk_log2 = pl.chunk == 128 ? 7 : pl.chunk == 64 ? 6 : 5;
   p.small = pl.small;
   p.part_o = static_cast<float*>(a->workspace);

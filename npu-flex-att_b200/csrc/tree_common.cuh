@@ -31,6 +31,7 @@ struct TreeParams {
   int32_t* status;
   int64_t num_pages;
   int B, Hq, Hkv, G, N, D, page, cap_tokens;  // cap_tokens: max_pages·page_size
+  int page_log2;  // -1: no power of two
   int window;
   float scale, soft_cap;
   int grid, rb, n_rb, chunk, chunk_log2, tree_chunks;
@@ -187,7 +188,7 @@ __device__ __forceinline__ void tree_key_rows(const TreeParams& p, const TreeCur
     return;
   }
   if (key >= cur.len) return;
-  const int pg = key / p.page, slot = key - pg * p.page;
+  const int pg = p.page_log2 >= 0 ? key >> p.page_log2 : key / p.page, slot = key - pg * p.page;
   const int32_t page = p.table[cur.b * p.table_stride + pg];
   if (page < 0 || page >= p.num_pages) {
     if (p.status) *p.status = BFA_ERR_INDEX;

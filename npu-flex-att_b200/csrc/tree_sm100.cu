@@ -11,11 +11,10 @@
 //
 // Split. Persistent blocks, one per SM, each with an equal stretch of the list
 // of chunks (tree_common.cuh). Warp roles:
-//   warp 0      producer: looks a chunk's pages up one chunk ahead and loads K
-//               and V by TMA, a lane per box, into a ring that runs on across
-//               items
+//   warps 0, 2  producers of K and of V: find a chunk's pages and load it by
+//               TMA, a lane per box, into a ring that runs on across items
 //   warp 1      MMA issuer
-//   warp 2      TMEM allocator
+//   warp 2      also allocates TMEM
 //   warp 3      the tree's ancestor sets, one item ahead
 //   warps 4..   softmax, 8 warps per 128-row tile: two threads share a row (TMEM
 //               lane), each with half of the chunk's keys and of O's columns;
@@ -159,8 +158,9 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = mi.tmem;
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ producer
+  if (warp == 0 || warp == 2) {
+    // ------------------------------------------------------------ producers
+    const int kv = warp >> 1;
     // Lane i·kSub + s: columns [64s, 64s + 64) of box i, tokens [key0 + i·box,
     // + box) of one page (the tree's chunk: one box of 64 nodes).
     const int my_box = lane / L::kSub, my_sub = lane % L::kSub;
@@ -171,9 +171,10 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
     auto entry = [&](const TreeCursor& at, int pg) {
       return (int64_t)pg * p.page < at.len ? p.table[at.b * p.table_stride + pg] : 0;
     };
+    auto page_of = [&](int token) { return p.page_log2 >= 0 ? token >> p.page_log2 : token / p.page; };
     auto fill = [&](const TreeCursor& at) {
       if (at.in_tree(p)) return;
-      const int pg = at.key0(p) / p.page;
+      const int pg = page_of(at.key0(p));
       if (at.b != wseq || pg < wb || pg >= wb + 64) {
         wseq = at.b;
         wb = pg;
@@ -197,7 +198,7 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
       }
       const int t0 = at.key0(p) + my_box * box;
       r.mine = my_box < CH / box && t0 < at.len;
-      const int pg = r.mine ? t0 / p.page : wb;
+      const int pg = r.mine ? page_of(t0) : wb;
       r.slot = t0 - pg * p.page;
       r.page = __shfl_sync(0xffffffffu, w0, pg - wb);  // the lane is taken modulo 32
       if (__any_sync(0xffffffffu, pg - wb >= 32)) {
@@ -207,7 +208,7 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
       return r;
     };
     bool ok = true;
-    int n = 0;
+    int n = kv;
     if (n_x > 0) fill(cur);
     for (int x = 0; x < n_x && ok; ++x) {
       Box me = find(cur);
@@ -221,26 +222,29 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
         if (p.status) *p.status = BFA_ERR_INDEX;
       }
       const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xffffffffu, me.mine)) * (tree ? 64 : box) * 128u;
-      for (int kv = 0; kv < 2; ++kv, ++n) {
-        const int st = n % NS;
-        if (n >= NS) {
-          int w = 1;
-          if (lane == 0) w = mbar_wait(bar(kKVEmpty + st), ((n / NS) & 1) ^ 1, ctl, BFA_ERR_DEVICE_TIMEOUT) ? 1 : 0;
-          ok = __shfl_sync(0xffffffffu, w, 0) != 0;
-          if (!ok) break;
-        }
-        if (lane == 0) mbar_arrive_expect_tx(bar(kKVFull + st), bytes);
-        __syncwarp();
-        if (me.mine) {
-          const uint32_t dst = sbase + L::kOffKV + st * L::kKV + my_sub * (CH * 128) + my_box * box * 128;
-          if (tree) tma_load_4d(dst, kv ? &tmV : &tmK, bar(kKVFull + st), my_sub * 64, 0, hkv, here.b);
-          else tma_load_4d(dst, kv ? &tmVp : &tmKp, bar(kKVFull + st), my_sub * 64, me.slot, hkv, me.page);
-        }
-        __syncwarp();
+      n = 2 * x + kv;
+      const int st = n % NS;
+      if (n >= NS) {
+        int w = 1;
+        if (lane == 0) w = mbar_wait(bar(kKVEmpty + st), ((n / NS) & 1) ^ 1, ctl, BFA_ERR_DEVICE_TIMEOUT) ? 1 : 0;
+        ok = __shfl_sync(0xffffffffu, w, 0) != 0;
+        if (!ok) break;
       }
+      if (lane == 0) mbar_arrive_expect_tx(bar(kKVFull + st), bytes);
+      __syncwarp();
+      if (me.mine) {
+        const uint32_t dst = sbase + L::kOffKV + st * L::kKV + my_sub * (CH * 128) + my_box * box * 128;
+        if (tree) tma_load_4d(dst, kv ? &tmV : &tmK, bar(kKVFull + st), my_sub * 64, 0, hkv, here.b);
+        else tma_load_4d(dst, kv ? &tmVp : &tmKp, bar(kKVFull + st), my_sub * 64, me.slot, hkv, me.page);
+      }
+      __syncwarp();
+      n += 2;  // the next one; past the last one issued after the loop
     }
+    // This warp's loads among the block's last NS (one per slot; earlier ones
+    // have been consumed, and their slots hold later loads of either producer)
+    // have landed before the block may end.
     if (lane == 0)
-      for (int i = (n > NS ? n - NS : 0); i < n; ++i) drain_wait(bar(kKVFull + i % NS), (i / NS) & 1, timeout_ns);
+      for (int i = n - 2; i >= 0 && i >= 2 * n_x - NS; i -= 2) drain_wait(bar(kKVFull + i % NS), (i / NS) & 1, timeout_ns);
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer

@@ -131,7 +131,7 @@ __device__ __forceinline__ void load_vec(float (&f)[V], const T* p) {
 
 // Entries per access: 16 bytes of T where every row allows it, else one.
 template <typename T, int E>
-__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyParams p) {
+__global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyParams p) {
   __shared__ Shared sh;
   const int tid = threadIdx.x;
   const uint32_t rank = cluster_rank();
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyPara
         const T* pr = target + cur * p.st[1];
         const T* qr = draft + cur * p.sd[1];
         float sum = 0.f;
-#pragma unroll 4
+#pragma unroll (E == 1 ? 8 : 4)
         for (int v = lo + tid * E; v < hi; v += kVerifyThreads * E) {
           float pv[E], qv[E];
           load_vec<T, E>(pv, pr + v);
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyPara
     const int use_gone = pass == 0 ? gone1 : gone0;
     float top = -1.f;
     int at = lo;
-#pragma unroll 2
+#pragma unroll (E == 1 ? 8 : 2)
     for (int v = lo + tid * E; v < hi; v += kVerifyThreads * E) {
       float pv[E], qv[E], ev[E];
       load_vec<T, E>(pv, pr + v);
@@ -275,10 +275,10 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyPara
 
 template <typename T, int E>
 int launch_verify(VerifyParams& p, int B, cudaStream_t st) {
-  // The largest cluster whose blocks are all resident at once (four of 512
-  // threads per SM) and keep at least 2048 entries each.
+  // The largest cluster whose blocks are all resident at once (two of 512
+  // threads per SM: about 60 registers) and keep at least 2048 entries each.
   int cluster = 1;
-  while (cluster < kMaxCluster && (int64_t)B * cluster * 2 <= (int64_t)sm_count() * 4 && p.V / (cluster * 2) >= 2048) cluster *= 2;
+  while (cluster < kMaxCluster && (int64_t)B * cluster * 2 <= (int64_t)sm_count() * 2 && p.V / (cluster * 2) >= 2048) cluster *= 2;
   p.slice = ((p.V + cluster - 1) / cluster + 7) / 8 * 8;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)B * cluster);
