@@ -12,11 +12,14 @@
 // Split. A unit is what one thread holds of a row: two 16-byte vectors that
 // make whole pairs (half layout), or one (interleaved, and the copied dims).
 // A thread keeps its unit's cos/sin in registers and goes over a span of heads,
-// kHeads at a time, all loads before the first store, so that kHeads·2 vectors
-// are in flight per thread. kHeads is 4 where that still fills the GPU and 1
-// below (a decoding step, where the launch's latency is all there is). Rows that 16-byte vectors
-// cannot address (strides, alignment, R/2 not a multiple of the vector) take
-// the element-wise form of the same kernel.
+// one after another; what hides the memory's latency is many resident threads:
+// one head at a time in 40 registers (six blocks of 256 an SM, 32 bytes in
+// flight a thread) ran at 92% of the copy rate where four heads in flight in
+// 111 registers ran at 70%, and four squeezed into 64 with spills at 47%.
+// Interleaved, with one vector in flight, eight blocks (31 registers): 88%
+// against 81% with six. (B=4, S=4096, 32 + 8 heads of 128, bf16.)
+// Rows that 16-byte vectors cannot address (strides, alignment, R/2 not a
+// multiple of the vector) take the element-wise form of the same kernel.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -79,8 +82,8 @@ __device__ __forceinline__ void load_table(float (&f)[kPairs], const float* p) {
 }
 
 // V: elements per vector access (1: element-wise, any strides).
-template <typename T, bool IL, int V, int kHeads>
-__global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
+template <typename T, bool IL, int V>
+__global__ void __launch_bounds__(256, IL ? 8 : 6) rope_kernel(const RopeParams p) {
   const int idx = (int)(blockIdx.x * blockDim.x + threadIdx.x);
   if (idx >= p.S * p.units) return;
   const int s = idx / p.units, u = idx - s * p.units;
@@ -113,42 +116,31 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
         sn[i] = ok ? sn[i] * p.sign : __int_as_float(0x7fc00000);
       }
     }
-    for (int h0 = first; h0 < last; h0 += kHeads) {
-      Pack<T, V> x0[kHeads], x1[kHeads];
+    // The unit's place in head 0 of each tensor (rows of V > 1 have unit stride).
+    const int64_t dq = d0 * (V > 1 ? 1 : p.sq[3]), dk = d0 * (V > 1 ? 1 : p.sk[3]);
+    const T* q = static_cast<const T*>(p.q) + b * p.sq[0] + s * p.sq[2] + dq;
+    const T* k = static_cast<const T*>(p.k) + b * p.sk[0] + s * p.sk[2] + dk;
+    T* qo = static_cast<T*>(p.qo) + b * p.sqo[0] + s * p.sqo[2] + d0 * (V > 1 ? 1 : p.sqo[3]);
+    T* ko = static_cast<T*>(p.ko) + b * p.sko[0] + s * p.sko[2] + d0 * (V > 1 ? 1 : p.sko[3]);
+    const int step = d1 - d0;  // to the second vector
+    for (int h = first; h < last; ++h) {
+      const bool isq = h < p.Hq;
+      const T* from = isq ? q + h * p.sq[1] : k + (h - p.Hq) * p.sk[1];
+      T* to = isq ? qo + h * p.sqo[1] : ko + (h - p.Hq) * p.sko[1];
+      Pack<T, V> x0 = load_pack<T, V>(from), x1;
+      if (kTwo && turn) x1 = load_pack<T, V>(from + step * (V > 1 ? 1 : isq ? p.sq[3] : p.sk[3]));
+      if (turn) {
 #pragma unroll
-      for (int j = 0; j < kHeads; ++j) {
-        const int h = h0 + j;
-        if (h < last) {
-          const bool isq = h < p.Hq;
-          const int64_t* st = isq ? p.sq : p.sk;
-          const T* base = static_cast<const T*>(isq ? p.q : p.k) + b * st[0] + (int64_t)(isq ? h : h - p.Hq) * st[1] + s * st[2];
-          const int64_t sd = V > 1 ? 1 : st[3];
-          x0[j] = load_pack<T, V>(base + d0 * sd);
-          if (kTwo && turn) x1[j] = load_pack<T, V>(base + d1 * sd);
+        for (int i = 0; i < kPairs; ++i) {
+          T& ra = kTwo ? x0.x[i] : x0.x[(2 * i) % V];
+          T& rb = kTwo ? x1.x[i] : x0.x[(2 * i + 1) % V];
+          const float a = to_f32(ra), bb = to_f32(rb);
+          ra = from_f32<T>(a * c[i] - bb * sn[i]);
+          rb = from_f32<T>(a * sn[i] + bb * c[i]);
         }
       }
-#pragma unroll
-      for (int j = 0; j < kHeads; ++j) {
-        const int h = h0 + j;
-        if (h < last) {
-          const bool isq = h < p.Hq;
-          const int64_t* st = isq ? p.sqo : p.sko;
-          T* base = static_cast<T*>(isq ? p.qo : p.ko) + b * st[0] + (int64_t)(isq ? h : h - p.Hq) * st[1] + s * st[2];
-          const int64_t sd = V > 1 ? 1 : st[3];
-          if (turn) {
-#pragma unroll
-            for (int i = 0; i < kPairs; ++i) {
-              T& ra = kTwo ? x0[j].x[i] : x0[j].x[(2 * i) % V];
-              T& rb = kTwo ? x1[j].x[i] : x0[j].x[(2 * i + 1) % V];
-              const float a = to_f32(ra), bb = to_f32(rb);
-              ra = from_f32<T>(a * c[i] - bb * sn[i]);
-              rb = from_f32<T>(a * sn[i] + bb * c[i]);
-            }
-          }
-          store_pack<T, V>(base + d0 * sd, x0[j]);
-          if (kTwo && turn) store_pack<T, V>(base + d1 * sd, x1[j]);
-        }
-      }
+      store_pack<T, V>(to, x0);
+      if (kTwo && turn) store_pack<T, V>(to + step * (V > 1 ? 1 : isq ? p.sqo[3] : p.sko[3]), x1);
     }
   }
 }
@@ -167,19 +159,16 @@ int launch_rope(RopeParams& p, bool in_place, cudaStream_t st) {
   const int64_t per_head = (int64_t)p.S * p.units;
   if (per_head > INT32_MAX - 256) return BFA_ERR_UNSUPPORTED;
   const int H = p.Hq + p.Hk;
-  // Four heads in flight per thread where that leaves a full wave of threads,
-  // and more of them, one group of four after another (the table's values stay
-  // in registers), while two waves remain.
+  // More heads per thread (the table's values stay in registers) while two
+  // full waves of threads remain.
   const int64_t wave = (int64_t)sm_count() * 2048;
-  const bool four = per_head * p.B * ((H + 3) / 4) >= wave;
-  p.span = four ? 4 : 1;
-  while (four && p.span < H && per_head * p.B * ((H + 2 * p.span - 1) / (2 * p.span)) >= 2 * wave) p.span *= 2;
+  p.span = 1;
+  while (p.span < H && per_head * p.B * ((H + 2 * p.span - 1) / (2 * p.span)) >= 2 * wave) p.span *= 2;
   const int threads = (int)std::min<int64_t>(256, (per_head + 31) / 32 * 32);
   const int heads = (H + p.span - 1) / p.span;
   if (heads > 65535) return BFA_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)((per_head + threads - 1) / threads), (unsigned)heads, (unsigned)std::min(p.B, 65535));
-  if (four) rope_kernel<T, IL, V, 4><<<grid, threads, 0, st>>>(p);
-  else rope_kernel<T, IL, V, 1><<<grid, threads, 0, st>>>(p);
+  rope_kernel<T, IL, V><<<grid, threads, 0, st>>>(p);
   note_launch();
   return launch_status("rope kernel launch");
 }

@@ -37,6 +37,7 @@ namespace {
 
 constexpr int kMaxNodes = 64;
 constexpr int kVerifyThreads = 512;
+constexpr int kVerifyPerSm = 2;  // resident blocks per SM: 64 registers a thread
 constexpr int kMaxCluster = 8;
 
 struct VerifyParams {
@@ -97,7 +98,7 @@ __device__ __forceinline__ uint64_t combine(Shared& sh, uint64_t x, int round) {
   if (warp == 0) {
     x = lane < kVerifyThreads / 32 ? sh.warp[lane] : 0;
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) x = join(x, __shfl_xor_sync(0xffffffffu, x, o));
+    for (int o = kVerifyThreads / 64; o > 0; o >>= 1) x = join(x, __shfl_xor_sync(0xffffffffu, x, o));
     const uint32_t n = cluster_size();
     x = __shfl_sync(0xffffffffu, x, 0);
     if (lane < n) store_remote(&sh.slot[round & 1][cluster_rank()], lane, x);
@@ -131,7 +132,8 @@ __device__ __forceinline__ void load_vec(float (&f)[V], const T* p) {
 
 // Entries per access: 16 bytes of T where every row allows it, else one.
 template <typename T, int E>
-__global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyParams p) {
+__global__ void __launch_bounds__(kVerifyThreads, kVerifyPerSm) verify_kernel(const VerifyParams p) {
+  constexpr int kFinalUnroll = E == 1 ? 8 : 2;
   __shared__ Shared sh;
   const int tid = threadIdx.x;
   const uint32_t rank = cluster_rank();
@@ -141,21 +143,23 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
   const T* draft = p.draft ? static_cast<const T*>(p.draft) + b * p.sd[0] : nullptr;
   const float* noise = p.noise + b * p.noise_stride;
 
+  // The noise row is needed however the walk goes: on its way to L2 meanwhile.
+  if (E > 1 && tid == 0 && hi > lo)
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(noise + lo), "r"((uint32_t)(hi - lo) * 4u) : "memory");
   if (tid < p.N) {
     int32_t up = tid == 0 ? -1 : p.parents ? p.parents[b * p.parents_stride + tid] : tid - 1;
-    int64_t x = 0;
-    float px = 0.f, qx = 0.f, u = 2.f;
+    const int64_t at = b * p.tokens_stride + tid;
+    const int64_t x = p.token_bytes == 8 ? static_cast<const int64_t*>(p.tokens)[at] : (int64_t) static_cast<const int32_t*>(p.tokens)[at];
+    const float u = p.uniforms[b * p.uniforms_stride + tid];
+    float px = 0.f, qx = 0.f;
     if (tid > 0 && (up < -1 || up >= tid)) {
       up = -1;
       if (p.status) *p.status = BFA_ERR_INDEX;
     }
     if (up >= 0) {
-      const int64_t at = b * p.tokens_stride + tid;
-      x = p.token_bytes == 8 ? static_cast<const int64_t*>(p.tokens)[at] : (int64_t) static_cast<const int32_t*>(p.tokens)[at];
       if (x >= 0 && x < p.V) {
         px = to_f32<T>(target[up * p.st[1] + x]);
         if (draft) qx = to_f32<T>(draft[up * p.sd[1] + x]);
-        u = p.uniforms[b * p.uniforms_stride + tid];
       } else {
         up = -1;  // never a candidate
         if (p.status) *p.status = BFA_ERR_INDEX;
@@ -233,7 +237,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
     const int use_gone = pass == 0 ? gone1 : gone0;
     float top = -1.f;
     int at = lo;
-#pragma unroll (E == 1 ? 8 : 2)
+#pragma unroll kFinalUnroll
     for (int v = lo + tid * E; v < hi; v += kVerifyThreads * E) {
       float pv[E], qv[E], ev[E];
       load_vec<T, E>(pv, pr + v);
@@ -243,19 +247,17 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
 #pragma unroll
         for (int i = 0; i < E; ++i) pv[i] = pv[i] - a * qv[i];
       }
-      for (int i = gone0; i < use_gone; ++i) {
-        const int g = sh.gone[i] - v;
-#pragma unroll
-        for (int j = 0; j < E; ++j)
-          if (g == j) pv[j] = 0.f;
-      }
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         float r = pv[i] > 0.f ? pv[i] / ev[i] : 0.f;
         r = r >= 0.f ? r : 0.f;
-        if (r > top) {
-          top = r;
-          at = v + i;
+        if (r > top) {  // a few times per thread: only here the rejected tokens matter
+          bool out = false;
+          for (int g = gone0; g < use_gone; ++g) out |= sh.gone[g] == v + i;
+          if (!out) {
+            top = r;
+            at = v + i;
+          }
         }
       }
     }
@@ -275,10 +277,10 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
 
 template <typename T, int E>
 int launch_verify(VerifyParams& p, int B, cudaStream_t st) {
-  // The largest cluster whose blocks are all resident at once (two of 512
-  // threads per SM: about 60 registers) and keep at least 2048 entries each.
+  // The largest cluster whose blocks are all resident at once and keep at
+  // least 2048 entries each.
   int cluster = 1;
-  while (cluster < kMaxCluster && (int64_t)B * cluster * 2 <= (int64_t)sm_count() * 2 && p.V / (cluster * 2) >= 2048) cluster *= 2;
+  while (cluster < kMaxCluster && (int64_t)B * cluster * 2 <= (int64_t)sm_count() * kVerifyPerSm && p.V / (cluster * 2) >= 2048) cluster *= 2;
   p.slice = ((p.V + cluster - 1) / cluster + 7) / 8 * 8;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)B * cluster);
