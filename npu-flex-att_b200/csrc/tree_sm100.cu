@@ -18,7 +18,8 @@
 //   warp 3      the tree's ancestor sets, one item ahead
 //   warps 4..   softmax, 8 warps per 128-row tile: two threads share a row (TMEM
 //               lane), each with half of the chunk's keys and of O's columns;
-//               they agree on the row's maximum through shared memory
+//               they agree on the row's maximum through shared memory. P (16-bit)
+//               takes the first half of each thread's own columns of S
 // With two tiles (NT = 2) one tile's softmax runs under the other's products:
 // S_0(j), S_1(j), then PV_0(j), S_0(j+1), PV_1(j), S_1(j+1). With one tile S is
 // double-buffered: S(j+1) is formed before PV(j). P·V goes out in two halves
@@ -47,7 +48,6 @@ using namespace sm100;
 
 constexpr int kBM = 128;
 constexpr float kRescaleThreshold = 8.0f;
-constexpr int kPolyEvery = 8;
 
 // CH keys per chunk: 128, or 64 at D = 256 (64 KB of K and V either way).
 template <int D, int NT>
@@ -110,17 +110,25 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
   using L = TreeLayout<D, NT>;
   constexpr int CH = L::kCH, NS = L::kStages;
   constexpr int HC = CH / 2;  // keys of a softmax thread per chunk
+  // With one tile a softmax thread holds its S row in registers from the
+  // maximum to the exponentials. Two tiles' 512 softmax threads have 96
+  // registers each: they read S twice, 32 columns at a time (holding it
+  // spilled to local memory).
+  constexpr bool kHold = NT == 1;
+  constexpr int kGroups = HC / 32, kUnroll = kHold ? kGroups : 1;
   enum {
     kQFull = 0,
     kKVFull = 1,
     kKVEmpty = kKVFull + NS,
     kMask = kKVEmpty + NS,   // the item's ancestor sets, by its parity
     kMaskFree = kMask + 2,   // an item's softmax is done with them
-    kSFull = kMaskFree + 2,  // NT = 2: S_t formed; NT = 1: the S buffer of that parity
+    // Two of each: NT = 2: of tile t, a phase a chunk; NT = 1: of the chunk's
+    // parity (its S buffer), a phase every second chunk.
+    kSFull = kMaskFree + 2,  // S formed
     kPHalf = kSFull + 2,     // P of the first half of the keys, and a final O, in TMEM
-    kPFull = kPHalf + NT,    // P of the second half
-    kODone = kPFull + NT,
-    kDrain = kODone + NT,
+    kPFull = kPHalf + 2,     // P of the second half
+    kODone = kPFull + 2,     // P·V done
+    kDrain = kODone + 2,
     kNumBars = kDrain + 1
   };
   static_assert(kNumBars <= 40, "barriers");
@@ -130,6 +138,7 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
   const uint32_t sbase = smem_u32(smem);
   TreeMisc& mi = *reinterpret_cast<TreeMisc*>(smem + L::kOffMisc);
   auto bar = [&](int i) -> uint32_t { return sbase + L::kOffMisc + 8u * (uint32_t)i; };
+  auto phase = [](int x) { return (NT == 2 ? x : x >> 1) & 1; };  // of chunk x's barriers
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -275,15 +284,15 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
         const uint64_t dv = desc_mnmajor(kv_addr(2 * x + 1), CH * 128);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          if (!wait(half ? kPFull + t : kPHalf + t, x & 1)) return false;
+          if (!wait((half ? kPFull : kPHalf) + buf, phase(x))) return false;
 #pragma unroll
           for (int k4 = 0; k4 < CH / 32; ++k4) {
             const int kk = half * (CH / 32) + k4;
             if (kk < steps)
-              mma_ts(tmem + L::kTmemO + t * D, tmem + buf * CH + kk * 8, dv + ((kk * 16 * 128) >> 4), idO, 1u);
+              mma_ts(tmem + L::kTmemO + t * D, tmem + buf * CH + half * HC + k4 * 8, dv + ((kk * 16 * 128) >> 4), idO, 1u);
           }
         }
-        mma_commit(bar(kODone + t));
+        mma_commit(bar(kODone + buf));
         return true;
       };
       bool ok = true;
@@ -398,6 +407,14 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
       ok = ok && warp_wait(bar(kMask + (seg & 1)), (uint32_t)((seg >> 1) & 1), ctl);
       const int all_from = p.window > 0 ? cur.len + p.N - 1 - p.window : 0;
       float m = neg_inf(), l = 0.f;  // l: of this thread's keys
+      float slope2 = 0.f;            // ALiBi, times log2 e
+      int ref = 0;
+      if (ALIBI) {
+        int hq, node;
+        where(&hq, &node);
+        slope2 = p.alibi[hq] * kLog2e;
+        ref = tree_alibi_ref(p, slope2, cur.len + masks.depth[node]);
+      }
 
       for (int it = 0; it < count; ++it, ++x) {
         const int c = cur.c + it;
@@ -441,74 +458,78 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
           hold = (bad[0] | bad[1]) != 0;
         }
 
-        ok = ok && warp_wait(bar(kSFull + buf), (uint32_t)(NT == 2 ? x & 1 : (x >> 1) & 1), ctl);
+        ok = ok && warp_wait(bar(kSFull + buf), (uint32_t)phase(x), ctl);
         tc_fence_after();
-        uint32_t r[HC / 32][32];
-#pragma unroll
-        for (int ch = 0; ch < HC / 32; ++ch) tmem_ld32(tS + h * HC + 32 * ch, r[ch]);
-        tmem_ld_wait();
+        // Groups of 32 columns past the last key are left out: P·V stops at the
+        // last 16 keys that hold one.
+        const int used = valid - h * HC;  // of this thread's columns
         const bool formed = CAP || ALIBI || masked || !(sl2 > 0.f);  // logits in r, else raw products
-        float mx;
-        if (formed) {
-          // Logits in base 2 (cap's tanh: the series on the FMA pipe where
-          // every |s/cap| of the warp is small, else the closed form).
-          float slope2 = 0.f;
-          int ref = 0, depth = 0, pos = 0;
-          uint64_t seen = 0;
-          if (ALIBI || masked) {
-            int hq, node;
-            const bool live = where(&hq, &node);
-            depth = masks.depth[node];
-            pos = cur.len + depth;
-            seen = live ? masks.anc[node] : 0ull;
+        // What masked chunks keep: columns [lo, hi) of cached tokens, or the seen nodes.
+        int lo = 0, hi = 0;
+        uint64_t seen = 0;
+        if (masked && used > 0) {
+          int hq, node;
+          const bool live = where(&hq, &node);
+          const int depth = masks.depth[node];
+          seen = live ? masks.anc[node] : 0ull;
+          lo = p.window > 0 ? max(0, cur.len + depth - p.window - key0) : 0;
+          hi = seen ? valid : 0;
+          if (tree && p.window > 0 && p.window < p.N)
+            for (int i = 0; i < p.N; ++i)
+              if (depth - masks.depth[i] > p.window) seen &= ~(1ull << i);
+        }
+        // Logits in base 2 of a group (cap's tanh: the series on the FMA pipe
+        // where every |s/cap| of the warp is small, else the closed form).
+        auto form = [&](uint32_t(&u)[32], int k0, auto tier_tag) {
+          constexpr int TIER = decltype(tier_tag)::value;
+          const float abase = ALIBI ? slope2 * (float)(ref - key0 - k0) : 0.f;
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float2 raw = make_float2(__uint_as_float(u[e]), __uint_as_float(u[e + 1]));
+            float2 y, bias = make_float2(0.f, 0.f);
             if (ALIBI) {
-              slope2 = p.alibi[hq] * kLog2e;
-              ref = tree_alibi_ref(p, slope2, pos);
-            }
-          }
-          auto form = [&](auto tier_tag) {
-            constexpr int TIER = decltype(tier_tag)::value;
-            const float abase = ALIBI ? slope2 * (float)(ref - key0 - h * HC) : 0.f;
-#pragma unroll
-            for (int ch = 0; ch < HC / 32; ++ch)
-#pragma unroll
-              for (int e = 0; e < 32; e += 2) {
-                const float2 raw = make_float2(__uint_as_float(r[ch][e]), __uint_as_float(r[ch][e + 1]));
-                float2 y;
-                if (CAP) {
-                  float2 th;
-                  y = cap_logit2x2<TIER>(raw, cap_in, cap_out, &th);
-                } else {
-                  y = __fmul2_rn(raw, make_float2(sl2, sl2));
-                }
-                if (ALIBI) {
-                  const int k = 32 * ch + e;
-                  if (tree) {
-                    y.x += slope2 * (float)(ref - cur.len - masks.depth[(h * HC + k) & (kTreeNodes - 1)]);
-                    y.y += slope2 * (float)(ref - cur.len - masks.depth[(h * HC + k + 1) & (kTreeNodes - 1)]);
-                  } else {
-                    y.x += fmaf(-slope2, (float)k, abase);
-                    y.y += fmaf(-slope2, (float)(k + 1), abase);
-                  }
-                }
-                r[ch][e] = __float_as_uint(y.x);
-                r[ch][e + 1] = __float_as_uint(y.y);
+              if (tree) {
+                const int from = ref - cur.len;
+                bias.x = slope2 * (float)(from - masks.depth[(k0 + e) & (kTreeNodes - 1)]);
+                bias.y = slope2 * (float)(from - masks.depth[(k0 + e + 1) & (kTreeNodes - 1)]);
+              } else {
+                bias = __ffma2_rn(make_float2(-slope2, -slope2), make_float2((float)e, (float)(e + 1)), make_float2(abase, abase));
               }
-          };
-          const int tier = CAP ? cap_tier<HC>(&r[0][0], cap_in) : 0;
-          if (CAP && tier == 2) form(std::integral_constant<int, 2>{});
-          else if (CAP && tier == 1) form(std::integral_constant<int, 1>{});
-          else form(std::integral_constant<int, 0>{});
-          if (masked) {
-            // Kept columns: [lo, hi) of cached tokens, or the seen nodes.
-            const int lo = p.window > 0 ? max(0, pos - p.window - key0) : 0;
-            const int hi = seen ? valid : 0;
-            if (tree && p.window > 0 && p.window < p.N)
-              for (int i = 0; i < p.N; ++i)
-                if (depth - masks.depth[i] > p.window) seen &= ~(1ull << i);
+            }
+            if (CAP) {
+              float2 th;
+              y = cap_logit2x2<TIER>(raw, cap_in, cap_out, &th);
+              if (ALIBI) y = __fadd2_rn(y, bias);
+            } else {
+              y = __ffma2_rn(raw, make_float2(sl2, sl2), bias);
+            }
+            u[e] = __float_as_uint(y.x);
+            u[e + 1] = __float_as_uint(y.y);
+          }
+        };
+        uint32_t r[kHold ? kGroups : 1][32];
+        float m4[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
+        if (kHold) {
 #pragma unroll
-            for (int ch = 0; ch < HC / 32; ++ch) {
-              const int k0 = h * HC + 32 * ch;
+          for (int ch = 0; ch < kGroups; ++ch)
+            if (32 * ch < used) tmem_ld32(tS + h * HC + 32 * ch, r[kHold ? ch : 0]);
+          tmem_ld_wait();
+        }
+#pragma unroll kUnroll
+        for (int ch = 0; ch < kGroups; ++ch) {
+          if (32 * ch >= used) continue;
+          uint32_t(&u)[32] = r[kHold ? ch : 0];
+          const int k0 = h * HC + 32 * ch;
+          if (!kHold) {
+            tmem_ld32(tS + k0, u);
+            tmem_ld_wait();
+          }
+          if (formed) {
+            const int tier = CAP ? cap_tier<32>(u, cap_in) : 0;
+            if (CAP && tier == 2) form(u, k0, std::integral_constant<int, 2>{});
+            else if (CAP && tier == 1) form(u, k0, std::integral_constant<int, 1>{});
+            else form(u, k0, std::integral_constant<int, 0>{});
+            if (masked) {
               uint32_t keep = 0;  // bit e: column k0 + e
               if (tree) {
                 keep = k0 < kTreeNodes ? (uint32_t)(seen >> (k0 & 63)) : 0u;
@@ -517,26 +538,22 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
                 if (to > from) keep = (0xffffffffu >> (32 - (to - from))) << from;
               }
 #pragma unroll
-              for (int e = 0; e < 32; ++e) r[ch][e] = (keep >> e) & 1u ? r[ch][e] : 0xff800000u;
+              for (int e = 0; e < 32; ++e) u[e] = (keep >> e) & 1u ? u[e] : 0xff800000u;
+            }
+            if (!kHold) {
+              tmem_st32(tS + k0, u);
+              tmem_st_wait();
             }
           }
-        }
-        {
-          float m4[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
 #pragma unroll
-          for (int ch = 0; ch < HC / 32; ++ch)
-#pragma unroll
-            for (int e = 0; e < 32; e += 2)
-              m4[(e >> 1) & 3] = fmax3(m4[(e >> 1) & 3], __uint_as_float(r[ch][e]), __uint_as_float(r[ch][e + 1]));
-          mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-          if (!formed) mx *= sl2;
+          for (int e = 0; e < 32; e += 2)
+            m4[(e >> 1) & 3] = fmax3(m4[(e >> 1) & 3], __uint_as_float(u[e]), __uint_as_float(u[e + 1]));
         }
-        // The row's maximum over both halves. The barrier also lets the second
-        // half store P over columns of S that the first half has read by now.
+        float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        if (!formed) mx *= sl2;
+        // The row's maximum over both halves.
         mi.top[x & 1][t][h][row] = mx;
-        tc_fence_before();
         named_sync(1 + t, 256);
-        tc_fence_after();
         mx = fmaxf(mx, mi.top[x & 1][t][h ^ 1][row]);
         const bool grow = (mx > m + kRescaleThreshold) || (m == neg_inf() && mx != neg_inf());
         float m_new = m;
@@ -548,11 +565,17 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
         const float m_use = m_new == neg_inf() ? 0.f : m_new;
         const float alpha = ex2(m - m_use);
         m = m_new;
-        // O stands still: the last P·V is done.
-        if (it > 0) {
-          ok = ok && warp_wait(bar(kODone + t), (uint32_t)((x - 1) & 1), ctl);
-          tc_fence_after();
+        // O may be rescaled once the last P·V is done. NT = 2: S of this chunk
+        // was issued after it, so it is. NT = 1: only a rescale waits for it;
+        // every chunk waits for the one before, long done, so that no phase of
+        // the barriers is passed over.
+        if (NT == 2) {
+          if (it > 0) ok = ok && warp_wait(bar(kODone + buf), (uint32_t)phase(x - 1), ctl);
+        } else {
+          if (x > 1) ok = ok && warp_wait(bar(kODone + buf), (uint32_t)phase(x - 2), ctl);
+          if (rescale) ok = ok && warp_wait(bar(kODone + (buf ^ 1)), (uint32_t)phase(x - 1), ctl);
         }
+        tc_fence_after();
         if (rescale) {
 #pragma unroll 1
           for (int i = 0; i < D / 32; ++i) {
@@ -568,31 +591,29 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
         if (h == 1 && !hold) {  // this half of O is final before the first P·V half
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar(kPHalf + t));
+          if (lane == 0) mbar_arrive(bar(kPHalf + buf));
         }
         {
           float2 s2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
           const float2 xs2 = make_float2(formed ? 1.f : sl2, formed ? 1.f : sl2), nm2 = make_float2(-m_use, -m_use);
-          // On chunks that every row keeps whole, every kPolyEvery-th
-          // exponential runs on the FMA pipe.
-          auto exps = [&](auto split_tag) {
-            constexpr bool SPLIT = decltype(split_tag)::value;
-#pragma unroll
-            for (int ch = 0; ch < HC / 32; ++ch) {
-              uint32_t pk[16];
-#pragma unroll
-              for (int e = 0; e < 32; e += 2) {
-                const float2 y = __ffma2_rn(make_float2(__uint_as_float(r[ch][e]), __uint_as_float(r[ch][e + 1])), xs2, nm2);
-                const float p0 = ex2(y.x);
-                const float p1 = (SPLIT && e % kPolyEvery == kPolyEvery - 2) ? ex2_poly(y.y) : ex2(y.y);
-                s2[(e >> 1) & 1] = __fadd2_rn(s2[(e >> 1) & 1], make_float2(p0, p1));
-                pk[e / 2] = pack2<BF16>(p0, p1);
-              }
-              tmem_st16(tS + h * (HC / 2) + 16 * ch, pk);
+#pragma unroll kUnroll
+          for (int ch = 0; ch < kGroups; ++ch) {
+            if (32 * ch >= used) continue;
+            uint32_t(&u)[32] = r[kHold ? ch : 0];
+            if (!kHold) {
+              tmem_ld32(tS + h * HC + 32 * ch, u);
+              tmem_ld_wait();
             }
-          };
-          if (masked) exps(std::false_type{});
-          else exps(std::true_type{});
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float2 y = __ffma2_rn(make_float2(__uint_as_float(u[e]), __uint_as_float(u[e + 1])), xs2, nm2);
+              const float p0 = ex2(y.x), p1 = ex2(y.y);
+              s2[(e >> 1) & 1] = __fadd2_rn(s2[(e >> 1) & 1], make_float2(p0, p1));
+              pk[e / 2] = pack2<BF16>(p0, p1);
+            }
+            tmem_st16(tS + h * HC + 16 * ch, pk);
+          }
           l = l * alpha + ((s2[0].x + s2[0].y) + (s2[1].x + s2[1].y));
           tmem_st_wait();
         }
@@ -606,7 +627,7 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
 #pragma unroll 1
           for (int n = 0; n < valid; ++n) {
             if (!((mi.bad[x & 1][n >> 6] >> (n & 63)) & 1)) continue;
-            const uint32_t w = tmem_ld1(tS + (n >> 1));
+            const uint32_t w = tmem_ld1(tS + n / HC * HC + (n % HC >> 1));
             tmem_ld_wait();
             const float pr = half_of<BF16>(w, n & 1);
 #pragma unroll 1
@@ -640,8 +661,8 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          if (h == 0 || hold) mbar_arrive(bar(kPHalf + t));
-          if (h == 1) mbar_arrive(bar(kPFull + t));
+          if (h == 0 || hold) mbar_arrive(bar(kPHalf + buf));
+          if (h == 1) mbar_arrive(bar(kPFull + buf));
         }
       }
 
@@ -649,7 +670,7 @@ __global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
       mi.sum[t][h][row] = l;
       named_sync(1 + t, 256);
       l = mi.sum[t][0][row] + mi.sum[t][1][row];
-      ok = ok && warp_wait(bar(kODone + t), (uint32_t)((x - 1) & 1), ctl);
+      ok = ok && warp_wait(bar(kODone + (NT == 2 ? t : (x - 1) & 1)), (uint32_t)phase(x - 1), ctl);
       tc_fence_after();
       if (ok) {
         const bool whole = cur.c == 0 && count == cur.n;
