@@ -175,16 +175,9 @@ Plan make_plan(const bfa_tree_args* a, const TreeTile& tile) {
 
 TreeTile simt_tile(const bfa_tree_args* a) { return {kTreeSimtRows, kTreeSimtChunk, a->head_dim > 128 ? 1 : 2}; }
 
-// Rows per KV head from which the tcgen05 kernel is taken, where the layouts allow it.
-constexpr int64_t kTcgen05Rows = 1;
-
-bool tcgen05_on() {  // BFA_TREE_TCGEN05=0 keeps bf16/fp16 on the mma.sync kernel, =1 on tcgen05 at any row count
+bool tcgen05_on() {  // BFA_TREE_TCGEN05=0 keeps bf16/fp16 on the mma.sync kernel
   const char* e = std::getenv("BFA_TREE_TCGEN05");
   return !(e && e[0] == '0');
-}
-bool tcgen05_always() {
-  const char* e = std::getenv("BFA_TREE_TCGEN05");
-  return e && e[0] == '1';
 }
 
 // Workspace for either 16-bit kernel: which one runs depends on the layouts,
@@ -192,7 +185,8 @@ bool tcgen05_always() {
 size_t workspace_bytes(const bfa_tree_args* a) {
   if (a->dtype == BFA_DTYPE_F32) return make_plan(a, simt_tile(a)).bytes;
   const int64_t rows = a->heads_q / a->heads_kv * a->nodes;
-  return std::max(make_plan(a, tree_mma_tile(rows, (int)a->head_dim)).bytes, make_plan(a, tree_sm100_tile(rows, (int)a->head_dim)).bytes);
+  return std::max(make_plan(a, tree_mma_tile(rows, (int)a->head_dim)).bytes,
+                  make_plan(a, tree_sm100_tile(rows, (int)a->head_dim, a->soft_cap > 0)).bytes);
 }
 
 template <typename T>
@@ -248,8 +242,13 @@ extern "C" int bfa_tree_fwd(const bfa_tree_args* a, void* stream) {
     return BFA_ERR_WORKSPACE;
   const int64_t rows = a->heads_q / a->heads_kv * a->nodes;
   const bool f32 = a->dtype == BFA_DTYPE_F32;
-  const bool tc = !f32 && tcgen05_on() && (rows >= kTcgen05Rows || tcgen05_always()) && tree_sm100_layout(a);
-  const Plan pl = make_plan(a, f32 ? simt_tile(a) : tc ? tree_sm100_tile(rows, (int)a->head_dim) : tree_mma_tile(rows, (int)a->head_dim));
+  // tcgen05 wherever TMA can read the layouts: it was the faster one at every
+  // size tried (B=16, L=8192, 8 KV heads of 128: 4 rows a KV head 95 against
+  // 125 us, 64 rows 109 against 184, 256 rows 195 against 551).
+  const bool tc = !f32 && tcgen05_on() && tree_sm100_layout(a);
+  const Plan pl = make_plan(a, f32  ? simt_tile(a)
+                               : tc ? tree_sm100_tile(rows, (int)a->head_dim, a->soft_cap > 0)
+                                    : tree_mma_tile(rows, (int)a->head_dim));
   TreeParams p{};
   p.q = a->q.data; p.k = a->k.data; p.v = a->v.data; p.o = a->o.data;
   p.lse = a->lse;

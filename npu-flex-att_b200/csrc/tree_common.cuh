@@ -295,7 +295,7 @@ TreeTile tree_mma_tile(int64_t rows, int D);
 int tree_mma(const TreeParams& p, int dtype, cudaStream_t st);
 
 // tree_sm100.cu: bf16 / fp16 on tcgen05, pages by TMA.
-TreeTile tree_sm100_tile(int64_t rows, int D);
+TreeTile tree_sm100_tile(int64_t rows, int D, bool cap);
 // Whether its layouts allow it (the sizes are the caller's rule).
 bool tree_sm100_layout(const bfa_tree_args* a);
 int tree_sm100(const TreeParams& p, int dtype, cudaStream_t st);

@@ -1,766 +1,25 @@
-// tree_sm100.cu -- attention of a tree of drafted tokens over a paged cache in
-// bf16 / fp16 on tcgen05, K/V pages by TMA.
-//
-// Mathematics: the online softmax of the other forwards (base 2; P rounded to
-// the input type and kept in TMEM as the A operand of P·V; O rescaled only when
-// a row's maximum grows by more than 2^8). The rows r = g·N + n of one KV head
-// are stacked into tiles of 128, so its K/V cross HBM once per block of rows.
-//
-// Bound: HBM (K/V read once) up to about 256 rows per KV head, the tensor cores
-// above; mma.sync falls behind HBM from about 64 rows.
-//
-// Split. Persistent blocks, one per SM, each with an equal stretch of the list
-// of chunks (tree_common.cuh). Warp roles:
-//   warps 0, 2  producers of K and of V: find a chunk's pages and load it by
-//               TMA, a lane per box, into a ring that runs on across items
-//   warp 1      MMA issuer
-//   warp 2      also allocates TMEM
-//   warp 3      the tree's ancestor sets, one item ahead
-//   warps 4..   softmax, 8 warps per 128-row tile: two threads share a row (TMEM
-//               lane), each with half of the chunk's keys and of O's columns;
-//               they agree on the row's maximum through shared memory. P (16-bit)
-//               takes the first half of each thread's own columns of S
-// With two tiles (NT = 2) one tile's softmax runs under the other's products:
-// S_0(j), S_1(j), then PV_0(j), S_0(j+1), PV_1(j), S_1(j+1). With one tile S is
-// double-buffered: S(j+1) is formed before PV(j). P·V goes out in two halves
-// of the keys, the first when the first half's threads have stored P.
-//
-// A box is gcd(page_size, chunk) tokens of one page, so any page size that is a
-// multiple of 8 works (8 rows of 128 bytes are the swizzle's atom). Tokens past
-// a sequence's end arrive as whatever the page holds: their logits are masked,
-// P·V stops at the last 16 keys that hold one, and the softmax warps clear the
-// rest of those 16 in V before the product may read it.
-#include <cuda.h>
-#include <cuda_runtime.h>
-
+// tree_sm100.cu -- which problems the tcgen05 tree attention takes, and its tile.
 #include <climits>
-#include <numeric>
-#include <type_traits>
 
 #include "sm100_host.h"
-#include "sm100_ptx.cuh"
 #include "tree_common.cuh"
 
 namespace bfa {
-namespace {
 
-using namespace sm100;
+int tree_sm100_d64(const TreeParams& p, int dtype, cudaStream_t st);
+int tree_sm100_d128(const TreeParams& p, int dtype, cudaStream_t st);
+int tree_sm100_d256(const TreeParams& p, int dtype, cudaStream_t st);
 
-constexpr int kBM = 128;
-constexpr float kRescaleThreshold = 8.0f;
-
-// CH keys per chunk: 128, or 64 at D = 256 (64 KB of K and V either way).
-template <int D, int NT>
-struct TreeLayout {
-  static constexpr int kCH = D == 256 ? 64 : 128;
-  static constexpr int kSub = D / 64;
-  static constexpr uint32_t kQTile = kBM * D * 2;
-  static constexpr uint32_t kKV = kCH * D * 2;
-  static constexpr uint32_t kMisc = 10240;
-  static constexpr int kFit = (int)((232448u - 1024u - kMisc - NT * kQTile) / kKV);
-  static constexpr int kStages = kFit < 8 ? kFit : 8;
-  static constexpr uint32_t kOffKV = NT * kQTile;
-  static constexpr uint32_t kOffMisc = kOffKV + kStages * kKV;
-  static constexpr uint32_t kBytes = kOffMisc + kMisc + 1024;  // 1024: alignment of the tiles
-  static constexpr uint32_t kTmemO = 2 * kCH;
-  static constexpr int kThreads = 128 + 256 * NT;
-  static_assert(kStages >= 4, "K and V of two chunks");
-  static_assert(kTmemO + NT * D <= 512, "TMEM");
-  static_assert(kBytes <= 232448, "shared memory");
-};
-
-struct TreeMisc {
-  uint64_t bar[40];
-  uint32_t tmem;
-  int abort;
-  unsigned long long bad[2][2];  // by the chunk's parity: its keys whose values are not finite
-  float top[2][2][2][kBM];       // row maxima: chunk's parity, tile, half of the keys, row
-  float sum[2][2][kBM];          // row sums at an item's end: tile, half, row
-  TreeMasks masks[2];            // by the item's parity
-};
-static_assert(sizeof(TreeMisc) <= 10240, "misc");
-
-// One column (32 bits per lane) of TMEM.
-__device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr) {
-  uint32_t r;
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
-  return r;
-}
-
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  return BF16 ? pack_bf16(a, b) : pack_f16(a, b);
-}
-template <bool BF16>
-__device__ __forceinline__ float half_of(uint32_t w, int hi) {
-  const uint32_t h = hi ? w >> 16 : w & 0xffffu;
-  return BF16 ? __uint_as_float(h << 16) : __half2float(__ushort_as_half((unsigned short)h));
-}
-template <bool BF16>
-__device__ __forceinline__ bool any_not_finite(uint32_t w) {
-  constexpr uint32_t e = BF16 ? 0x7f80u : 0x7c00u;
-  return (w & e) == e || ((w >> 16) & e) == e;
-}
-
-template <int D, int NT, bool BF16, bool CAP, bool ALIBI>
-__global__ void __launch_bounds__(TreeLayout<D, NT>::kThreads, 1)
-    tree_kernel(const __grid_constant__ CUtensorMap tmKp, const __grid_constant__ CUtensorMap tmVp,
-                const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeParams p, int box,
-                uint64_t timeout_ns) {
-  using L = TreeLayout<D, NT>;
-  constexpr int CH = L::kCH, NS = L::kStages;
-  constexpr int HC = CH / 2;  // keys of a softmax thread per chunk
-  // With one tile a softmax thread holds its S row in registers from the
-  // maximum to the exponentials. Two tiles' 512 softmax threads have 96
-  // registers each: they read S twice, 32 columns at a time (holding it
-  // spilled to local memory).
-  constexpr bool kHold = NT == 1;
-  constexpr int kGroups = HC / 32, kUnroll = kHold ? kGroups : 1;
-  enum {
-    kQFull = 0,
-    kKVFull = 1,
-    kKVEmpty = kKVFull + NS,
-    kMask = kKVEmpty + NS,   // the item's ancestor sets, by its parity
-    kMaskFree = kMask + 2,   // an item's softmax is done with them
-    // Two of each: NT = 2: of tile t, a phase a chunk; NT = 1: of the chunk's
-    // parity (its S buffer), a phase every second chunk.
-    kSFull = kMaskFree + 2,  // S formed
-    kPHalf = kSFull + 2,     // P of the first half of the keys, and a final O, in TMEM
-    kPFull = kPHalf + 2,     // P of the second half
-    kODone = kPFull + 2,     // P·V done
-    kDrain = kODone + 2,
-    kNumBars = kDrain + 1
-  };
-  static_assert(kNumBars <= 40, "barriers");
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t raw_addr = smem_u32(smem_raw);
-  uint8_t* smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
-  const uint32_t sbase = smem_u32(smem);
-  TreeMisc& mi = *reinterpret_cast<TreeMisc*>(smem + L::kOffMisc);
-  auto bar = [&](int i) -> uint32_t { return sbase + L::kOffMisc + 8u * (uint32_t)i; };
-  auto phase = [](int x) { return (NT == 2 ? x : x >> 1) & 1; };  // of chunk x's barriers
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (threadIdx.x == 32) {
-    tma_prefetch_desc(&tmKp);
-    tma_prefetch_desc(&tmVp);
-    tma_prefetch_desc(&tmK);
-    tma_prefetch_desc(&tmV);
-    for (int i = 0; i < kNumBars; ++i)
-      mbar_init(bar(i), i == kQFull || i == kMaskFree || i == kMaskFree + 1 ? 8u * NT
-                        : i >= kPHalf && i < kPFull                         ? 8u
-                        : i >= kPFull && i < kODone                         ? 4u
-                                                                            : 1u);
-    mi.abort = 0;
-    fence_barrier_init();
-  }
-  if (warp == 2) {
-    tmem_alloc(smem_u32(&mi.tmem), 512);
-    tmem_relinquish();
-  }
-  TreeCursor cur;
-  const int n_x = tree_stretch(p, cur);  // 0 in a block without work: it only passes through
-  WaitCtl ctl{(volatile int*)&mi.abort, p.status, timeout_ns};
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = mi.tmem;
-
-  if (warp == 0 || warp == 2) {
-    // ------------------------------------------------------------ producers
-    const int kv = warp >> 1;
-    // Lane i·kSub + s: columns [64s, 64s + 64) of box i, tokens [key0 + i·box,
-    // + box) of one page (the tree's chunk: one box of 64 nodes).
-    const int my_box = lane / L::kSub, my_sub = lane % L::kSub;
-    // The sequence's page table, 64 entries at a time: lane i holds entries
-    // wb + i and wb + 32 + i; the second half is loaded 32 pages before it is
-    // used.
-    int wb = 0, wseq = -1, w0 = 0, w1 = 0;
-    auto entry = [&](const TreeCursor& at, int pg) {
-      return (int64_t)pg * p.page < at.len ? p.table[at.b * p.table_stride + pg] : 0;
-    };
-    auto page_of = [&](int token) { return p.page_log2 >= 0 ? token >> p.page_log2 : token / p.page; };
-    auto fill = [&](const TreeCursor& at) {
-      if (at.in_tree(p)) return;
-      const int pg = page_of(at.key0(p));
-      if (at.b != wseq || pg < wb || pg >= wb + 64) {
-        wseq = at.b;
-        wb = pg;
-        w0 = entry(at, wb + lane);
-        w1 = entry(at, wb + 32 + lane);
-      } else if (pg >= wb + 32) {
-        w0 = w1;
-        wb += 32;
-        w1 = entry(at, wb + 32 + lane);
-      }
-    };
-    struct Box {
-      int page, slot;
-      bool mine;
-    };
-    auto find = [&](const TreeCursor& at) -> Box {
-      Box r{0, 0, false};
-      if (at.in_tree(p)) {
-        r.mine = my_box == 0;
-        return r;
-      }
-      const int t0 = at.key0(p) + my_box * box;
-      r.mine = my_box < CH / box && t0 < at.len;
-      const int pg = r.mine ? page_of(t0) : wb;
-      r.slot = t0 - pg * p.page;
-      r.page = __shfl_sync(0xffffffffu, w0, pg - wb);  // the lane is taken modulo 32
-      if (__any_sync(0xffffffffu, pg - wb >= 32)) {
-        const int v = __shfl_sync(0xffffffffu, w1, pg - wb);
-        if (pg - wb >= 32) r.page = v;
-      }
-      return r;
-    };
-    bool ok = true;
-    int n = kv;
-    if (n_x > 0) fill(cur);
-    for (int x = 0; x < n_x && ok; ++x) {
-      Box me = find(cur);
-      const TreeCursor here = cur;
-      cur.next(p);
-      if (x + 1 < n_x) fill(cur);  // in flight while this chunk's slots are waited for
-      const bool tree = here.in_tree(p);
-      const int hkv = here.item / p.n_rb;
-      if (!tree && me.mine && (me.page < 0 || me.page >= p.num_pages)) {
-        me.page = (int)p.num_pages;  // outside the tensor: reads as zeros
-        if (p.status) *p.status = BFA_ERR_INDEX;
-      }
-      const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xffffffffu, me.mine)) * (tree ? 64 : box) * 128u;
-      n = 2 * x + kv;
-      const int st = n % NS;
-      if (n >= NS) {
-        int w = 1;
-        if (lane == 0) w = mbar_wait(bar(kKVEmpty + st), ((n / NS) & 1) ^ 1, ctl, BFA_ERR_DEVICE_TIMEOUT) ? 1 : 0;
-        ok = __shfl_sync(0xffffffffu, w, 0) != 0;
-        if (!ok) break;
-      }
-      if (lane == 0) mbar_arrive_expect_tx(bar(kKVFull + st), bytes);
-      __syncwarp();
-      if (me.mine) {
-        const uint32_t dst = sbase + L::kOffKV + st * L::kKV + my_sub * (CH * 128) + my_box * box * 128;
-        if (tree) tma_load_4d(dst, kv ? &tmV : &tmK, bar(kKVFull + st), my_sub * 64, 0, hkv, here.b);
-        else tma_load_4d(dst, kv ? &tmVp : &tmKp, bar(kKVFull + st), my_sub * 64, me.slot, hkv, me.page);
-      }
-      __syncwarp();
-      n += 2;  // the next one; past the last one issued after the loop
-    }
-    // This warp's loads among the block's last NS (one per slot; earlier ones
-    // have been consumed, and their slots hold later loads of either producer)
-    // have landed before the block may end.
-    if (lane == 0)
-      for (int i = n - 2; i >= 0 && i >= 2 * n_x - NS; i -= 2) drain_wait(bar(kKVFull + i % NS), (i / NS) & 1, timeout_ns);
-    __syncwarp();
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t idS = idesc_f16(kBM, CH, BF16, false);
-      constexpr uint32_t idO = idesc_f16(kBM, D, BF16, true);
-      auto kv_addr = [&](int idx) -> uint32_t { return sbase + L::kOffKV + (uint32_t)(idx % NS) * L::kKV; };
-      auto issue_s = [&](int t, int buf, int idx) {
-        const uint64_t dq = desc_kmajor(sbase + t * L::kQTile);
-        const uint64_t dk = desc_kmajor(kv_addr(idx));
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t offq = (kk >> 2) * (kBM * 128) + (kk & 3) * 32;
-          const uint32_t offk = (kk >> 2) * (CH * 128) + (kk & 3) * 32;
-          mma_ss(tmem + buf * CH, dq + (offq >> 4), dk + (offk >> 4), idS, kk > 0 ? 1u : 0u);
-        }
-        mma_commit(bar(kSFull + buf));
-      };
-      auto wait = [&](int i, int parity) {
-        if (!mbar_wait(bar(i), (uint32_t)parity, ctl, BFA_ERR_DEVICE_TIMEOUT)) return false;
-        tc_fence_after();
-        return true;
-      };
-      auto wait_load = [&](int idx) { return wait(kKVFull + idx % NS, (idx / NS) & 1); };
-      // P·V of chunk x over its first `steps`·16 keys, in two halves. O is
-      // zeroed by the softmax warps at an item's start: every product adds.
-      auto pv = [&](int t, int buf, int x, int steps) {
-        const uint64_t dv = desc_mnmajor(kv_addr(2 * x + 1), CH * 128);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (!wait((half ? kPFull : kPHalf) + buf, phase(x))) return false;
-#pragma unroll
-          for (int k4 = 0; k4 < CH / 32; ++k4) {
-            const int kk = half * (CH / 32) + k4;
-            if (kk < steps)
-              mma_ts(tmem + L::kTmemO + t * D, tmem + buf * CH + half * HC + k4 * 8, dv + ((kk * 16 * 128) >> 4), idO, 1u);
-          }
-        }
-        mma_commit(bar(kODone + buf));
-        return true;
-      };
-      bool ok = true;
-      int seg = 0;
-      for (int x = 0; x < n_x && ok; ++seg) {
-        const int count = min(cur.n - cur.c, n_x - x);  // chunks of this item that are this block's
-        ok = wait(kQFull, seg & 1) && wait_load(2 * x);
-        if (!ok) break;
-        issue_s(0, NT == 2 ? 0 : x & 1, 2 * x);
-        if constexpr (NT == 2) issue_s(1, 1, 2 * x);
-        mma_commit(bar(kKVEmpty + (2 * x) % NS));
-        for (int it = 0; it < count; ++it, ++x) {
-          const int iv = 2 * x + 1, ik = 2 * x + 2;
-          const bool more = it + 1 < count;
-          const int c = cur.c + it;
-          const int keys = c >= cur.n - p.tree_chunks ? p.N : min(CH, cur.len - (cur.lo + c * CH));
-          const int steps = (keys + 15) / 16;
-          if constexpr (NT == 2) {
-            if (!(ok = wait_load(iv) && pv(0, 0, x, steps))) break;
-            if (more) {
-              if (!(ok = wait_load(ik))) break;
-              issue_s(0, 0, ik);
-            }
-            if (!(ok = pv(1, 1, x, steps))) break;
-            mma_commit(bar(kKVEmpty + iv % NS));
-            if (more) {
-              issue_s(1, 1, ik);
-              mma_commit(bar(kKVEmpty + ik % NS));
-            }
-          } else {
-            if (more) {
-              if (!(ok = wait_load(ik))) break;
-              issue_s(0, (x + 1) & 1, ik);
-              mma_commit(bar(kKVEmpty + ik % NS));
-            }
-            if (!(ok = wait_load(iv) && pv(0, x & 1, x, steps))) break;
-            mma_commit(bar(kKVEmpty + iv % NS));
-          }
-        }
-        cur.next(p, count);
-      }
-      mma_commit(bar(kDrain));
-      drain_wait(bar(kDrain), 0, timeout_ns);
-    }
-  } else if (warp == 3) {
-    // ------------------------------------------------------------ ancestor sets
-    bool ok = true;
-    int seg = 0;
-    for (int x = 0; x < n_x && ok; ++seg) {
-      const int count = min(cur.n - cur.c, n_x - x);
-      if (seg > 1) ok = warp_wait(bar(kMaskFree + (seg & 1)), (uint32_t)(((seg >> 1) - 1) & 1), ctl);
-      tree_masks(p, cur.b, mi.masks[seg & 1]);
-      if (lane == 0) {
-        if (p.status && p.lens[cur.b] != cur.len) *p.status = BFA_ERR_INDEX;
-        mbar_arrive(bar(kMask + (seg & 1)));
-      }
-      x += count;
-      cur.next(p, count);
-    }
-  } else if (warp >= 4) {
-    // ------------------------------------------------------------ softmax
-    const int t = NT == 2 ? (warp - 4) >> 3 : 0, h = ((warp - 4) >> 2) & 1, wq = warp & 3;
-    const int row = wq * 32 + lane;     // of the tile
-    const int sid = threadIdx.x - 128;  // among the softmax threads
-    constexpr int kSoft = 256 * NT;
-    const uint32_t lane_base = (uint32_t)(wq * 32) << 16;
-    const uint32_t tO = tmem + lane_base + L::kTmemO + t * D + h * (D / 2);  // this thread's half of O
-    const float sl2 = p.scale * kLog2e;
-    const float cap_in = CAP ? p.scale / p.soft_cap : 0.f, cap_out = CAP ? p.soft_cap * kLog2e : 0.f;
-    bool ok = true;  // false: this block gave up on a wait; the flow goes on without waiting
-    int seg = 0;
-    for (int x = 0; x < n_x; ++seg) {
-      // ---------------------------------------------------- an item begins
-      // (`cur` stands at its first chunk of this block's. Little else is kept
-      // over the loop: what only masked chunks and the end need is formed
-      // again there, from values made opaque so that none stays in registers.)
-      const int count = min(cur.n - cur.c, n_x - x);
-      auto where = [&](int* hq, int* node) -> bool {  // the row's head and node; false past the rows
-        int item = cur.item;
-        asm volatile("" : "+r"(item));
-        const int hkv = item / p.n_rb, r = (item - hkv * p.n_rb) * (NT * kBM) + t * kBM + row;
-        const bool live = r < p.G * p.N;
-        tree_row(p, hkv, live ? r : 0, hq, node);
-        return live;
-      };
-      {
-        // Half of q's row into the swizzled tile (its readers, the last item's
-        // S products, are done: their barrier was waited for).
-        int hq, node;
-        const bool live = where(&hq, &node);
-        const uint4* src =
-            reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + cur.b * p.sq[0] + hq * p.sq[1] + node * p.sq[2]);
-        uint8_t* dst = smem + t * L::kQTile;
-#pragma unroll 8
-        for (int i = 0; i < D / 16; ++i) {
-          const int c = h * (D / 16) + i;
-          uint4 w = make_uint4(0u, 0u, 0u, 0u);
-          if (live && c * 8 < p.D) w = src[c];
-          *reinterpret_cast<uint4*>(dst + (c >> 3) * (kBM * 128) + sw128_offset(row, c & 7)) = w;
-        }
-        fence_async_shared();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(kQFull));
-        uint32_t z[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) z[i] = 0u;
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) tmem_st16(tO + 16 * c, z);
-        tmem_st_wait();
-      }
-      TreeMasks& masks = mi.masks[seg & 1];
-      ok = ok && warp_wait(bar(kMask + (seg & 1)), (uint32_t)((seg >> 1) & 1), ctl);
-      const int all_from = p.window > 0 ? cur.len + p.N - 1 - p.window : 0;
-      float m = neg_inf(), l = 0.f;  // l: of this thread's keys
-      float slope2 = 0.f;            // ALiBi, times log2 e
-      int ref = 0;
-      if (ALIBI) {
-        int hq, node;
-        where(&hq, &node);
-        slope2 = p.alibi[hq] * kLog2e;
-        ref = tree_alibi_ref(p, slope2, cur.len + masks.depth[node]);
-      }
-
-      for (int it = 0; it < count; ++it, ++x) {
-        const int c = cur.c + it;
-        const bool tree = c >= cur.n - p.tree_chunks;
-        const int key0 = tree ? 0 : cur.lo + c * CH;
-        const int valid = tree ? p.N : min(CH, cur.len - key0);  // rows of the chunk that hold keys
-        const bool masked = tree || valid < CH || key0 < all_from;
-        const int buf = NT == 2 ? t : x & 1;
-        const uint32_t tS = tmem + lane_base + buf * CH;
-
-        // The last P·V's rows of V that no key holds are cleared (the tree's
-        // come as zeros); where rows differ in what they see, values that are
-        // not finite are looked for: 0·inf must not reach a row that does not
-        // see the key.
-        bool hold = false;
-        const bool differ = (tree && p.N > 1) || key0 < all_from;
-        if (differ || (!tree && (valid & 15))) {
-          ok = ok && warp_wait(bar(kKVFull + (2 * x + 1) % NS), (uint32_t)(((2 * x + 1) / NS) & 1), ctl);
-          uint8_t* vt = smem + L::kOffKV + ((2 * x + 1) % NS) * L::kKV;
-          unsigned long long* bad = mi.bad[x & 1];  // the other one may still be read by a slower warp
-          if (sid < 2) bad[sid] = 0ull;
-          named_sync(3, kSoft);
-          // Piece i: 16 bytes of row i / 8 of a 64-column sub-tile.
-          const int upto = (valid + 15) / 16 * 16;
-          for (int i = (differ ? 0 : valid * 8) + sid; i < upto * 8; i += kSoft) {
-            const int r = i >> 3;
-#pragma unroll
-            for (int sub = 0; sub < L::kSub; ++sub) {
-              uint4* at = reinterpret_cast<uint4*>(vt + sub * (CH * 128) + r * 128 + (i & 7) * 16);
-              if (r >= valid) {
-                *at = make_uint4(0u, 0u, 0u, 0u);
-              } else {
-                const uint4 w = *at;
-                if (any_not_finite<BF16>(w.x) || any_not_finite<BF16>(w.y) || any_not_finite<BF16>(w.z) || any_not_finite<BF16>(w.w))
-                  atomicOr(&bad[r >> 6], 1ull << (r & 63));
-              }
-            }
-          }
-          fence_async_shared();
-          named_sync(3, kSoft);
-          hold = (bad[0] | bad[1]) != 0;
-        }
-
-        ok = ok && warp_wait(bar(kSFull + buf), (uint32_t)phase(x), ctl);
-        tc_fence_after();
-        // Groups of 32 columns past the last key are left out: P·V stops at the
-        // last 16 keys that hold one.
-        const int used = valid - h * HC;  // of this thread's columns
-        const bool formed = CAP || ALIBI || masked || !(sl2 > 0.f);  // logits in r, else raw products
-        // What masked chunks keep: columns [lo, hi) of cached tokens, or the seen nodes.
-        int lo = 0, hi = 0;
-        uint64_t seen = 0;
-        if (masked && used > 0) {
-          int hq, node;
-          const bool live = where(&hq, &node);
-          const int depth = masks.depth[node];
-          seen = live ? masks.anc[node] : 0ull;
-          lo = p.window > 0 ? max(0, cur.len + depth - p.window - key0) : 0;
-          hi = seen ? valid : 0;
-          if (tree && p.window > 0 && p.window < p.N)
-            for (int i = 0; i < p.N; ++i)
-              if (depth - masks.depth[i] > p.window) seen &= ~(1ull << i);
-        }
-        // Logits in base 2 of a group (cap's tanh: the series on the FMA pipe
-        // where every |s/cap| of the warp is small, else the closed form).
-        auto form = [&](uint32_t(&u)[32], int k0, auto tier_tag) {
-          constexpr int TIER = decltype(tier_tag)::value;
-          const float abase = ALIBI ? slope2 * (float)(ref - key0 - k0) : 0.f;
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float2 raw = make_float2(__uint_as_float(u[e]), __uint_as_float(u[e + 1]));
-            float2 y, bias = make_float2(0.f, 0.f);
-            if (ALIBI) {
-              if (tree) {
-                const int from = ref - cur.len;
-                bias.x = slope2 * (float)(from - masks.depth[(k0 + e) & (kTreeNodes - 1)]);
-                bias.y = slope2 * (float)(from - masks.depth[(k0 + e + 1) & (kTreeNodes - 1)]);
-              } else {
-                bias = __ffma2_rn(make_float2(-slope2, -slope2), make_float2((float)e, (float)(e + 1)), make_float2(abase, abase));
-              }
-            }
-            if (CAP) {
-              float2 th;
-              y = cap_logit2x2<TIER>(raw, cap_in, cap_out, &th);
-              if (ALIBI) y = __fadd2_rn(y, bias);
-            } else {
-              y = __ffma2_rn(raw, make_float2(sl2, sl2), bias);
-            }
-            u[e] = __float_as_uint(y.x);
-            u[e + 1] = __float_as_uint(y.y);
-          }
-        };
-        uint32_t r[kHold ? kGroups : 1][32];
-        float m4[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
-        if (kHold) {
-#pragma unroll
-          for (int ch = 0; ch < kGroups; ++ch)
-            if (32 * ch < used) tmem_ld32(tS + h * HC + 32 * ch, r[kHold ? ch : 0]);
-          tmem_ld_wait();
-        }
-#pragma unroll kUnroll
-        for (int ch = 0; ch < kGroups; ++ch) {
-          if (32 * ch >= used) continue;
-          uint32_t(&u)[32] = r[kHold ? ch : 0];
-          const int k0 = h * HC + 32 * ch;
-          if (!kHold) {
-            tmem_ld32(tS + k0, u);
-            tmem_ld_wait();
-          }
-          if (formed) {
-            const int tier = CAP ? cap_tier<32>(u, cap_in) : 0;
-            if (CAP && tier == 2) form(u, k0, std::integral_constant<int, 2>{});
-            else if (CAP && tier == 1) form(u, k0, std::integral_constant<int, 1>{});
-            else form(u, k0, std::integral_constant<int, 0>{});
-            if (masked) {
-              uint32_t keep = 0;  // bit e: column k0 + e
-              if (tree) {
-                keep = k0 < kTreeNodes ? (uint32_t)(seen >> (k0 & 63)) : 0u;
-              } else {
-                const int from = min(max(lo - k0, 0), 32), to = min(max(hi - k0, 0), 32);
-                if (to > from) keep = (0xffffffffu >> (32 - (to - from))) << from;
-              }
-#pragma unroll
-              for (int e = 0; e < 32; ++e) u[e] = (keep >> e) & 1u ? u[e] : 0xff800000u;
-            }
-            if (!kHold) {
-              tmem_st32(tS + k0, u);
-              tmem_st_wait();
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 32; e += 2)
-            m4[(e >> 1) & 3] = fmax3(m4[(e >> 1) & 3], __uint_as_float(u[e]), __uint_as_float(u[e + 1]));
-        }
-        float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-        if (!formed) mx *= sl2;
-        // The row's maximum over both halves.
-        mi.top[x & 1][t][h][row] = mx;
-        named_sync(1 + t, 256);
-        mx = fmaxf(mx, mi.top[x & 1][t][h ^ 1][row]);
-        const bool grow = (mx > m + kRescaleThreshold) || (m == neg_inf() && mx != neg_inf());
-        float m_new = m;
-        bool rescale = false;
-        if (__any_sync(0xffffffffu, grow)) {  // alike in both halves: the same rows and maxima
-          m_new = fmaxf(m, mx);
-          rescale = it > 0;
-        }
-        const float m_use = m_new == neg_inf() ? 0.f : m_new;
-        const float alpha = ex2(m - m_use);
-        m = m_new;
-        // O may be rescaled once the last P·V is done. NT = 2: S of this chunk
-        // was issued after it, so it is. NT = 1: only a rescale waits for it;
-        // every chunk waits for the one before, long done, so that no phase of
-        // the barriers is passed over.
-        if (NT == 2) {
-          if (it > 0) ok = ok && warp_wait(bar(kODone + buf), (uint32_t)phase(x - 1), ctl);
-        } else {
-          if (x > 1) ok = ok && warp_wait(bar(kODone + buf), (uint32_t)phase(x - 2), ctl);
-          if (rescale) ok = ok && warp_wait(bar(kODone + (buf ^ 1)), (uint32_t)phase(x - 1), ctl);
-        }
-        tc_fence_after();
-        if (rescale) {
-#pragma unroll 1
-          for (int i = 0; i < D / 32; ++i) {
-            uint32_t o16[16];
-            tmem_ld16(tO + 16 * i, o16);
-            tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o16[e] = __float_as_uint(__uint_as_float(o16[e]) * alpha);
-            tmem_st16(tO + 16 * i, o16);
-          }
-          tmem_st_wait();
-        }
-        if (h == 1 && !hold) {  // this half of O is final before the first P·V half
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(kPHalf + buf));
-        }
-        {
-          float2 s2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-          const float2 xs2 = make_float2(formed ? 1.f : sl2, formed ? 1.f : sl2), nm2 = make_float2(-m_use, -m_use);
-#pragma unroll kUnroll
-          for (int ch = 0; ch < kGroups; ++ch) {
-            if (32 * ch >= used) continue;
-            uint32_t(&u)[32] = r[kHold ? ch : 0];
-            if (!kHold) {
-              tmem_ld32(tS + h * HC + 32 * ch, u);
-              tmem_ld_wait();
-            }
-            uint32_t pk[16];
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float2 y = __ffma2_rn(make_float2(__uint_as_float(u[e]), __uint_as_float(u[e + 1])), xs2, nm2);
-              const float p0 = ex2(y.x), p1 = ex2(y.y);
-              s2[(e >> 1) & 1] = __fadd2_rn(s2[(e >> 1) & 1], make_float2(p0, p1));
-              pk[e / 2] = pack2<BF16>(p0, p1);
-            }
-            tmem_st16(tS + h * HC + 16 * ch, pk);
-          }
-          l = l * alpha + ((s2[0].x + s2[0].y) + (s2[1].x + s2[1].y));
-          tmem_st_wait();
-        }
-        if (hold) {
-          // Values that are not finite: O += p·v by hand for the rows that see
-          // them, then the rows of V are cleared for the product.
-          uint8_t* vt = smem + L::kOffKV + ((2 * x + 1) % NS) * L::kKV;
-          tc_fence_before();
-          named_sync(3, kSoft);  // all of P is stored
-          tc_fence_after();
-#pragma unroll 1
-          for (int n = 0; n < valid; ++n) {
-            if (!((mi.bad[x & 1][n >> 6] >> (n & 63)) & 1)) continue;
-            const uint32_t w = tmem_ld1(tS + n / HC * HC + (n % HC >> 1));
-            tmem_ld_wait();
-            const float pr = half_of<BF16>(w, n & 1);
-#pragma unroll 1
-            for (int i = 0; i < D / 32; ++i) {
-              const int col = h * (D / 2) + 16 * i;
-              uint32_t o16[16];
-              tmem_ld16(tO + 16 * i, o16);
-              tmem_ld_wait();
-#pragma unroll
-              for (int e8 = 0; e8 < 2; ++e8) {
-                const uint4 v = *reinterpret_cast<const uint4*>(vt + (col >> 6) * (CH * 128) + sw128_offset(n, ((col & 63) >> 3) + e8));
-                const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                  if (pr != 0.f)
-                    o16[8 * e8 + e] = __float_as_uint(__uint_as_float(o16[8 * e8 + e]) + pr * half_of<BF16>(vw[e >> 1], e & 1));
-              }
-              tmem_st16(tO + 16 * i, o16);
-              tmem_st_wait();
-            }
-          }
-          named_sync(3, kSoft);
-          for (int i = sid; i < valid * 8; i += kSoft)
-            if ((mi.bad[x & 1][i >> 9] >> ((i >> 3) & 63)) & 1)
-#pragma unroll
-              for (int sub = 0; sub < L::kSub; ++sub)
-                *reinterpret_cast<uint4*>(vt + sub * (CH * 128) + (i >> 3) * 128 + (i & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-          fence_async_shared();
-          named_sync(3, kSoft);
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          if (h == 0 || hold) mbar_arrive(bar(kPHalf + buf));
-          if (h == 1) mbar_arrive(bar(kPFull + buf));
-        }
-      }
-
-      // ------------------------------------------------------ the item ends
-      mi.sum[t][h][row] = l;
-      named_sync(1 + t, 256);
-      l = mi.sum[t][0][row] + mi.sum[t][1][row];
-      ok = ok && warp_wait(bar(kODone + (NT == 2 ? t : (x - 1) & 1)), (uint32_t)phase(x - 1), ctl);
-      tc_fence_after();
-      if (ok) {
-        const bool whole = cur.c == 0 && count == cur.n;
-        int hq, node;
-        const bool live = where(&hq, &node);
-        if (masks.anc[node] == 0) l = 0.f;  // absent: chunks that are not masked were summed for it too
-        const float inv = l > 0.f ? 1.f / l : 0.f;
-        const int64_t prow = ((int64_t)blockIdx.x * 2 + (cur.c > 0 ? 0 : 1)) * p.rb + t * kBM + row;
-        uint16_t* og = static_cast<uint16_t*>(p.o) + cur.b * p.so[0] + hq * p.so[1] + node * p.so[2] + h * (D / 2);
-        float* pg = p.part_o + prow * p.D + h * (D / 2);
-        const int d_end = live ? p.D - h * (D / 2) : 0;
-#pragma unroll 1
-        for (int c = 0; c < D / 64; ++c) {
-          uint32_t r[32];
-          tmem_ld32(tO + 32 * c, r);
-          tmem_ld_wait();
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int d = 32 * c + 8 * q;
-            if (d >= d_end) continue;
-            float f[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = inv > 0.f ? __uint_as_float(r[8 * q + e]) * inv : 0.f;
-            if (whole) {
-              *reinterpret_cast<uint4*>(og + d) =
-                  make_uint4(pack2<BF16>(f[0], f[1]), pack2<BF16>(f[2], f[3]), pack2<BF16>(f[4], f[5]), pack2<BF16>(f[6], f[7]));
-            } else {
-              *reinterpret_cast<float4*>(pg + d) = make_float4(f[0], f[1], f[2], f[3]);
-              *reinterpret_cast<float4*>(pg + d + 4) = make_float4(f[4], f[5], f[6], f[7]);
-            }
-          }
-          __syncwarp();
-        }
-        if (live && h == 0) {
-          const float l2 = l > 0.f ? m + lg2(l) : neg_inf();
-          if (!whole) p.part_lse[prow] = l2;
-          else if (p.lse)
-            p.lse[((int64_t)cur.b * p.Hq + hq) * p.N + node] =
-                l2 == neg_inf() ? l2 : l2 * kLn2 + tree_row_shift(p, hq, cur.len + masks.depth[node]);
-        }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kMaskFree + (seg & 1)));
-      cur.next(p, count);
-    }
-  }
-
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 2) {
-    tc_fence_after();
-    tmem_dealloc(tmem, 512);
-  }
-}
-
-constexpr uint64_t kTimeoutNs = 1000000000ull;
-
-template <int D, int NT, bool BF16>
-int launch(const TreeParams& p, int dtype, cudaStream_t st) {
-  using L = TreeLayout<D, NT>;
-  const int box = std::gcd(p.page, L::kCH);
-  CUtensorMap tm[4];
-  if (!make_tmap_bhsd(&tm[0], p.kp, dtype, p.D, p.page, p.Hkv, (int)p.num_pages, p.skp, box) ||
-      !make_tmap_bhsd(&tm[1], p.vp, dtype, p.D, p.page, p.Hkv, (int)p.num_pages, p.svp, box) ||
-      !make_tmap_bhsd(&tm[2], p.k, dtype, p.D, p.N, p.Hkv, p.B, p.sk, 64) ||
-      !make_tmap_bhsd(&tm[3], p.v, dtype, p.D, p.N, p.Hkv, p.B, p.sv, 64))
-    return BFA_ERR_CUDA;
-  const bool cap = p.soft_cap > 0.f, alibi = p.alibi != nullptr;
-  auto kernel = cap ? (alibi ? tree_kernel<D, NT, BF16, true, true> : tree_kernel<D, NT, BF16, true, false>)
-                    : (alibi ? tree_kernel<D, NT, BF16, false, true> : tree_kernel<D, NT, BF16, false, false>);
-  static std::atomic<uint64_t> done[4];
-  const int rc = allow_shared(kernel, (int)L::kBytes, done[2 * cap + alibi], "tree attention shared memory");
-  if (rc) return rc;
-  kernel<<<p.grid, L::kThreads, L::kBytes, st>>>(tm[0], tm[1], tm[2], tm[3], p, box, kTimeoutNs);
-  note_launch();
-  return launch_status("tree attention launch");
-}
-
-template <bool BF16>
-int launch_d(const TreeParams& p, int dtype, cudaStream_t st) {
-  const bool two = p.rb == 2 * kBM;
-  if (p.D <= 64) return two ? launch<64, 2, BF16>(p, dtype, st) : launch<64, 1, BF16>(p, dtype, st);
-  if (p.D <= 128) return two ? launch<128, 2, BF16>(p, dtype, st) : launch<128, 1, BF16>(p, dtype, st);
-  return launch<256, 1, BF16>(p, dtype, st);
-}
-
-}  // namespace
-
-TreeTile tree_sm100_tile(int64_t rows, int D) {
-  return {rows > kBM && D <= 128 ? 2 * kBM : kBM, D > 128 ? 64 : 128, 1};
+// Rows per block: 32 (stored four times), 128, or 256 (two tiles; O of two
+// tiles does not fit TMEM at head dim 256). Joining the four quarters costs
+// more the wider O is: at head dim 256 it pays only where the softmax is the
+// longer part, with a soft-cap (device times with and without the four copies:
+// B=16, 8 KV heads, one node: head dim 64, L=4096 45 and 57 us, head dim 128,
+// L=8192 95 and 104 us; head dim 256, B=8, L=4096 61 and 58 us, and 67 against
+// 69 us with a soft-cap, 15 nodes and a window).
+TreeTile tree_sm100_tile(int64_t rows, int D, bool cap) {
+  const bool four = rows <= 32 && (D <= 128 || cap);
+  return {four ? 32 : rows > 128 && D <= 128 ? 256 : 128, D > 128 ? 64 : 128, 1};
 }
 
 bool tree_sm100_layout(const bfa_tree_args* a) {
@@ -771,7 +30,9 @@ bool tree_sm100_layout(const bfa_tree_args* a) {
 }
 
 int tree_sm100(const TreeParams& p, int dtype, cudaStream_t st) {
-  return dtype == BFA_DTYPE_BF16 ? launch_d<true>(p, dtype, st) : launch_d<false>(p, dtype, st);
+  if (p.D <= 64) return tree_sm100_d64(p, dtype, st);
+  if (p.D <= 128) return tree_sm100_d128(p, dtype, st);
+  return tree_sm100_d256(p, dtype, st);
 }
 
 }  // namespace bfa

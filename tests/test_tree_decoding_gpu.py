@@ -19,10 +19,10 @@ from tree_reference import attention, dense, page_cache, verify
 DEV = "cuda:0"
 
 
-@pytest.fixture(params=["", "0", "1"], ids=["rule", "mma", "tcgen05"], autouse=True)
+@pytest.fixture(params=["", "0"], ids=["tcgen05", "mma"], autouse=True)
 def kernel(request, monkeypatch):
-    """Attention tests run by the library's own choice of kernel and on either
-    16-bit kernel at every size that its layouts allow."""
+    """Attention tests run on the kernel that the library chooses (tcgen05
+    wherever TMA can read the layouts) and on the mma.sync kernel."""
     name = request.node.name
     if request.param and ("verify" in name or "append" in name or "refusals" in name):
         pytest.skip("one kernel")
