@@ -437,19 +437,24 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
         return live;
       };
       {
-        // Half of q's row into the swizzled tile (its readers, the last item's
-        // S products, are done: their barrier was waited for).
+        // Half of q's rows of this warp into the swizzled tile (its readers, the
+        // last item's S products, are done: their barrier was waited for). The
+        // lanes take the 16-byte pieces of a row side by side: a lane per row
+        // would touch 32 lines with every load, and the page table's loads
+        // would queue behind them (5 us at the start of an item of 256 rows).
         int hq, node;
         const bool live = where(&hq, &node);
-        const uint4* src =
-            reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + cur.b * p.sq[0] + hq * p.sq[1] + node * p.sq[2]);
+        const int64_t mine = live ? cur.b * p.sq[0] + hq * p.sq[1] + node * p.sq[2] : -1;
         uint8_t* dst = smem + t * L::kQTile;
+        if (D == 64) named_sync(4 + 4 * t + wq, 64);  // the other half's rows of the last item have left these lines
+        constexpr int kPer = D / 16;  // pieces of a half row
 #pragma unroll 8
-        for (int i = 0; i < D / 16; ++i) {
-          const int c = h * (D / 16) + i;
+        for (int i = 0; i < kPer; ++i) {
+          const int idx = i * 32 + lane, r = idx / kPer, c = h * kPer + idx % kPer;
+          const int64_t at = __shfl_sync(0xffffffffu, mine, r);
           uint4 w = make_uint4(0u, 0u, 0u, 0u);
-          if (live && c * 8 < p.D) w = src[c];
-          *reinterpret_cast<uint4*>(dst + (c >> 3) * (kBM * 128) + sw128_offset(trow, c & 7)) = w;
+          if (at >= 0 && c * 8 < p.D) w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + at + c * 8);
+          *reinterpret_cast<uint4*>(dst + (c >> 3) * (kBM * 128) + sw128_offset(wq * 32 + r, c & 7)) = w;
         }
         fence_async_shared();
         __syncwarp();
@@ -753,33 +758,30 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
           m = top;
           l = sum;
         }
-        const int64_t prow = ((int64_t)blockIdx.x * 2 + (cur.c > 0 ? 0 : 1)) * p.rb + t * kBM + row;
-        uint16_t* og = static_cast<uint16_t*>(p.o) + cur.b * p.so[0] + hq * p.so[1] + node * p.so[2] + h * (D / 2);
-        float* pg = p.part_o + prow * p.D + h * (D / 2);
+        const int64_t prow0 = ((int64_t)blockIdx.x * 2 + (cur.c > 0 ? 0 : 1)) * p.rb + t * kBM;
+        const int64_t prow = prow0 + row;
+        // Where the row's half goes (elements), -1: not stored.
         const bool store = ok && live && (REP == 1 || wq == 0);
-        const int d_end = store ? p.D - h * (D / 2) : 0;
+        const int64_t place = !store ? -1 : whole ? cur.b * p.so[0] + hq * p.so[1] + node * p.so[2] : prow * p.D;
+        const int d0 = h * (D / 2);
+        uint16_t* og = static_cast<uint16_t*>(p.o);
         // 16 columns of O, scaled (an empty row is zero even where the values
         // that it does not see are not finite).
-        auto columns = [&](int c, float(&f)[16]) {
+        auto columns = [&](int c, float* f) {
           uint32_t r[16];
           tmem_ld16(tO + c, r);
           tmem_ld_wait();
 #pragma unroll
           for (int e = 0; e < 16; ++e) f[e] = scale > 0.f ? __uint_as_float(r[e]) * scale : 0.f;
         };
-        auto put = [&](int c, const float(&f)[16]) {
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const int d = c + 8 * q;
-            if (d >= d_end) continue;
-            const float* g = f + 8 * q;
-            if (whole) {
-              *reinterpret_cast<uint4*>(og + d) =
-                  make_uint4(pack2<BF16>(g[0], g[1]), pack2<BF16>(g[2], g[3]), pack2<BF16>(g[4], g[5]), pack2<BF16>(g[6], g[7]));
-            } else {
-              *reinterpret_cast<float4*>(pg + d) = make_float4(g[0], g[1], g[2], g[3]);
-              *reinterpret_cast<float4*>(pg + d + 4) = make_float4(g[4], g[5], g[6], g[7]);
-            }
+        auto put8 = [&](int64_t at, int d, const float4& x, const float4& y) {
+          if (at < 0 || d >= p.D) return;
+          if (whole) {
+            *reinterpret_cast<uint4*>(og + at + d) =
+                make_uint4(pack2<BF16>(x.x, x.y), pack2<BF16>(x.z, x.w), pack2<BF16>(y.x, y.y), pack2<BF16>(y.z, y.w));
+          } else {
+            *reinterpret_cast<float4*>(p.part_o + at + d) = x;
+            *reinterpret_cast<float4*>(p.part_o + at + d + 4) = y;
           }
         };
         if constexpr (REP == 4) {
@@ -804,16 +806,33 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
               for (int q = 0; q < 3; ++q)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) f[e] += join[((q * 2 + h) * (D / 4) + c - c0 + e) * 32 + lane];
-              put(c, f);
+#pragma unroll
+              for (int q = 0; q < 16; q += 8)
+                put8(place, d0 + c + q, make_float4(f[q], f[q + 1], f[q + 2], f[q + 3]), make_float4(f[q + 4], f[q + 5], f[q + 6], f[q + 7]));
             }
             named_sync(3, kSoft);
           }
         } else {
+          // Turned in shared memory, kW columns at a time, so that lanes side by
+          // side store one row's pieces (a lane per row: 32 lines a store). The
+          // place is this warp's own part of q's tile: no other warp reads it,
+          // or writes it before the next item's q.
+          constexpr int kW = D == 64 ? 16 : 32, kUnits = kW / 4;
+          uint8_t* turn = smem + t * L::kQTile + (D == 64 ? wq * 4096 + h * 2048 : h * (D / 128) * (kBM * 128) + wq * 4096);
+          auto unit = [&](int r, int u) { return reinterpret_cast<float4*>(turn + r * (kW * 4) + ((u ^ r) & (kUnits - 1)) * 16); };
 #pragma unroll 1
-          for (int c = 0; c < D / 2; c += 16) {
-            float f[16];
-            columns(c, f);
-            put(c, f);
+          for (int c = 0; c < D / 2; c += kW) {
+            float f[kW];
+#pragma unroll
+            for (int e = 0; e < kW; e += 16) columns(c + e, f + e);
+#pragma unroll
+            for (int u = 0; u < kUnits; ++u) *unit(lane, u) = make_float4(f[4 * u], f[4 * u + 1], f[4 * u + 2], f[4 * u + 3]);
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < kW / 8; ++i) {
+              const int idx = i * 32 + lane, r = idx / (kW / 8), u = idx % (kW / 8) * 2;
+              put8(__shfl_sync(0xffffffffu, place, r), d0 + c + 4 * u, *unit(r, u), *unit(r, u + 1));
+            }
             __syncwarp();
           }
         }
