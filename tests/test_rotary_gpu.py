@@ -181,3 +181,35 @@ def test_other_streams():
         got = rotary.rotary_embedding(q, k, cos, sin)
     st.synchronize()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
+def test_gradient_of_the_gradient():
+    """The backward is the transposed rotation, differentiable in its turn: the
+    gradient of <dq, v> in the output gradient is the rotation of v."""
+    cos, sin = rotary.rotary_table(64, 40, device=DEV)
+    q, k = make(2, 3, 1, 20, 64, torch.float32, seed=5)
+    v, u = make(2, 3, 1, 20, 64, torch.float32, seed=6)
+    q.requires_grad_(True), k.requires_grad_(True)
+    out = rotary.rotary_embedding(q, k, cos, sin)
+    g = [torch.randn_like(t).requires_grad_(True) for t in out]
+    dq, dk = torch.autograd.grad(out, (q, k), g, create_graph=True)
+    gg = torch.autograd.grad((dq * v).sum() + (dk * u).sum(), g)
+    pos = torch.arange(20, device=DEV)[None].expand(2, -1)
+    for got, x in zip(gg, (v, u)):
+        close(got, *exact(x, cos, sin, pos, False))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", [0, 1])
+def test_gradient_of_one_output(which):
+    """Only one of q', k' is used: the other input's gradient is None."""
+    cos, sin = rotary.rotary_table(64, 40, device=DEV)
+    q, k = make(1, 2, 2, 9, 64, torch.bfloat16, seed=7)
+    q.requires_grad_(True), k.requires_grad_(True)
+    out = rotary.rotary_embedding(q, k, cos, sin, interleaved=True)
+    w = torch.randn_like(out[which])
+    grads = torch.autograd.grad(out[which], (q, k), w, allow_unused=True)
+    pos = torch.arange(9, device=DEV)[None]
+    close(grads[which], *exact(w, cos, sin, pos, True, True))
+    assert grads[1 - which] is None

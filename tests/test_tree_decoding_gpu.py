@@ -205,6 +205,47 @@ def test_mixed_lengths_and_many_sequences(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("page", [8, 24, 40, 64, 192, 256])
+@pytest.mark.parametrize("D,N,Hq", [(128, 4, 4), (64, 20, 8), (256, 6, 2)])
+def test_page_sizes_and_windows(page, D, N, Hq):
+    """Pages smaller and larger than a chunk of keys, that divide it and that do
+    not, windows that begin inside a page, lengths that end inside one."""
+    check([1300, 257, 40], N, Hq, 1, D, BF, page, tree("binary", N, 3))
+    check([1300, 257, 40], N, Hq, 1, D, BF, page, tree("chain", N, 3), sliding_window=301)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("kw", [dict(), dict(soft_cap=20.0)])
+def test_row_counts_around_the_tiles(D, kw):
+    """Rows per KV head at and around 32, 128 and 256, where the tile changes."""
+    for N, G in ((32, 1), (33, 1), (31, 4), (32, 4), (43, 3), (64, 4), (52, 5)):
+        check([400, 70], N, G, 1, D, BF, 16, tree("binary", N, 2), seed=N * G, **kw)
+
+
+@pytest.mark.gpu
+def test_values_at_the_types_ends():
+    """Keys and queries whose logits reach +-10^4, an fp16 cache near its
+    largest value, and a soft-cap over them."""
+    g = gen(12)
+    for dtype, size in ((BF, 30.0), (HF, 30.0)):
+        cache = td.PagedKVCache(*page_cache([300], 320, 16, 1, 128, dtype, DEV, g))
+        cache.k_pages.mul_(size)
+        q = (torch.randn(1, 4, 5, 128, generator=g, device=DEV) * size).to(dtype)
+        k, v = (torch.randn(1, 1, 5, 128, generator=g, device=DEV).to(dtype) for _ in range(2))
+        parents = tree("binary", 5)
+        up = torch.tensor(parents, dtype=torch.int32, device=DEV)
+        for cap in (0.0, 50.0):
+            ro, rl, size_ = attention(q, k, v, cache, parents, cap=cap)
+            o, lse = td.tree_attention(q, k, v, cache, up, soft_cap=cap, return_lse=True)
+            # Logits near 10^4 carry an fp32 error of a few 2^-10, which moves
+            # probabilities by as much; with the cap at most 50 * 1e-5.
+            tol = 1.5 * U[dtype] * size_ + U[dtype] * ro.abs() + (2e-2 if cap == 0.0 else 1e-3) * (size_ + 1)
+            assert ((o.double() - ro).abs() <= tol).all()
+            assert ((lse.double() - rl).abs() <= 1e-5 * (1 + rl.abs()) + 1e-3).all()
+
+
+@pytest.mark.gpu
 def test_long_cache_and_peaked_rows():
     check([20011], 17, 4, 1, 128, BF, 64, tree("binary", 17), peak=3.0)
     check([9001], 64, 4, 1, 128, HF, 64, tree("binary", 64), peak=3.0)
