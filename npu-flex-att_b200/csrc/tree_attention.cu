@@ -193,10 +193,11 @@ template <typename T>
 int launch_merge(const TreeParams& p, cudaStream_t st) {
   const int64_t items = (int64_t)p.B * p.Hkv * p.n_rb;
   // Four warps per row where an item is spread over at least four blocks on
-  // average; a warp per row while all rows' warps fit the GPU at once (16
-  // blocks of 128 threads an SM), four rows a warp, one after another, above.
+  // average; else a warp per row, or four rows a warp where there are so many
+  // that the blocks' own start costs more (16384 rows: 1.2 to 2 us less with a
+  // warp per row, 32768: alike, 65536: 9 us more).
   const bool wide = p.grid >= 4 * items;
-  const int rows = wide ? 1 : items * std::min(p.rb, p.G * p.N) <= (int64_t)sm_count() * 64 ? 4 : 16;
+  const int rows = wide ? 1 : items * std::min(p.rb, p.G * p.N) <= (int64_t)sm_count() * 128 ? 4 : 16;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(items * ((std::min(p.rb, p.G * p.N) + rows - 1) / rows)));
   cfg.blockDim = dim3(128);
