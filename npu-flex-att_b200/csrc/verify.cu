@@ -27,7 +27,7 @@
 // takes the same decisions and results do not depend on scheduling.
 // Measured: one sequence, five nodes, 32768 entries 5.5 us, nearly all latency
 // (gather, walk, one pass); 64 sequences of 15 nodes, 131072 entries in fp32
-// 28 to 31 us for the 119 MB that the accepted paths read (59% of the copy rate:
+// 30 us for the 119 MB that the accepted paths read (59% of the copy rate:
 // sequences end their walks at different times and leave SMs idle).
 #include <cuda_runtime.h>
 
@@ -118,26 +118,37 @@ template <typename T, int V>
 struct alignas(V * sizeof(T)) Vec {
   T x[V];
 };
+// Entries p[0, V) as they are stored (converted where they are used: fewer
+// registers in flight).
 template <typename T, int V>
-__device__ __forceinline__ void load_vec(float (&f)[V], const T* p) {
+__device__ __forceinline__ Vec<T, V> load_vec(const T* p) {
+  Vec<T, V> t;
   if constexpr (V == 1) {
-    f[0] = to_f32<T>(*p);
+    t.x[0] = *p;
   } else {
     constexpr int kPer = 16 / (int)sizeof(T);
 #pragma unroll
     for (int i = 0; i < V / kPer; ++i) {
       const uint4 w = __ldg(reinterpret_cast<const uint4*>(p) + i);
-      Vec<T, kPer> t = *reinterpret_cast<const Vec<T, kPer>*>(&w);
+      const Vec<T, kPer> u = *reinterpret_cast<const Vec<T, kPer>*>(&w);
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) f[i * kPer + j] = to_f32<T>(t.x[j]);
+      for (int j = 0; j < kPer; ++j) t.x[i * kPer + j] = u.x[j];
     }
   }
+  return t;
 }
 
 // Entries per access: 16 bytes of T where every row allows it, else one.
 template <typename T, int E>
 __global__ void __launch_bounds__(kVerifyThreads, kVerifyPerSm) verify_kernel(const VerifyParams p) {
-  constexpr int kFinalUnroll = E == 1 ? 8 : 2;
+  // Accesses of a thread in flight together. One entry per access: those past
+  // the slice's end are predicated off, since a loop that only unrolls leaves
+  // its last, partial round to loads one after another (16 sequences of 50021
+  // entries in bf16 12.7 -> 10.7 us). Vectors have few rounds, and predicated
+  // ones were slower (64 sequences of 131072 30 -> 34 us): unrolled.
+  constexpr int kSumBatch = E == 1 ? 16 : 1, kDrawBatch = E == 1 ? 8 : 1;
+  constexpr int kSumUnroll = E == 1 ? 1 : 4, kDrawUnroll = E == 1 ? 1 : 2;
+  constexpr int kStep = kVerifyThreads * E;
   __shared__ Shared sh;
   const int tid = threadIdx.x;
   const uint32_t rank = cluster_rank();
@@ -194,13 +205,20 @@ __global__ void __launch_bounds__(kVerifyThreads, kVerifyPerSm) verify_kernel(co
         const T* pr = target + cur * p.st[1];
         const T* qr = draft + cur * p.sd[1];
         float sum = 0.f;
-#pragma unroll (E == 1 ? 8 : 4)
-        for (int v = lo + tid * E; v < hi; v += kVerifyThreads * E) {
-          float pv[E], qv[E];
-          load_vec<T, E>(pv, pr + v);
-          load_vec<T, E>(qv, qr + v);
+#pragma unroll kSumUnroll
+        for (int v0 = lo + tid * E; v0 < hi; v0 += kStep * kSumBatch) {
+          Vec<T, E> pv[kSumBatch], qv[kSumBatch];
 #pragma unroll
-          for (int i = 0; i < E; ++i) sum += fmaxf(pv[i] - a * qv[i], 0.f);
+          for (int j = 0; j < kSumBatch; ++j)
+            if (v0 + j * kStep < hi) {
+              pv[j] = load_vec<T, E>(pr + v0 + j * kStep);
+              qv[j] = load_vec<T, E>(qr + v0 + j * kStep);
+            }
+#pragma unroll
+          for (int j = 0; j < kSumBatch; ++j)
+            if (v0 + j * kStep < hi)
+#pragma unroll
+              for (int i = 0; i < E; ++i) sum += fmaxf(to_f32<T>(pv[j].x[i]) - a * to_f32<T>(qv[j].x[i]), 0.f);
         }
         w = __uint_as_float((uint32_t)combine<true>(sh, __float_as_uint(sum), round++));
         stale = false;
@@ -241,26 +259,38 @@ __global__ void __launch_bounds__(kVerifyThreads, kVerifyPerSm) verify_kernel(co
     const int use_gone = pass == 0 ? gone1 : gone0;
     float top = -1.f;
     int at = lo;
-#pragma unroll kFinalUnroll
-    for (int v = lo + tid * E; v < hi; v += kVerifyThreads * E) {
-      float pv[E], qv[E], ev[E];
-      load_vec<T, E>(pv, pr + v);
-      load_vec<float, E>(ev, noise + v);
-      if (use_q) {
-        load_vec<T, E>(qv, qr + v);
+#pragma unroll kDrawUnroll
+    for (int v0 = lo + tid * E; v0 < hi; v0 += kStep * kDrawBatch) {
+      Vec<T, E> pv[kDrawBatch], qv[kDrawBatch];
+      Vec<float, E> ev[kDrawBatch];
 #pragma unroll
-        for (int i = 0; i < E; ++i) pv[i] = pv[i] - a * qv[i];
-      }
+      for (int j = 0; j < kDrawBatch; ++j)
+        if (v0 + j * kStep < hi) {
+          pv[j] = load_vec<T, E>(pr + v0 + j * kStep);
+          ev[j] = load_vec<float, E>(noise + v0 + j * kStep);
+          if (use_q) qv[j] = load_vec<T, E>(qr + v0 + j * kStep);
+        }
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        float r = pv[i] > 0.f ? pv[i] / ev[i] : 0.f;
-        r = r >= 0.f ? r : 0.f;
-        if (r > top) {  // a few times per thread: only here the rejected tokens matter
-          bool out = false;
-          for (int g = gone0; g < use_gone; ++g) out |= sh.gone[g] == v + i;
-          if (!out) {
-            top = r;
-            at = v + i;
+      for (int j = 0; j < kDrawBatch; ++j) {
+        if (v0 + j * kStep >= hi) break;
+        float r[E], most = -1.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          float x = to_f32<T>(pv[j].x[i]);
+          if (use_q) x -= a * to_f32<T>(qv[j].x[i]);
+          r[i] = x > 0.f ? x / ev[j].x[i] : 0.f;
+          r[i] = r[i] >= 0.f ? r[i] : 0.f;
+          most = fmaxf(most, r[i]);
+        }
+        if (most > top) {  // a few times per thread: only here the rejected tokens matter
+#pragma unroll
+          for (int i = 0; i < E; ++i) {
+            bool out = !(r[i] > top);
+            for (int g = gone0; g < use_gone && !out; ++g) out = sh.gone[g] == v0 + j * kStep + i;
+            if (!out) {
+              top = r[i];
+              at = v0 + j * kStep + i;
+            }
           }
         }
       }
