@@ -223,82 +223,81 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
     // Lane i·kSub + s: columns [64s, 64s + 64) of box i, tokens [key0 + i·box,
     // + box) of one page (the tree's chunk: one box of 64 nodes).
     const int my_box = lane / L::kSub, my_sub = lane % L::kSub;
-    // The sequence's page table, 64 entries at a time: lane i holds entries
-    // wb + i and wb + 32 + i; the second half is loaded 32 pages before it is
-    // used.
-    int wb = 0, wseq = -1, w0 = 0, w1 = 0;
-    auto entry = [&](const TreeCursor& at, int pg) {
-      return (int64_t)pg * p.page < at.len ? p.table[at.b * p.table_stride + pg] : 0;
-    };
-    auto page_of = [&](int token) { return p.page_log2 >= 0 ? token >> p.page_log2 : token / p.page; };
-    auto fill = [&](const TreeCursor& at) {
-      if (at.in_tree(p)) return;
-      const int pg = page_of(at.key0(p));
-      if (at.b != wseq || pg < wb || pg >= wb + 64) {
-        wseq = at.b;
-        wb = pg;
-        w0 = entry(at, wb + lane);
-        w1 = entry(at, wb + 32 + lane);
-      } else if (pg >= wb + 32) {
-        w0 = w1;
-        wb += 32;
-        w1 = entry(at, wb + 32 + lane);
-      }
-    };
-    struct Box {
-      int page, slot;
-      bool mine;
-    };
-    auto find = [&](const TreeCursor& at) -> Box {
-      Box r{0, 0, false};
-      if (at.in_tree(p)) {
-        r.mine = my_box == 0;
-        return r;
-      }
-      const int t0 = at.key0(p) + my_box * box;
-      r.mine = my_box < CH / box && t0 < at.len;
-      const int pg = r.mine ? page_of(t0) : wb;
-      r.slot = t0 - pg * p.page;
-      r.page = __shfl_sync(0xffffffffu, w0, pg - wb);  // the lane is taken modulo 32
-      if (__any_sync(0xffffffffu, pg - wb >= 32)) {
-        const int v = __shfl_sync(0xffffffffu, w1, pg - wb);
-        if (pg - wb >= 32) r.page = v;
-      }
-      return r;
+    const int boxes = CH / box, per = 32 / boxes;  // powers of 2
+    // The boxes of `per` chunks of an item from its chunk `c`, one per lane:
+    // their pages (0 past the cache) and first tokens in them.
+    int page = 0, slot = 0, next_page = 0, next_slot = 0;
+    auto lookup = [&](const TreeCursor& at, int c) {
+      const int t = at.lo + c * CH + lane * box;
+      const int pg = p.page_log2 >= 0 ? t >> p.page_log2 : t / p.page;
+      next_slot = t - pg * p.page;
+      next_page = t < at.len ? p.table[at.b * p.table_stride + pg] : 0;
     };
     bool ok = true;
-    int n = kv;
-    if (n_x > 0) fill(cur);
-    for (int x = 0; x < n_x && ok; ++x) {
-      Box me = find(cur);
+    int x = 0, st = kv, round = 0;  // the next load's slot and that slot's round
+    auto begin = [&](uint32_t bytes) -> bool {
+      if (round > 0) ok = warp_wait(bar(kKVEmpty + st), (uint32_t)((round & 1) ^ 1), ctl);
+      if (ok && lane == 0) mbar_arrive_expect_tx(bar(kKVFull + st), bytes);
+      __syncwarp();
+      return ok;
+    };
+    auto end = [&]() {
+      __syncwarp();
+      ++x;
+      st += 2;
+      if (st >= NS) {
+        st -= NS;
+        ++round;
+      }
+    };
+    if (n_x > 0) lookup(cur, cur.c);
+    while (x < n_x && ok) {
       const TreeCursor here = cur;
-      cur.next(p);
-      if (x + 1 < n_x) fill(cur);  // in flight while this chunk's slots are waited for
-      const bool tree = here.in_tree(p);
+      const int count = min(here.n - here.c, n_x - x);
+      const int cached = min(max(here.n - p.tree_chunks - here.c, 0), count);
       const int hkv = here.item / p.n_rb;
-      if (!tree && me.mine && (me.page < 0 || me.page >= p.num_pages)) {
-        me.page = (int)p.num_pages;  // outside the tensor: reads as zeros
-        if (p.status) *p.status = BFA_ERR_INDEX;
+      const bool more = x + count < n_x;
+      // The next pages that will be needed, this item's or the next one's:
+      // looked up as soon as the last ones are in use.
+      auto ahead = [&](int it) {
+        if (it < cached) {
+          lookup(here, here.c + it);
+        } else {
+          cur.next(p, count);
+          if (more) lookup(cur, cur.c);
+        }
+      };
+      if (cached == 0) ahead(0);
+      for (int it = 0; it < cached; ++it) {
+        const int j = it & (per - 1);
+        if (j == 0) {
+          page = next_page;
+          slot = next_slot;
+          if (page < 0 || page >= p.num_pages) {
+            page = (int)p.num_pages;  // outside the tensor: reads as zeros
+            if (p.status) *p.status = BFA_ERR_INDEX;
+          }
+        }
+        const int pg = __shfl_sync(0xffffffffu, page, j * boxes + my_box);  // the lane is taken modulo 32
+        const int sl = __shfl_sync(0xffffffffu, slot, j * boxes + my_box);
+        const int left = here.len - (here.lo + (here.c + it) * CH);
+        const bool mine = my_box < boxes && my_box * box < left;
+        const uint32_t bytes = left >= CH ? L::kKV : (uint32_t)__popc(__ballot_sync(0xffffffffu, mine)) * box * 128u;
+        if (!begin(bytes)) break;
+        if (mine)
+          tma_load_4d(sbase + L::kOffKV + st * L::kKV + my_sub * (CH * 128) + my_box * box * 128, kv ? &tmVp : &tmKp,
+                      bar(kKVFull + st), my_sub * 64, sl, hkv, pg);
+        end();
+        if (j == 0) ahead(it + per);
       }
-      const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xffffffffu, me.mine)) * (tree ? 64 : box) * 128u;
-      n = 2 * x + kv;
-      const int st = n % NS;
-      if (n >= NS) {
-        int w = 1;
-        if (lane == 0) w = mbar_wait(bar(kKVEmpty + st), ((n / NS) & 1) ^ 1, ctl, BFA_ERR_DEVICE_TIMEOUT) ? 1 : 0;
-        ok = __shfl_sync(0xffffffffu, w, 0) != 0;
-        if (!ok) break;
+      if (ok && cached < count && begin(L::kSub * 64 * 128u)) {  // the tree
+        if (my_box == 0)
+          tma_load_4d(sbase + L::kOffKV + st * L::kKV + my_sub * (CH * 128), kv ? &tmV : &tmK, bar(kKVFull + st), my_sub * 64, 0, hkv,
+                      here.b);
+        end();
       }
-      if (lane == 0) mbar_arrive_expect_tx(bar(kKVFull + st), bytes);
-      __syncwarp();
-      if (me.mine) {
-        const uint32_t dst = sbase + L::kOffKV + st * L::kKV + my_sub * (CH * 128) + my_box * box * 128;
-        if (tree) tma_load_4d(dst, kv ? &tmV : &tmK, bar(kKVFull + st), my_sub * 64, 0, hkv, here.b);
-        else tma_load_4d(dst, kv ? &tmVp : &tmKp, bar(kKVFull + st), my_sub * 64, me.slot, hkv, me.page);
-      }
-      __syncwarp();
-      n += 2;  // the next one; past the last one issued after the loop
     }
+    const int n = 2 * x + kv;  // past the last load issued
     // This warp's loads among the block's last NS (one per slot; earlier ones
     // have been consumed, and their slots hold later loads of either producer)
     // have landed before the block may end.
