@@ -135,6 +135,16 @@ __device__ __forceinline__ void tmem_store(uint32_t taddr, const uint32_t (&r)[N
                  : "memory");
 }
 
+// One lane of a converged warp. The compiler knows that a branch on it holds one
+// thread, and issues tcgen05 and TMA instructions without a loop over the lanes
+// that may be active (a branch on lane 0: 72 against 61 us at head dim 64, B=16,
+// L=8192; 320 against 303 us on 512 rows).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return BF16 ? pack_bf16(a, b) : pack_f16(a, b);
@@ -306,7 +316,7 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
+    if (elect_one()) {
       constexpr uint32_t idS = idesc_f16(kBM, CH, BF16, false);
       constexpr uint32_t idO = idesc_f16(kBM, D, BF16, true);
       auto kv_addr = [&](int idx) -> uint32_t { return sbase + L::kOffKV + (uint32_t)(idx % NS) * L::kKV; };
@@ -332,10 +342,15 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
       auto pv = [&](int t, int buf, int x, int steps) {
         const uint64_t dv = desc_mnmajor(kv_addr(2 * x + 1), CH * 128);
         if (!wait(kPFull + buf, phase(x))) return false;
+        if (steps == CH / 16) {  // nearly always: no branch per product
 #pragma unroll
-        for (int kk = 0; kk < CH / 16; ++kk)
-          if (kk < steps)
+          for (int kk = 0; kk < CH / 16; ++kk)
             mma_ts(tmem + L::kTmemO + t * D, p_at(buf, kk / (CH / 32)) + kk % (CH / 32) * 8, dv + ((kk * 16 * 128) >> 4), idO, 1u);
+        } else {
+#pragma unroll 1
+          for (int kk = 0; kk < steps; ++kk)
+            mma_ts(tmem + L::kTmemO + t * D, p_at(buf, kk / (CH / 32)) + kk % (CH / 32) * 8, dv + ((kk * 16 * 128) >> 4), idO, 1u);
+        }
         mma_commit(bar(kODone + buf));
         return true;
       };
