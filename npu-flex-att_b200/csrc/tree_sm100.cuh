@@ -89,7 +89,7 @@ struct TreeLayout {
   static_assert(kStages >= 4, "K and V of two chunks");
   static_assert(kTmemP + (NT == 1 ? kCH : 0) <= 512, "TMEM");
   static_assert(REP == 1 || (REP == 4 && NT == 1), "rows");
-  static_assert(REP == 1 || 3 * 2 * 32 * (D / 4) * 4 <= kQTile, "the quarters' O are joined in q's tile");
+  static_assert(REP == 1 || 4 * 2 * 32 * (D / 4) * 4 <= kQTile, "the quarters' O are joined in q's tile");
   static_assert(kBytes <= 232448, "shared memory");
 };
 
@@ -766,7 +766,7 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
         const int64_t prow0 = ((int64_t)blockIdx.x * 2 + (cur.c > 0 ? 0 : 1)) * p.rb + t * kBM;
         const int64_t prow = prow0 + row;
         // Where the row's half goes (elements), -1: not stored.
-        const bool store = ok && live && (REP == 1 || wq == 0);
+        const bool store = ok && live;
         const int64_t place = !store ? -1 : whole ? cur.b * p.so[0] + hq * p.so[1] + node * p.so[2] : prow * p.D;
         const int d0 = h * (D / 2);
         uint16_t* og = static_cast<uint16_t*>(p.o);
@@ -790,30 +790,34 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
           }
         };
         if constexpr (REP == 4) {
-          // Joined in q's tile (its readers are done), in the order of the
-          // quarters: [quarter - 1][half][column][lane], D / 4 columns at a time.
-          float* join = reinterpret_cast<float*>(smem);
+          // Joined in q's tile (its readers are done), D / 4 columns of each half
+          // at a time: [quarter][row][16-byte unit of the row's D / 2 columns,
+          // swizzled]. Every thread then adds the quarters, in their order, of
+          // 8 columns of a row; threads side by side store one row's pieces.
+          constexpr int kU = D / 8;
+          float4* join = reinterpret_cast<float4*>(smem);
+          auto unit = [&](int q, int r, int u) { return join + (q * 32 + r) * kU + (u ^ (r & 7)); };
 #pragma unroll 1
           for (int c0 = 0; c0 < D / 2; c0 += D / 4) {
-#pragma unroll 1
-            for (int c = c0; c < c0 + D / 4 && wq > 0; c += 16) {
-              float f[16];
-              columns(c, f);
 #pragma unroll
-              for (int e = 0; e < 16; ++e) join[(((wq - 1) * 2 + h) * (D / 4) + c - c0 + e) * 32 + lane] = f[e];
+            for (int c = 0; c < D / 4; c += 16) {
+              float f[16];
+              columns(c0 + c, f);
+#pragma unroll
+              for (int e = 0; e < 16; e += 4) *unit(wq, lane, h * (kU / 2) + (c + e) / 4) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
             }
             named_sync(3, kSoft);
-#pragma unroll 1
-            for (int c = c0; c < c0 + D / 4 && wq == 0; c += 16) {
-              float f[16];
-              columns(c, f);
 #pragma unroll
-              for (int q = 0; q < 3; ++q)
+            for (int i = sid; i < 32 * (kU / 2); i += kSoft) {  // whole warps
+              const int r = i / (kU / 2), u = i % (kU / 2) * 2;
+              float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) f[e] += join[((q * 2 + h) * (D / 4) + c - c0 + e) * 32 + lane];
-#pragma unroll
-              for (int q = 0; q < 16; q += 8)
-                put8(place, d0 + c + q, make_float4(f[q], f[q + 1], f[q + 2], f[q + 3]), make_float4(f[q + 4], f[q + 5], f[q + 6], f[q + 7]));
+              for (int q = 0; q < 4; ++q) {
+                const float4 a = *unit(q, r, u), b = *unit(q, r, u + 1);
+                x.x += a.x, x.y += a.y, x.z += a.z, x.w += a.w;
+                y.x += b.x, y.y += b.y, y.z += b.z, y.w += b.w;
+              }
+              put8(__shfl_sync(0xffffffffu, place, r), u / (kU / 2) * (D / 2) + c0 + u % (kU / 2) * 4, x, y);
             }
             named_sync(3, kSoft);
           }
@@ -841,7 +845,7 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
             __syncwarp();
           }
         }
-        if (store && h == 0) {
+        if (store && h == 0 && (REP == 1 || wq == 0)) {
           const float l2 = l > 0.f ? m + lg2(l) : neg_inf();
           if (!whole) p.part_lse[prow] = l2;
           else if (p.lse)
