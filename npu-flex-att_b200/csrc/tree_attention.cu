@@ -23,7 +23,7 @@ namespace {
 // else 1). Launched to start under the attention kernel's tail: what it needs
 // of the inputs alone comes before it waits for the partials.
 template <typename T, int kWarps, int kVec, int kMergeRows>
-__global__ void __launch_bounds__(128) tree_merge_kernel(const TreeParams p) {
+__global__ void __launch_bounds__(128, 7) tree_merge_kernel(const TreeParams p) {
   constexpr int kLoads = kVec == 4 ? 2 : 8;  // of 32·kVec columns: 256
   __shared__ float part[4][kVec * kLoads * 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % kWarps;
@@ -51,6 +51,25 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeParams p) {
     const int r = row0 + rr;
     if (r >= p.rb || rb0 + r >= GN) break;  // alike for the warps of a row
     auto slot = [&](int i) { return ((int64_t)i * 2 + (i == i0 ? 1 : 0)) * p.rb + r; };
+    // kBatch partial results in flight, those past the last predicated off (an
+    // item mostly has two to six; a loop that only unrolls would take them one
+    // after another: one token over 4095 14.4 -> 13.1 us), the first ones beside
+    // the LSEs.
+    constexpr int kBatch = kWarps > 1 ? 4 : 2;
+    float f[kBatch][kLoads][kVec];
+    auto fetch = [&](int j0, int j, int n) {
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k, j += kWarps)
+#pragma unroll
+        for (int c = 0; c < kLoads; ++c) {
+          const int d = (lane + 32 * c) * kVec;
+          if (j >= n || d >= p.D) continue;
+          const float* po = p.part_o + slot(j0 + j) * p.D + d;
+          if constexpr (kVec == 4) *reinterpret_cast<float4*>(f[k][c]) = *reinterpret_cast<const float4*>(po);
+          else f[k][c][0] = *po;
+        }
+    };
+    fetch(i0, sub, min(32, i1 - i0 + 1));
     float m = neg_inf();
     for (int i = i0 + lane; i <= i1; i += 32) m = fmaxf(m, p.part_lse[slot(i)]);
 #pragma unroll
@@ -68,19 +87,18 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeParams p) {
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         total += sum;
         const int n = min(32, i1 - j0 + 1);
-#pragma unroll 8
-        for (int j = sub; j < n; j += kWarps) {
-          const float wj = __shfl_sync(0xffffffffu, w, j);
-          const float* po = p.part_o + slot(j0 + j) * p.D;
+        for (int j = sub; j < n; j += kBatch * kWarps) {
+          if (j0 > i0 || j > sub) fetch(j0, j, n);
 #pragma unroll
-          for (int c = 0; c < kLoads; ++c) {
-            const int d = (lane + 32 * c) * kVec;
-            if (d >= p.D) continue;
-            float f[kVec];
-            if constexpr (kVec == 4) *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(po + d);
-            else f[0] = po[d];
+          for (int k = 0; k < kBatch; ++k) {
+            if (j + k * kWarps >= n) break;
+            const float wj = __shfl_sync(0xffffffffu, w, j + k * kWarps);
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) acc[c][e] = fmaf(wj, f[e], acc[c][e]);
+            for (int c = 0; c < kLoads; ++c) {
+              if ((lane + 32 * c) * kVec >= p.D) continue;
+#pragma unroll
+              for (int e = 0; e < kVec; ++e) acc[c][e] = fmaf(wj, f[k][c][e], acc[c][e]);
+            }
           }
         }
       }
@@ -193,11 +211,15 @@ template <typename T>
 int launch_merge(const TreeParams& p, cudaStream_t st) {
   const int64_t items = (int64_t)p.B * p.Hkv * p.n_rb;
   // Four warps per row where an item is spread over at least four blocks on
-  // average; else a warp per row, or four rows a warp where there are so many
-  // that the blocks' own start costs more (16384 rows: 1.2 to 2 us less with a
-  // warp per row, 32768: alike, 65536: 9 us more).
-  const bool wide = p.grid >= 4 * items;
-  const int rows = wide ? 1 : items * std::min(p.rb, p.G * p.N) <= (int64_t)sm_count() * 128 ? 4 : 16;
+  // average and all rows' blocks are resident at once (7 per SM; 4096 rows with
+  // 5 partial results each 30 us with a warp per row, 37 with four, the
+  // attention included, 512 rows 38 against 41); else a warp per row, or four
+  // rows a warp where there are so many that the blocks' own start costs more
+  // (16384 rows: 1.2 to 2 us less with a warp per row, 32768: alike, 65536: 9 us
+  // more).
+  const int64_t all = items * std::min(p.rb, p.G * p.N);
+  const bool wide = p.grid >= 4 * items && all <= (int64_t)sm_count() * 7;
+  const int rows = wide ? 1 : all <= (int64_t)sm_count() * 128 ? 4 : 16;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(items * ((std::min(p.rb, p.G * p.N) + rows - 1) / rows)));
   cfg.blockDim = dim3(128);
@@ -244,8 +266,8 @@ extern "C" int bfa_tree_fwd(const bfa_tree_args* a, void* stream) {
   const int64_t rows = a->heads_q / a->heads_kv * a->nodes;
   const bool f32 = a->dtype == BFA_DTYPE_F32;
   // tcgen05 wherever TMA can read the layouts: it was the faster one at every
-  // size tried (B=16, L=8192, 8 KV heads of 128: 4 rows a KV head 95 against
-  // 125 us, 64 rows 109 against 184, 256 rows 195 against 551).
+  // size tried (B=16, L=8192, 8 KV heads of 128: 4 rows a KV head 91 against
+  // 125 us, 64 rows 103 against 184, 256 rows 171 against 551).
   const bool tc = !f32 && tcgen05_on() && tree_sm100_layout(a);
   const Plan pl = make_plan(a, f32  ? simt_tile(a)
                                : tc ? tree_sm100_tile(rows, (int)a->head_dim, a->soft_cap > 0)

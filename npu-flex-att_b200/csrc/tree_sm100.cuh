@@ -8,11 +8,12 @@
 //
 // Bound: HBM (K/V read once) up to about 256 rows per KV head, the tensor cores
 // above. Measured with its merge, bf16, 8 KV heads of 128, B=16, L=8192 (537 MB
-// of K/V): 4 to 32 rows per KV head 95 to 100 us (86 to 82% of the HBM floor),
-// 64 rows 109, 128 rows 117; 256 rows 185 us, where one tile's chain of softmax
-// and products sets the pace (2.6 us per 128 keys for 1.1 us of products). A call
-// that reads next to nothing takes 15 us: launch, work split, page table, one
-// chunk, merge, each waiting for the one before.
+// of K/V): 4 to 32 rows per KV head 91 to 94 us (90 to 87% of the HBM floor),
+// 64 rows 103, 128 rows 113; 256 rows 171 us, where one tile's chain of softmax
+// and products sets the pace (2.4 us per 128 keys for 1.1 us of products). Head
+// dim 64, L=8192, 16 rows (268 MB): 61 us, the softmax's chain of latencies, 0.85
+// us per chunk. A call that reads next to nothing takes 13 us: launch, work
+// split, page table, one chunk, merge, each waiting for the one before.
 //
 // Split. Persistent blocks, one per SM, each with an equal stretch of the list
 // of chunks (tree_common.cuh). Warp roles:
