@@ -644,15 +644,16 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
         const float m_use = m_new == neg_inf() ? 0.f : m_new;
         const float alpha = ex2(m - m_use);
         m = m_new;
-        // O may be rescaled once the last P·V is done. NT = 2: S of this chunk
-        // was issued after it, so it is. NT = 1: only a rescale waits for it;
-        // every chunk waits for the one before, long done, so that no phase of
-        // the barriers is passed over.
+        // O may be rescaled, or added to by hand (below), once the last P·V is
+        // done. NT = 2: S of this chunk was issued after it, so it is. NT = 1: S
+        // was issued before it, and only what touches O waits for it; every
+        // chunk waits for the one before, long done, so that no phase of the
+        // barriers is passed over.
         if (NT == 2) {
           if (it > 0) ok = ok && warp_wait(bar(kODone + buf), (uint32_t)phase(x - 1), ctl);
         } else {
           if (x > 1) ok = ok && warp_wait(bar(kODone + buf), (uint32_t)phase(x - 2), ctl);
-          if (rescale) ok = ok && warp_wait(bar(kODone + (buf ^ 1)), (uint32_t)phase(x - 1), ctl);
+          if (rescale || (hold && it > 0)) ok = ok && warp_wait(bar(kODone + (buf ^ 1)), (uint32_t)phase(x - 1), ctl);
         }
         tc_fence_after();
         if (rescale) {
