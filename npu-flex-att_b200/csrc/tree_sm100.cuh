@@ -100,7 +100,7 @@ struct TreeMisc {
   uint64_t bar[40];
   uint32_t tmem;
   int abort;
-  unsigned long long bad[2][2];  // by the chunk's parity: its keys whose values are not finite
+  unsigned long long bad[3][2];  // by the chunk's number mod 3: its keys whose values are not finite
   float top[2][2][2][kBM];       // row maxima: chunk's parity, tile, half of the keys, row
   float sum[2][2][kBM];          // row sums at an item's end: tile, half, row
   float quarter[2][kBM];         // REP = 4: maxima and sums of the quarters
@@ -513,7 +513,10 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
         if (differ || (!tree && (valid & 15))) {
           ok = ok && warp_wait(bar(kKVFull + (2 * x + 1) % NS), (uint32_t)(((2 * x + 1) / NS) & 1), ctl);
           uint8_t* vt = smem + L::kOffKV + ((2 * x + 1) % NS) * L::kKV;
-          unsigned long long* bad = mi.bad[x & 1];  // the other one may still be read by a slower warp
+          // A warp that clears this has seen S(x - 1), which is issued after
+          // every warp has stored P of chunk x - 3 (the slot's last use); one of
+          // chunk x - 2 may still be on its way to read its own slot.
+          unsigned long long* bad = mi.bad[x % 3];
           if (sid < 2) bad[sid] = 0ull;
           named_sync(3, kSoft);
           // Piece i: 16 bytes of row i / 8 of a 64-column sub-tile.
@@ -701,7 +704,7 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
           tc_fence_after();
 #pragma unroll 1
           for (int n = 0; n < valid; ++n) {
-            if (!((mi.bad[x & 1][n >> 6] >> (n & 63)) & 1)) continue;
+            if (!((mi.bad[x % 3][n >> 6] >> (n & 63)) & 1)) continue;
             const uint32_t w = tmem_ld1(p_at(buf, n / HC) + lane_base + (n % HC >> 1));
             tmem_ld_wait();
             const float pr = half_of<BF16>(w, n & 1);
@@ -726,7 +729,7 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
           }
           named_sync(3, kSoft);
           for (int i = sid; i < valid * 8; i += kSoft)
-            if ((mi.bad[x & 1][i >> 9] >> ((i >> 3) & 63)) & 1)
+            if ((mi.bad[x % 3][i >> 9] >> ((i >> 3) & 63)) & 1)
 #pragma unroll
               for (int sub = 0; sub < L::kSub; ++sub)
                 *reinterpret_cast<uint4*>(vt + sub * (CH * 128) + (i >> 3) * 128 + (i & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);

@@ -75,3 +75,28 @@ def test_bad_cached_values_at_the_windows_edge(dtype, bad, N, Hq, D, window):
         o, lse = td.tree_attention(q, k, v, cache, up, sliding_window=window, return_lse=True)
         compare(o[keep], lse[keep], ref[0][keep], ref[1][keep], ref[2][keep])
     nfa.check_device_status(DEV)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("N,Hq,D,window", [(20, 1, 64, 200), (20, 1, 128, 200), (40, 3, 128, 200), (64, 4, 128, 200), (20, 4, 256, 100)])
+def test_bad_values_two_chunks_apart(dtype, N, Hq, D, window):
+    """The window's edge and the tree hold them, the whole chunk between does
+    not: each chunk's own are found, none left over from the other."""
+    n = 1152  # whole chunks: the window's first one, one that every row sees, the tree
+    q, k, v, cache, parents, up = problem([n] * 3, N, Hq, D, dtype, "chain", 23)
+    ref = attention(q, k, v, cache, parents, window=window)
+    keep = torch.ones(3, Hq, N, dtype=torch.bool, device=DEV)
+    depth = torch.arange(N, device=DEV)
+    for b in range(3):
+        at = n - window + 3 + b
+        if b != 1:
+            cache.v_pages[slot(cache, b, at)] = math.nan
+            keep[b] &= (n + depth - at > window)[None]
+        if b != 2:
+            v[b, :, N - 2 + b] = math.inf
+            keep[b] &= (depth < N - 2 + b)[None]
+    for _ in range(3):
+        o, lse = td.tree_attention(q, k, v, cache, up, sliding_window=window, return_lse=True)
+        compare(o[keep], lse[keep], ref[0][keep], ref[1][keep], ref[2][keep])
+    nfa.check_device_status(DEV)
