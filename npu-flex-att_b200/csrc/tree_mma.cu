@@ -170,8 +170,10 @@ __global__ void __launch_bounds__(32 * RW * KW, (Tile<D, RW, KW>::kPerSm)) tree_
           const char* kr = krow[buf * kKeys + n0 + i * kRowsPerPass];
           const char* vr = vrow[buf * kKeys + n0 + i * kRowsPerPass];
           const uint32_t d = dst + (uint32_t)(i * kRowsPerPass * L::kRowBytes);
-          cp_async16(d, kr ? kr + pc * 16 : static_cast<const char*>(p.q), kr ? 16 : 0);
-          cp_async16(d + L::kTileBytes, vr ? vr + pc * 16 : static_cast<const char*>(p.q), vr ? 16 : 0);
+          // No row: zeros, from an address that is on the 16-byte grid like the
+          // others (the copy asks for that even where it reads nothing).
+          cp_async16(d, kr ? kr + pc * 16 : static_cast<const char*>(p.k), kr ? 16 : 0);
+          cp_async16(d + L::kTileBytes, vr ? vr + pc * 16 : static_cast<const char*>(p.k), vr ? 16 : 0);
         }
       }
     } else {

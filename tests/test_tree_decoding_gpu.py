@@ -574,3 +574,22 @@ def test_append_refusals_and_bad_indices():
     with pytest.raises(RuntimeError):
         td.cache_append(cache, k.float(), v.float())
     assert td.cache_append(cache, k[:, :, :0], v[:, :, :0]).tolist() == ln.tolist()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("D,N,Hq", [(64, 5, 4), (128, 3, 8), (256, 20, 4), (80, 9, 2)])
+def test_queries_off_the_grid(dtype, D, N, Hq):
+    """Only q lies off the 16-byte grid (odd element offsets): K, V and the pages
+    are still read in vectors, with missing rows in nearly every chunk."""
+    g = gen(14)
+    lens = [100, 37, 0]
+    cache = td.PagedKVCache(*page_cache(lens, 128, 16, 2, D, dtype, DEV, g))
+    k, v = (torch.randn(3, 2, N, D, generator=g, device=DEV).to(dtype) for _ in range(2))
+    parents = tree("binary", N, 3)
+    up = torch.tensor(parents, dtype=torch.int32, device=DEV)
+    for offset in (1, 3, 6):
+        flat = torch.randn(3 * Hq * N * D + offset, generator=g, device=DEV).to(dtype)
+        q = flat[offset:].view(3, Hq, N, D)
+        compare(*td.tree_attention(q, k, v, cache, up, return_lse=True), *attention(q, k, v, cache, parents))
+    nfa.check_device_status(DEV)
