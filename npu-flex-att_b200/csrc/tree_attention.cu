@@ -71,9 +71,16 @@ __global__ void __launch_bounds__(128, 7) tree_merge_kernel(const TreeParams p) 
     };
     fetch(i0, sub, min(32, i1 - i0 + 1));
     float m = neg_inf();
-    for (int i = i0 + lane; i <= i1; i += 32) m = fmaxf(m, p.part_lse[slot(i)]);
+    bool nan = false;
+    for (int i = i0 + lane; i <= i1; i += 32) {
+      const float x = p.part_lse[slot(i)];
+      nan |= x != x;
+      m = fmaxf(m, x);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    // A NaN among them, which the maximum leaves out, makes the sums NaN.
+    if (__any_sync(0xffffffffu, nan) && m == neg_inf()) m = 0.f;
     float total = 0.f, acc[kLoads][kVec];
 #pragma unroll
     for (int c = 0; c < kLoads; ++c)
@@ -121,7 +128,7 @@ __global__ void __launch_bounds__(128, 7) tree_merge_kernel(const TreeParams p) 
     int hq, n;
     tree_row(p, hkv, rb0 + r, &hq, &n);
     T* out = static_cast<T*>(p.o) + b * p.so[0] + hq * p.so[1] + n * p.so[2];
-    const float inv = total > 0.f ? 1.f / total : 0.f;
+    const float inv = total != 0.f ? 1.f / total : 0.f;  // 0: no part of the row saw anything
 #pragma unroll
     for (int c = 0; c < kLoads; ++c)
 #pragma unroll
@@ -131,7 +138,7 @@ __global__ void __launch_bounds__(128, 7) tree_merge_kernel(const TreeParams p) 
       }
     if (lane == 0 && p.lse) {
       float l = neg_inf();
-      if (total > 0.f) {
+      if (total != 0.f) {
         l = (m + log2f(total)) * kLn2;
         if (p.alibi) {  // the row's depth, by the way up to the root
           int depth = 0;

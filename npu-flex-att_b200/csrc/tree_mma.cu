@@ -525,7 +525,9 @@ __global__ void __launch_bounds__(32 * RW * KW, (Tile<D, RW, KW>::kPerSm)) tree_
       for (int h = 0; h < 2; ++h) {
         const int r = rw * 16 + g + 8 * h;
         if (r >= R) continue;
-        const float inv = l[h] > 0.f ? 1.f / l[h] : 0.f;
+        // l = 0: the row saw nothing and is empty. NaN (a logit that it saw was
+        // NaN or +inf) goes on into O and LSE.
+        const float inv = l[h] != 0.f ? 1.f / l[h] : 0.f;
         int hq, n;
         tree_row(p, hkv, rb0 + r, &hq, &n);
         uint16_t* og = static_cast<uint16_t*>(p.o) + seq * p.so[0] + hq * p.so[1] + n * p.so[2];
@@ -535,7 +537,7 @@ __global__ void __launch_bounds__(32 * RW * KW, (Tile<D, RW, KW>::kPerSm)) tree_
           const int c = 8 * i + 2 * t;
           if (c >= p.D) continue;
           // An empty row is zero even where the values it does not see are not finite.
-          const float a = inv > 0.f ? o[i][2 * h] * inv : 0.f, b = inv > 0.f ? o[i][2 * h + 1] * inv : 0.f;
+          const float a = inv != 0.f ? o[i][2 * h] * inv : 0.f, b = inv != 0.f ? o[i][2 * h + 1] * inv : 0.f;
           if (whole) {
             const uint32_t w = pack2<T>(a, b);
             if (fl.pair) {
@@ -552,7 +554,7 @@ __global__ void __launch_bounds__(32 * RW * KW, (Tile<D, RW, KW>::kPerSm)) tree_
           }
         }
         if (t == 0) {
-          const float l2 = l[h] > 0.f ? m[h] + __log2f(l[h]) : neg_inf();
+          const float l2 = l[h] != 0.f ? m[h] + __log2f(l[h]) : neg_inf();
           if (!whole) p.part_lse[prow + r] = l2;
           else if (p.lse)
             p.lse[((int64_t)seq * p.Hq + hq) * p.N + n] =

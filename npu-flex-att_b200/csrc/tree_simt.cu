@@ -233,8 +233,10 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const TreeParams p,
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
       if (lane == 0) {
-        sh.alpha[4 * warp + i] = l > 0.f ? 1.f / l : 0.f;
-        sh.p[0][4 * warp + i] = l > 0.f ? row_m[i] + log2f(l) : neg_inf();
+        // l = 0: the row saw nothing and is empty. NaN (a logit that it saw was
+        // NaN or +inf) goes on into O and LSE.
+        sh.alpha[4 * warp + i] = l != 0.f ? 1.f / l : 0.f;
+        sh.p[0][4 * warp + i] = l != 0.f ? row_m[i] + log2f(l) : neg_inf();
       }
     }
     __syncthreads();
@@ -253,7 +255,7 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const TreeParams p,
         for (int c = 0; c < kC; ++c) {
           const int d = pg * kC + c;
           if (d >= p.D) continue;
-          const float o = inv > 0.f ? acc[a][i][c] * inv : 0.f;
+          const float o = inv != 0.f ? acc[a][i][c] * inv : 0.f;
           if (whole)
             static_cast<T*>(p.o)[done.b * p.so[0] + hq * p.so[1] + n * p.so[2] + d] = from_f32<T>(o);
           else

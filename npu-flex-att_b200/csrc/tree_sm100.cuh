@@ -752,11 +752,13 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
         int hq, node;
         const bool live = where(&hq, &node);
         if (masks.anc[node] == 0) l = 0.f;  // absent: chunks that are not masked were summed for it too
-        float scale = l > 0.f ? 1.f / l : 0.f;  // of this lane's O
+        // Only a row that saw nothing has l = 0, and is empty; l is NaN where a
+        // logit that the row saw was NaN or +inf, and stays so, in O and LSE.
+        float scale = l != 0.f ? 1.f / l : 0.f;  // of this lane's O
         if constexpr (REP == 4) {
           // The quarters' maxima and sums: weights 2^(m - top) / sum.
           if (h == 0) {
-            mi.quarter[0][trow] = l > 0.f ? m : neg_inf();
+            mi.quarter[0][trow] = l != 0.f ? m : neg_inf();
             mi.quarter[1][trow] = l;
           }
           named_sync(3, kSoft);
@@ -766,7 +768,7 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
           const float use = top == neg_inf() ? 0.f : top;
 #pragma unroll
           for (int q = 0; q < 4; ++q) sum += mi.quarter[1][q * 32 + lane] * ex2(mi.quarter[0][q * 32 + lane] - use);
-          scale = l > 0.f ? ex2(m - use) / sum : 0.f;
+          scale = l != 0.f ? ex2(m - use) / sum : 0.f;
           m = top;
           l = sum;
         }
@@ -784,7 +786,7 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
           tmem_ld16(tO + c, r);
           tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 16; ++e) f[e] = scale > 0.f ? __uint_as_float(r[e]) * scale : 0.f;
+          for (int e = 0; e < 16; ++e) f[e] = scale != 0.f ? __uint_as_float(r[e]) * scale : 0.f;
         };
         auto put8 = [&](int64_t at, int d, const float4& x, const float4& y) {
           if (at < 0 || d >= p.D) return;
@@ -853,7 +855,7 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
           }
         }
         if (store && h == 0 && (REP == 1 || wq == 0)) {
-          const float l2 = l > 0.f ? m + lg2(l) : neg_inf();
+          const float l2 = l != 0.f ? m + lg2(l) : neg_inf();
           if (!whole) p.part_lse[prow] = l2;
           else if (p.lse)
             p.lse[((int64_t)cur.b * p.Hq + hq) * p.N + node] =

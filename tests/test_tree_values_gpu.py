@@ -100,3 +100,50 @@ def test_bad_values_two_chunks_apart(dtype, N, Hq, D, window):
         o, lse = td.tree_attention(q, k, v, cache, up, sliding_window=window, return_lse=True)
         compare(o[keep], lse[keep], ref[0][keep], ref[1][keep], ref[2][keep])
     nfa.check_device_status(DEV)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("bad", BAD)
+@pytest.mark.parametrize("lens", [[3000], [20] * 170, [500, 0, 90]], ids=["split", "whole", "mixed"])
+@pytest.mark.parametrize("N,Hq,D", [(5, 2, 64), (40, 2, 128), (64, 4, 128), (6, 2, 256)])
+def test_logits_that_are_no_numbers_are_passed_on(dtype, bad, lens, N, Hq, D):
+    """A query or a visible key that is not finite gives NaN in O and LSE of
+    every row that sees it, whole or split over blocks, and leaves the others."""
+    q, k, v, cache, parents, up = problem(lens, N, Hq, D, dtype, "binary", 24)
+    ref = attention(q, k, v, cache, parents) if len(lens) < 10 else None
+    clean = td.tree_attention(q, k, v, cache, up, return_lse=True)
+    sees = torch.zeros(len(lens), Hq, N, dtype=torch.bool, device=DEV)
+    q[0, 1, 3] = bad                                                   # one row
+    sees[0, 1, 3] = True
+    below = [n for n, way in enumerate(climb(parents[0])) if 2 in way]  # a node and those under it
+    last = len(lens) - 1
+    k[last, :, 2] = bad
+    sees[last][:, below] = True
+    if lens[0] > 100:                                                  # a cached key: all of a sequence's rows
+        cache.k_pages[slot(cache, 0, lens[0] // 2)] = bad
+        sees[0] = True
+    o, lse = td.tree_attention(q, k, v, cache, up, return_lse=True)
+    assert o[sees].isnan().all() and lse[sees].isnan().all()
+    assert torch.equal(o[~sees], clean[0][~sees]) and torch.equal(lse[~sees], clean[1][~sees])
+    if ref is not None:
+        compare(o[~sees], lse[~sees], ref[0][~sees], ref[1][~sees], ref[2][~sees])
+    nfa.check_device_status(DEV)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("kw", [dict(soft_cap=20.0), dict(alibi=-0.1), dict(sliding_window=100)])
+def test_logits_that_are_no_numbers_in_the_other_forms(dtype, kw):
+    q, k, v, cache, parents, up = problem([1500, 30], 9, 2, 128, dtype, "binary", 25)
+    kw = dict(kw)
+    if "alibi" in kw:
+        kw["alibi_slope"] = torch.tensor([1.0, 0.5], device=DEV) * kw.pop("alibi")
+    clean = td.tree_attention(q, k, v, cache, up, return_lse=True, **kw)
+    q[1, 0, 4] = math.nan
+    cache.k_pages[slot(cache, 0, 1450)] = math.nan
+    sees = torch.zeros(2, 2, 9, dtype=torch.bool, device=DEV)
+    sees[1, 0, 4] = sees[0] = True
+    o, lse = td.tree_attention(q, k, v, cache, up, return_lse=True, **kw)
+    assert o[sees].isnan().all() and lse[sees].isnan().all()
+    assert torch.equal(o[~sees], clean[0][~sees]) and torch.equal(lse[~sees], clean[1][~sees])
