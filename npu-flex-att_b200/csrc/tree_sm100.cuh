@@ -163,10 +163,42 @@ __device__ __forceinline__ bool any_not_finite(uint32_t w) {
   return (w & e) == e || ((w >> 16) & e) == e;
 }
 
+// Eight columns of O, from column d on, of a row that sees cached keys [from, to)
+// and the nodes `seen` of this block's keys: where a column is not finite, it
+// is the sum of the values of V there that are not (a positive weight changes
+// none). With the rows stored four times such a value meets the zeros that P
+// holds for three of the quarters, and comes out as NaN in place of infinity.
+// Only broken inputs come here, so nothing is done for speed.
+template <bool BF16>
+__device__ __noinline__ void sum_not_finite(const TreeParams& p, int b, int hkv, int from, int to, uint64_t seen, int d, float* f) {
+  float sum[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sum[e] = 0.f;
+  auto add = [&](const void* v, int64_t at) {
+    const uint4 w4 = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(v) + at + d);
+    const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = half_of<BF16>(w[e >> 1], e & 1);
+      if (!(fabsf(x) < __int_as_float(0x7f800000))) sum[e] += x;
+    }
+  };
+  for (int key = from; key < to; ++key) {
+    const int page = p.table[b * p.table_stride + key / p.page];
+    if (page >= 0 && page < p.num_pages) add(p.vp, page * p.svp[0] + hkv * p.svp[1] + key % p.page * p.svp[2]);
+  }
+  for (int n = 0; n < p.N; ++n)
+    if ((seen >> n) & 1) add(p.v, b * p.sv[0] + hkv * p.sv[1] + n * p.sv[2]);
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (!(fabsf(f[e]) < __int_as_float(0x7f800000)) && sum[e] != 0.f) f[e] = sum[e];
+}
+
 template <int D, int NT, int REP, bool BF16, bool CAP, bool ALIBI>
 __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
     tree_kernel(const __grid_constant__ CUtensorMap tmKp, const __grid_constant__ CUtensorMap tmVp,
-                const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeParams p, int box,
+                const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                const __grid_constant__ TreeParams p, int box,
                 uint64_t timeout_ns) {
   using L = TreeLayout<D, NT, REP>;
   constexpr int CH = L::kCH, NS = L::kStages;
@@ -826,7 +858,30 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
                 x.x += a.x, x.y += a.y, x.z += a.z, x.w += a.w;
                 y.x += b.x, y.y += b.y, y.z += b.z, y.w += b.w;
               }
-              put8(__shfl_sync(0xffffffffu, place, r), u / (kU / 2) * (D / 2) + c0 + u % (kU / 2) * 4, x, y);
+              const int64_t at = __shfl_sync(0xffffffffu, place, r);
+              const int d = u / (kU / 2) * (D / 2) + c0 + u % (kU / 2) * 4;
+              // 0·x is 0, or NaN where x is not finite.
+              const float probe = ((x.x * 0.f + x.y * 0.f) + (x.z * 0.f + x.w * 0.f)) + ((y.x * 0.f + y.y * 0.f) + (y.z * 0.f + y.w * 0.f));
+              if (probe != 0.f && at >= 0 && d < p.D) {
+                const float all = (mi.quarter[1][r] + mi.quarter[1][32 + r]) + (mi.quarter[1][64 + r] + mi.quarter[1][96 + r]);
+                if (all == all) {  // else the logits were no numbers, and O stays NaN
+                  int hq_, node_;
+                  const int hkv = cur.item / p.n_rb;
+                  tree_row(p, hkv, (cur.item - hkv * p.n_rb) * p.rb + r, &hq_, &node_);
+                  const int depth = masks.depth[node_], end = cur.c + count;
+                  uint64_t sees = end > cur.n - p.tree_chunks ? masks.anc[node_] : 0ull;
+                  if (p.window > 0)
+                    for (int m_ = 0; m_ < p.N; ++m_)
+                      if (depth - masks.depth[m_] > p.window) sees &= ~(1ull << m_);
+                  int from = cur.lo + cur.c * CH;
+                  if (p.window > 0) from = max(from, cur.len + depth - p.window);
+                  float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+                  sum_not_finite<BF16>(p, cur.b, hkv, from, min(cur.len, cur.lo + end * CH), sees, d, f);
+                  x = make_float4(f[0], f[1], f[2], f[3]);
+                  y = make_float4(f[4], f[5], f[6], f[7]);
+                }
+              }
+              put8(at, d, x, y);
             }
             named_sync(3, kSoft);
           }

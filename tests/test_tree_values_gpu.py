@@ -147,3 +147,49 @@ def test_logits_that_are_no_numbers_in_the_other_forms(dtype, kw):
     o, lse = td.tree_attention(q, k, v, cache, up, return_lse=True, **kw)
     assert o[sees].isnan().all() and lse[sees].isnan().all()
     assert torch.equal(o[~sees], clean[0][~sees]) and torch.equal(lse[~sees], clean[1][~sees])
+
+
+def same_values(o, ref):
+    """NaN and the infinities lie where the definition has them."""
+    for which in (torch.isnan, torch.isposinf, torch.isneginf):
+        assert torch.equal(which(o), which(ref)), which.__name__
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("lens", [[1500], [20] * 170, [300, 70]], ids=["split", "whole", "mixed"])
+@pytest.mark.parametrize("N,Hq,D,window", [(5, 2, 64, 0), (8, 4, 128, 0), (8, 4, 128, 60), (40, 2, 128, 0), (64, 4, 64, 0), (6, 2, 256, 0),
+                                           (1, 1, 128, 0)])
+def test_values_that_all_rows_see_are_summed(dtype, lens, N, Hq, D, window):
+    """Infinite values of V give infinities of their sign in their own columns,
+    NaN where both signs meet or V is NaN; the other columns keep their values."""
+    q, k, v, cache, parents, up = problem(lens, N, Hq, D, dtype, "binary", 26)
+    B = len(lens)
+    some = list(range(B)) if B < 10 else [0, B - 1]
+    clean = td.tree_attention(q, k, v, cache, up, sliding_window=window, return_lse=True)
+    bad = [(11, math.inf), (13, -math.inf), (3, math.nan), (7, math.inf), (7, -math.inf), (20, math.inf), (20, math.inf)]
+    for b in some:
+        for i, (col, x) in enumerate(bad):
+            page, every, at = slot(cache, b, lens[b] - 1 - (i * 37) % min(lens[b], window // 2 or lens[b]))
+            cache.v_pages[page, every, at, col] = x
+        v[b, :, 0, 30] = -math.inf
+    sub = td.PagedKVCache(cache.k_pages, cache.v_pages, cache.page_table[some], cache.lens[some])
+    ref = attention(q[some], k[some], v[some], sub, [parents[b] for b in some], window=window)
+    o, lse = td.tree_attention(q, k, v, cache, up, sliding_window=window, return_lse=True)
+    same_values(o[some], ref[0])
+    touched = torch.zeros(D, dtype=torch.bool, device=DEV)
+    touched[[c for c, _ in bad] + [30]] = True
+    compare(o[some][..., ~touched], lse[some], ref[0][..., ~touched], ref[1], ref[2][..., ~touched])
+    others = [b for b in range(B) if b not in some]
+    assert torch.equal(o[others], clean[0][others]) and torch.equal(lse, clean[1])
+    nfa.check_device_status(DEV)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_infinite_values_with_a_cap_at_head_dim_256(dtype):
+    q, k, v, cache, parents, up = problem([700, 90], 6, 2, 256, dtype, "binary", 27)
+    cache.v_pages[slot(cache, 0, 400)] = math.inf
+    v[1, :, 1, 200] = -math.inf
+    ref = attention(q, k, v, cache, parents, cap=20.0)
+    same_values(td.tree_attention(q, k, v, cache, up, soft_cap=20.0), ref[0])
