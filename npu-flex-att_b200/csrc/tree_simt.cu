@@ -197,7 +197,9 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const TreeParams p,
 #pragma unroll
           for (int c = 0; c < kC; ++c) acc[a][i][c] *= f[i];
       }
-      const bool tree = cur.in_tree(p);
+      // Whether rows differ in what they see of this chunk: the tree's, and the
+      // cached ones that begin before the key from which on every row sees all.
+      const bool differ = cur.in_tree(p) || (p.window > 0 && cur.key0(p) < cur.len + p.N - 1 - p.window);
 #pragma unroll 4
       for (int n = 0; n < kKeys; ++n) {
         float vx[kC];
@@ -210,9 +212,9 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const TreeParams p,
           const float f[4] = {p4.x, p4.y, p4.z, p4.w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            // A node that a row does not see leaves the row alone even where
+            // A key that a row does not see leaves the row alone even where
             // its values are not finite.
-            if (tree && f[i] == 0.f) continue;
+            if (differ && f[i] == 0.f) continue;
 #pragma unroll
             for (int c = 0; c < kC; ++c) acc[a][i][c] = fmaf(f[i], vx[c], acc[a][i][c]);
           }

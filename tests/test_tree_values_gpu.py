@@ -193,3 +193,25 @@ def test_infinite_values_with_a_cap_at_head_dim_256(dtype):
     v[1, :, 1, 200] = -math.inf
     ref = attention(q, k, v, cache, parents, cap=20.0)
     same_values(td.tree_attention(q, k, v, cache, up, soft_cap=20.0), ref[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("bad", BAD)
+@pytest.mark.parametrize("N,Hq,D,window", [(5, 2, 64, 40), (20, 1, 128, 200), (40, 2, 80, 33), (64, 4, 128, 1), (6, 2, 256, 300)])
+def test_values_behind_the_window_do_not_spread(dtype, bad, N, Hq, D, window):
+    """Cached tokens before the window, and inside it for the root alone, whose
+    values are not finite: rows that do not see them keep theirs."""
+    lens = [511, 200, 1]
+    q, k, v, cache, parents, up = problem(lens, N, Hq, D, dtype, "chain", 28)
+    ref = attention(q, k, v, cache, parents, window=window)
+    keep = torch.ones(3, Hq, N, dtype=torch.bool, device=DEV)
+    for b, n in enumerate(lens):
+        for at in (n - window - 1, n - window - 2, n - window - 20, n - window - 150, n - window):
+            if 0 <= at < n:
+                cache.v_pages[slot(cache, b, at)] = bad
+        if n >= window:
+            keep[b, :, 0] = False  # the root sees the last one of them
+    o, lse = td.tree_attention(q, k, v, cache, up, sliding_window=window, return_lse=True)
+    compare(o[keep], lse[keep], ref[0][keep], ref[1][keep], ref[2][keep])
+    nfa.check_device_status(DEV)
