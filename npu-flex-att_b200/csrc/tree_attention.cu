@@ -172,6 +172,10 @@ int check_tree(const bfa_tree_args* a) {
   return BFA_OK;
 }
 
+// The window in 32 bits. Positions stay below INT32_MAX / 2, so that a window of
+// that size, or of any larger one, sees everything.
+int window_of(const bfa_tree_args* a) { return (int)std::min<int64_t>(a->sliding_window, INT32_MAX / 2); }
+
 // Row block, chunk and grid of a problem.
 struct Plan {
   int rb, n_rb, chunk, tree_chunks, grid;
@@ -188,7 +192,7 @@ Plan make_plan(const bfa_tree_args* a, const TreeTile& tile) {
   pl.tree_chunks = (int)((a->nodes + pl.chunk - 1) / pl.chunk);
   // At most one stretch per chunk that the tables could hold.
   int64_t seen = a->max_pages * a->page_size;
-  if (a->sliding_window > 0) seen = std::min(seen, a->sliding_window + pl.chunk);
+  if (a->sliding_window > 0) seen = std::min<int64_t>(seen, (int64_t)window_of(a) + pl.chunk);
   const int64_t chunks = ((seen + pl.chunk - 1) / pl.chunk + pl.tree_chunks) * a->batch * a->heads_kv * pl.n_rb;
   pl.grid = (int)std::min<int64_t>(chunks, (int64_t)sm_count() * tile.per_sm);
   pl.small = chunks < ((int64_t)1 << 31) / (pl.grid + 1);
@@ -296,7 +300,7 @@ extern "C" int bfa_tree_fwd(const bfa_tree_args* a, void* stream) {
   p.B = (int)a->batch; p.Hq = (int)a->heads_q; p.Hkv = (int)a->heads_kv; p.G = p.Hq / p.Hkv;
   p.N = (int)a->nodes; p.D = (int)a->head_dim; p.page = (int)a->page_size;
   p.cap_tokens = (int)(a->max_pages * a->page_size);
-  p.window = (int)std::min<int64_t>(a->sliding_window, INT32_MAX / 2);
+  p.window = window_of(a);
   p.scale = (float)a->scale;
   p.soft_cap = (float)a->soft_cap;
   p.grid = pl.grid; p.rb = pl.rb; p.n_rb = pl.n_rb; p.chunk = pl.chunk; p.tree_chunks = pl.tree_chunks;

@@ -98,3 +98,13 @@ def test_cpu_tensors_are_refused():
         td.cache_append(cache, k, k)
     with pytest.raises(RuntimeError, match="no CPU path"):
         td.verify_tree(torch.ones(1, 3, 4), torch.zeros(1, 3, dtype=torch.int64), None, torch.rand(1, 3), torch.ones(1, 4))
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_workspace_bytes_of_windows_without_end(dtype):
+    """The largest windows (no limit at all) plan like one that covers the table."""
+    lib = bfa_lib.load()
+    base = dict(TREE, dtype=dtype, batch=3, max_pages=50)
+    want = lib.bfa_tree_workspace_bytes(block(bfa_lib.TreeArgs, **dict(base, sliding_window=800)))
+    for window in (801, 2 ** 31 - 1, 2 ** 31, 2 ** 40, 2 ** 63 - 129, 2 ** 63 - 1):
+        assert lib.bfa_tree_workspace_bytes(block(bfa_lib.TreeArgs, **dict(base, sliding_window=window))) == want, window

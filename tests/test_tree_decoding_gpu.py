@@ -593,3 +593,13 @@ def test_queries_off_the_grid(dtype, D, N, Hq):
         q = flat[offset:].view(3, Hq, N, D)
         compare(*td.tree_attention(q, k, v, cache, up, return_lse=True), *attention(q, k, v, cache, parents))
     nfa.check_device_status(DEV)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_windows_without_end(dtype):
+    a, *more = (check([300, 20, 0], 9, 4, 2, 64, dtype, 16, tree("binary", 9, 3), sliding_window=w)
+                for w in (0, 400, 2 ** 31 - 1, 2 ** 31, 2 ** 63 - 1))
+    for b in more:
+        # The same chunks and products: a window that ends nowhere masks nothing.
+        assert torch.equal(a, b)
