@@ -248,7 +248,8 @@ int bfa_merge_partial(int32_t batch, int32_t heads, int32_t seqlen, int32_t head
  * v_pages, unit innermost stride), a page table int32 [B, max_pages] (row
  * stride page_table_stride) and the cached lengths int32 [B]: token t of
  * sequence b lies in page page_table[b, t / page_size], slot t % page_size.
- * Table entries past a sequence's length are not read.
+ * Table entries past a sequence's length are not read, nor, by attention with
+ * a sliding window W, those of pages that lie before position lens[b] - W whole.
  *
  * A tree of `nodes` drafted tokens per sequence is given by the parent of each
  * node, int32 [B, nodes] (row stride parents_stride, 0: one tree for all):

@@ -172,7 +172,8 @@ __device__ __forceinline__ int tree_stretch(const TreeParams& p, TreeCursor& cur
   return p.small ? tree_stretch_in<uint32_t>(p, cur) : tree_stretch_in<int64_t>(p, cur);
 }
 
-// The rows of K and V that key j of a chunk lies in (null reads as zeros).
+// The rows of K and V that key j of a chunk lies in (null reads as zeros: past
+// the keys, and before a window, where pages may have been given back).
 // Reports a bad page. Rows of absent nodes are read like the others: their
 // logits are masked, and the kernels keep values that a row does not see out
 // of its sum even where they are not finite.
@@ -187,7 +188,7 @@ __device__ __forceinline__ void tree_key_rows(const TreeParams& p, const TreeCur
     *vr = static_cast<const char*>(p.v) + (cur.b * p.sv[0] + hkv * p.sv[1] + key * p.sv[2]) * kBytes;
     return;
   }
-  if (key >= cur.len) return;
+  if (key >= cur.len || (p.window > 0 && key < cur.len - p.window)) return;
   const int pg = p.page_log2 >= 0 ? key >> p.page_log2 : key / p.page, slot = key - pg * p.page;
   const int32_t page = p.table[cur.b * p.table_stride + pg];
   if (page < 0 || page >= p.num_pages) {

@@ -270,13 +270,16 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
     const int my_box = lane / L::kSub, my_sub = lane % L::kSub;
     const int boxes = CH / box, per = 32 / boxes;  // powers of 2
     // The boxes of `per` chunks of an item from its chunk `c`, one per lane:
-    // their pages (0 past the cache) and first tokens in them.
+    // their pages (0 past the cache) and first tokens in them; -1 in a box that
+    // lies before the window whole, whose page may have been given back: its
+    // table entry is not read, and it is loaded as zeros.
     int page = 0, slot = 0, next_page = 0, next_slot = 0;
     auto lookup = [&](const TreeCursor& at, int c) {
       const int t = at.lo + c * CH + lane * box;
       const int pg = p.page_log2 >= 0 ? t >> p.page_log2 : t / p.page;
-      next_slot = t - pg * p.page;
-      next_page = t < at.len ? p.table[at.b * p.table_stride + pg] : 0;
+      const bool behind = p.window > 0 && t + box <= at.len - p.window;
+      next_slot = behind ? -1 : t - pg * p.page;
+      next_page = t < at.len && !behind ? p.table[at.b * p.table_stride + pg] : 0;
     };
     bool ok = true;
     int x = 0, st = kv, round = 0;  // the next load's slot and that slot's round
@@ -318,9 +321,10 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
         if (j == 0) {
           page = next_page;
           slot = next_slot;
-          if (page < 0 || page >= p.num_pages) {
+          if (slot < 0 || page < 0 || page >= p.num_pages) {
             page = (int)p.num_pages;  // outside the tensor: reads as zeros
-            if (p.status) *p.status = BFA_ERR_INDEX;
+            if (slot >= 0 && p.status) *p.status = BFA_ERR_INDEX;
+            slot = 0;
           }
         }
         const int pg = __shfl_sync(0xffffffffu, page, j * boxes + my_box);  // the lane is taken modulo 32

@@ -31,8 +31,9 @@ class PagedKVCache(NamedTuple):
     """K/V of cached tokens in pages: k_pages and v_pages [num_pages, Hkv,
     page_size, D], page_table int32 [B, max_pages], lens int32 [B]. Token t of
     sequence b lies in page page_table[b, t // page_size], slot t % page_size;
-    table entries past a sequence's length are not read. The caller owns the
-    tensors and hands out the pages."""
+    table entries past a sequence's length are not read, nor, with a sliding
+    window W, those of pages wholly before token lens[b] - W: they may be given
+    back. The caller owns the tensors and hands out the pages."""
     k_pages: torch.Tensor
     v_pages: torch.Tensor
     page_table: torch.Tensor

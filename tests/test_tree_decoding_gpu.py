@@ -603,3 +603,33 @@ def test_windows_without_end(dtype):
     for b in more:
         # The same chunks and products: a window that ends nowhere masks nothing.
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("page", [8, 16, 24, 7, 64, 128])
+@pytest.mark.parametrize("D,N,Hq,window", [(128, 4, 4, 200), (64, 20, 8, 37), (256, 6, 2, 301), (128, 64, 4, 1)])
+def test_pages_behind_the_window_may_be_given_back(dtype, page, D, N, Hq, window):
+    """Table entries of pages whose last token no row sees hold no page: the call
+    is valid, reports nothing and gives the same bits."""
+    g = gen(15)
+    lens = [1300, 257, 40, 0]
+    kp, vp, table, ln = page_cache(lens, 1312, page, 1, D, dtype, DEV, g)
+    q, k, v = (torch.randn(4, h, N, D, generator=g, device=DEV).to(dtype) for h in (Hq, 1, 1))
+    up = torch.tensor(tree("binary", N, 4), dtype=torch.int32, device=DEV)
+    want = td.tree_attention(q, k, v, td.PagedKVCache(kp, vp, table, ln), up, sliding_window=window, return_lse=True)
+    gone = table.clone()
+    for b, n in enumerate(lens):
+        for i in range(max(0, n - window) // page):  # the pages of tokens before n - window only
+            gone[b, i] = (-1, 2 ** 31 - 1, kp.shape[0])[i % 3]
+    assert (gone != table).any()
+    got = td.tree_attention(q, k, v, td.PagedKVCache(kp, vp, gone, ln), up, sliding_window=window, return_lse=True)
+    nfa.check_device_status(DEV)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    compare(*got, *attention(q, k, v, (kp, vp, table, ln), tree("binary", N, 4), window=window))
+    # A page that a row does see is still reported.
+    seen = gone.clone()
+    seen[0, (lens[0] - 1) // page] = -1
+    td.tree_attention(q, k, v, td.PagedKVCache(kp, vp, seen, ln), up, sliding_window=window)
+    with pytest.raises(RuntimeError, match="outside its table"):
+        nfa.check_device_status(DEV)
