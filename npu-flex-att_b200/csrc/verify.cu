@@ -43,6 +43,7 @@ constexpr int kMaxNodes = 64;
 constexpr int kVerifyThreads = 512;
 constexpr int kVerifyPerSm = 2;  // resident blocks per SM: 64 registers a thread
 constexpr int kMaxCluster = 8;
+constexpr int kVerifyStep = 16 * kVerifyThreads;  // the most entries that a thread's loop counter moves by
 
 struct VerifyParams {
   const void* target; const void* draft;
@@ -149,6 +150,7 @@ __global__ void __launch_bounds__(kVerifyThreads, kVerifyPerSm) verify_kernel(co
   constexpr int kSumBatch = E == 1 ? 16 : 1, kDrawBatch = E == 1 ? 8 : 1;
   constexpr int kSumUnroll = E == 1 ? 1 : 4, kDrawUnroll = E == 1 ? 1 : 2;
   constexpr int kStep = kVerifyThreads * E;
+  static_assert(kStep * kSumBatch <= kVerifyStep && kStep * kDrawBatch <= kVerifyStep, "bound of the vocabulary");
   __shared__ Shared sh;
   const int tid = threadIdx.x;
   const uint32_t rank = cluster_rank();
@@ -352,7 +354,7 @@ int launch_typed(VerifyParams& p, int B, cudaStream_t st) {
 extern "C" int bfa_verify_tree(const bfa_verify_args* a, void* stream) {
   using namespace bfa;
   if (!a || a->batch < 0 || a->nodes < 1 || a->vocab < 1) return BFA_ERR_INVALID_ARGUMENT;
-  if (a->nodes > kMaxNodes || a->vocab > INT32_MAX - 8 * kVerifyThreads || a->batch > INT32_MAX / kMaxCluster ||
+  if (a->nodes > kMaxNodes || a->vocab > INT32_MAX - kVerifyStep || a->batch > INT32_MAX / kMaxCluster ||
       a->dtype != (int)a->dtype || dtype_bytes((int)a->dtype) == 0)
     return BFA_ERR_UNSUPPORTED;
   if (a->batch == 0) return BFA_OK;

@@ -108,3 +108,11 @@ def test_workspace_bytes_of_windows_without_end(dtype):
     want = lib.bfa_tree_workspace_bytes(block(bfa_lib.TreeArgs, **dict(base, sliding_window=800)))
     for window in (801, 2 ** 31 - 1, 2 ** 31, 2 ** 40, 2 ** 63 - 129, 2 ** 63 - 1):
         assert lib.bfa_tree_workspace_bytes(block(bfa_lib.TreeArgs, **dict(base, sliding_window=window))) == want, window
+
+
+def test_verify_refuses_vocabularies_that_its_counters_cannot_pass():
+    """Entries are counted in 32 bits, in steps of up to 16 x 512."""
+    lib = bfa_lib.load()
+    for vocab, code in ((2 ** 31 - 1 - 8192, -1), (2 ** 31 - 8192, -3), (2 ** 31 - 1 - 4096, -3), (2 ** 31 - 1, -3), (2 ** 40, -3)):
+        # In range, the null pointers are the first thing wrong.
+        assert lib.bfa_verify_tree(block(bfa_lib.VerifyArgs, **dict(VERIFY, vocab=vocab)), None) == code, vocab
