@@ -72,6 +72,11 @@ inline int allow_shared(K kernel, int bytes, std::atomic<uint64_t>& done, const 
   return BFA_OK;
 }
 
+// Grid planes over the batch, and the largest batch whose index, moved on by
+// that many, stays in 32 bits.
+constexpr int kBatchPlanes = 65535;
+constexpr int64_t kMaxBatch = 0x7fffffffll - kBatchPlanes;
+
 // Whether 16-byte vectors can address every row of a tensor (unit innermost
 // stride, 16-byte aligned base and outer strides).
 inline bool vector_rows(const bfa_tensor& t, int bytes) {

@@ -90,7 +90,7 @@ int launch_append(AppendParams& p, int D, cudaStream_t st) {
   if (heads > 65535) return BFA_ERR_UNSUPPORTED;
   const int threads = (int)std::max<int64_t>(32, std::min<int64_t>(256, (per_head + 31) / 32 * 32));
   const dim3 grid((unsigned)std::max<int64_t>(1, (per_head + threads - 1) / threads), (unsigned)heads,
-                  (unsigned)std::min(p.B, 65535));
+                  (unsigned)std::min(p.B, kBatchPlanes));
   if (four) append_kernel<U, kPer, 4><<<grid, threads, 0, st>>>(p);
   else append_kernel<U, kPer, 1><<<grid, threads, 0, st>>>(p);
   note_launch();
@@ -107,7 +107,7 @@ extern "C" int bfa_cache_append(const bfa_append_args* a, void* stream) {
     return BFA_ERR_INVALID_ARGUMENT;
   const int bytes = a->dtype == (int)a->dtype ? dtype_bytes((int)a->dtype) : 0;
   if (bytes == 0 || a->head_dim > 256) return BFA_ERR_UNSUPPORTED;
-  if (a->batch > INT32_MAX || a->heads_kv > INT32_MAX || a->tokens > INT32_MAX || a->page_size > INT32_MAX / 2 ||
+  if (a->batch > kMaxBatch || a->heads_kv > INT32_MAX - 3 || a->tokens > INT32_MAX || a->page_size > INT32_MAX / 2 ||
       a->max_pages > INT32_MAX / 2 / a->page_size)
     return BFA_ERR_UNSUPPORTED;
   if (a->batch == 0) return BFA_OK;

@@ -158,16 +158,16 @@ int launch_rope(RopeParams& p, bool in_place, cudaStream_t st) {
   p.units = turn + (in_place ? 0 : (p.D - p.R) / V);
   const int64_t per_head = (int64_t)p.S * p.units;
   if (per_head > INT32_MAX - 256) return BFA_ERR_UNSUPPORTED;
-  const int H = p.Hq + p.Hk;
+  const int64_t H = (int64_t)p.Hq + p.Hk;
   // More heads per thread (the table's values stay in registers) while two
   // full waves of threads remain.
   const int64_t wave = (int64_t)sm_count() * 2048;
   p.span = 1;
   while (p.span < H && per_head * p.B * ((H + 2 * p.span - 1) / (2 * p.span)) >= 2 * wave) p.span *= 2;
   const int threads = (int)std::min<int64_t>(256, (per_head + 31) / 32 * 32);
-  const int heads = (H + p.span - 1) / p.span;
+  const int64_t heads = (H + p.span - 1) / p.span;
   if (heads > 65535) return BFA_ERR_UNSUPPORTED;
-  const dim3 grid((unsigned)((per_head + threads - 1) / threads), (unsigned)heads, (unsigned)std::min(p.B, 65535));
+  const dim3 grid((unsigned)((per_head + threads - 1) / threads), (unsigned)heads, (unsigned)std::min(p.B, kBatchPlanes));
   rope_kernel<T, IL, V><<<grid, threads, 0, st>>>(p);
   note_launch();
   return launch_status("rope kernel launch");
@@ -195,7 +195,7 @@ extern "C" int bfa_rope(const bfa_rope_args* a, void* stream) {
     return BFA_ERR_INVALID_ARGUMENT;
   if (a->rotary_dim > a->head_dim) return BFA_ERR_SHAPE;
   if (dtype_bytes((int)a->dtype) == 0 || a->dtype != (int)a->dtype) return BFA_ERR_UNSUPPORTED;
-  if (a->batch > INT32_MAX || a->heads_q > INT32_MAX / 2 || a->heads_k > INT32_MAX / 2 || a->seqlen > INT32_MAX ||
+  if (a->batch > kMaxBatch || a->heads_q > INT32_MAX / 2 || a->heads_k > INT32_MAX / 2 || a->seqlen > INT32_MAX ||
       a->head_dim > 65536)
     return BFA_ERR_UNSUPPORTED;
   const int64_t heads = a->heads_q + a->heads_k;

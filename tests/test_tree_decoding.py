@@ -116,3 +116,12 @@ def test_verify_refuses_vocabularies_that_its_counters_cannot_pass():
     for vocab, code in ((2 ** 31 - 1 - 8192, -1), (2 ** 31 - 8192, -3), (2 ** 31 - 1 - 4096, -3), (2 ** 31 - 1, -3), (2 ** 40, -3)):
         # In range, the null pointers are the first thing wrong.
         assert lib.bfa_verify_tree(block(bfa_lib.VerifyArgs, **dict(VERIFY, vocab=vocab)), None) == code, vocab
+
+
+@pytest.mark.parametrize("name,cls,base", [("bfa_rope", "RopeArgs", ROPE), ("bfa_cache_append", "AppendArgs", APPEND)])
+def test_batches_that_the_grids_counter_cannot_pass_are_refused(name, cls, base):
+    """A block goes on by up to 65535 sequences at a time, in 32 bits."""
+    lib = bfa_lib.load()
+    for batch, code in ((2 ** 31 - 1 - 65535, -1), (2 ** 31 - 65535, -3), (2 ** 31 - 1, -3), (2 ** 40, -3)):
+        # In range, the null pointers are the first thing wrong.
+        assert getattr(lib, name)(block(getattr(bfa_lib, cls), **dict(base, batch=batch)), None) == code, batch
