@@ -62,9 +62,6 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const TreeParams p,
   TreeCursor cur;
   const int n_x = tree_stretch(p, cur);
   if (n_x == 0) return;
-  if (tid == 0) {  // a clamped length is an error of the caller's
-    if (p.status && p.lens[cur.b] != cur.len) *p.status = BFA_ERR_INDEX;
-  }
   TreeCursor ahead = cur;  // the chunk whose rows are looked up next
   int masks_of = -1;
 
@@ -111,6 +108,8 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const TreeParams p,
       seg_c0 = cur.c;
       if (masks_of != cur.b) {
         masks_of = cur.b;
+        // A clamped length is an error of the caller's.
+        if (tid == 0 && p.status && p.lens[cur.b] != cur.len) *p.status = BFA_ERR_INDEX;
         if (warp == 0) tree_masks(p, cur.b, sh.masks);
       }
       for (int i = tid; i < kRows * D; i += kThreads) {

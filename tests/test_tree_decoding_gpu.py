@@ -633,3 +633,25 @@ def test_pages_behind_the_window_may_be_given_back(dtype, page, D, N, Hq, window
     td.tree_attention(q, k, v, td.PagedKVCache(kp, vp, seen, ln), up, sliding_window=window)
     with pytest.raises(RuntimeError, match="outside its table"):
         nfa.check_device_status(DEV)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_bad_lengths_are_reported_wherever_they_stand(dtype):
+    """Many short sequences, several to a block: a length outside the table is
+    reported for each of them, not for a block's first alone."""
+    g = gen(16)
+    B = 900
+    kp, vp = (torch.randn(4, 1, 16, 64, generator=g, device=DEV).to(dtype) for _ in range(2))
+    table = torch.randint(0, 4, (B, 1), generator=g, device=DEV, dtype=torch.int32)
+    q, k, v = (torch.randn(B, 1, 1, 64, generator=g, device=DEV).to(dtype) for _ in range(3))
+    nfa.check_device_status(DEV)
+    for at in (0, 1, 2, 3, 17, 450, 451, 452, 897, 898, 899):
+        for n in (-1, 17):
+            ln = torch.full((B,), 5, dtype=torch.int32, device=DEV)
+            ln[at] = n
+            td.tree_attention(q, k, v, td.PagedKVCache(kp, vp, table, ln))
+            with pytest.raises(RuntimeError, match="outside its table"):
+                nfa.check_device_status(DEV)
+    td.tree_attention(q, k, v, td.PagedKVCache(kp, vp, table, torch.full((B,), 16, dtype=torch.int32, device=DEV)))
+    nfa.check_device_status(DEV)
