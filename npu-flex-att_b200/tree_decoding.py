@@ -52,18 +52,23 @@ def _binding():
 
 def tree_depths(parents):
     """Edges from the root to each node, int32 of the shape of ``parents`` (0 at
-    the root and at absent nodes): with the cached lengths as offsets, the
-    rotary positions of the nodes. Works on host tensors too; a fixed tree's
-    depths are computed once."""
+    the root and at absent nodes, those under one among them): with the cached
+    lengths as offsets, the rotary positions of the nodes. A parent outside
+    -1 <= parents[n] < n makes its node absent, as in tree_attention, which
+    reports it. Works on host tensors too; a fixed tree's depths are computed
+    once."""
     n = parents.shape[-1]
-    up = parents.long().clone()
-    up[..., 0] = -1
-    depth = torch.zeros_like(up)
-    here = up
-    for _ in range(n - 1):
-        depth += here >= 0
-        here = torch.where(here >= 0, up.gather(-1, here.clamp(min=0)), here)
-    return depth.to(torch.int32)
+    node = torch.arange(n, device=parents.device)
+    # Node n is "no parent", above itself like the root.
+    up = torch.where((parents >= 0) & (parents < node), parents, n).long()
+    up = torch.nn.functional.pad(up, (0, 1), value=n)
+    up[..., 0] = 0
+    depth = torch.ones_like(up)
+    depth[..., 0] = depth[..., n] = 0
+    for _ in range((n - 1).bit_length()):  # each round doubles the climbed distance
+        depth = depth + depth.gather(-1, up)
+        up = up.gather(-1, up)
+    return torch.where(up == 0, depth, 0)[..., :n].to(torch.int32)
 
 
 def tree_attention(query, key, value, cache, parents=None, *, scale=None, sliding_window=0, soft_cap=0.0,

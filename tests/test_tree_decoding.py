@@ -125,3 +125,54 @@ def test_batches_that_the_grids_counter_cannot_pass_are_refused(name, cls, base)
     for batch, code in ((2 ** 31 - 1 - 65535, -1), (2 ** 31 - 65535, -3), (2 ** 31 - 1, -3), (2 ** 40, -3)):
         # In range, the null pointers are the first thing wrong.
         assert getattr(lib, name)(block(getattr(bfa_lib, cls), **dict(base, batch=batch)), None) == code, batch
+
+
+def climbed(row):
+    """Depths of one tree, a node at a time."""
+    depth = []
+    for n, up in enumerate(row):
+        depth.append(0 if n == 0 else depth[up] + 1 if 0 <= up < n and depth[up] is not None else None)
+    return [d or 0 for d in depth]
+
+
+@pytest.mark.parametrize("row", [[-1, -1, 1, 2], [-1, 0, -1, 2, 3, 1], [7, 0, 1, -1, 3], [0, 0, 0], [-1], [-1, -1], [-5, 0, 1, 1, 0, 4]])
+def test_depths_of_absent_nodes(row):
+    """A node under an absent one is absent too, at depth 0."""
+    assert td.tree_depths(torch.tensor(row, dtype=torch.int32)).tolist() == climbed(row)
+
+
+@pytest.mark.parametrize("row", [[-1, 0, 2, 1], [-1, 0, 9, 2, 1], [-1, 2, 1, 0], [-1, 1, 0], [-1, 0, 1, 2 ** 31 - 1, 3], [-1, -2, 1, -2 ** 31, 0],
+                                 [-1, 3, 1, 2]])
+def test_depths_of_parents_outside_their_range(row):
+    """A parent that is no earlier node is not followed: its node is absent."""
+    for t in (torch.tensor(row, dtype=torch.int32), torch.tensor([row, [-1] + list(range(len(row) - 1))], dtype=torch.int32)):
+        d = td.tree_depths(t)
+        assert d.dtype == torch.int32 and d.shape == t.shape
+        assert (d[0] if d.dim() == 2 else d).tolist() == climbed(row)
+        if d.dim() == 2:
+            assert d[1].tolist() == list(range(len(row)))
+
+
+@pytest.mark.parametrize("n", [1, 2, 3, 31, 32, 33, 64, 200])
+def test_depths_of_larger_trees(n):
+    g = torch.Generator().manual_seed(n)
+    rows = [[-1] + list(range(n - 1)), [-1] + [0] * (n - 1)]
+    rows += [[-1] + [int(torch.randint(-1, i, (), generator=g)) for i in range(1, n)] for _ in range(6)]
+    assert td.tree_depths(torch.tensor(rows, dtype=torch.int32)).tolist() == [climbed(row) for row in rows]
+    assert td.tree_depths(torch.tensor(rows)).tolist() == [climbed(row) for row in rows]
+
+
+def test_depths_take_few_operations():
+    """A decoding step of a changing tree forms them anew: a few operations a
+    doubling, not a few a node."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Count(TorchDispatchMode):
+        n = 0
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            Count.n += 1
+            return func(*args, **(kwargs or {}))
+    with Count():
+        td.tree_depths(torch.tensor([[-1] + list(range(63))], dtype=torch.int32))
+    assert Count.n <= 50
