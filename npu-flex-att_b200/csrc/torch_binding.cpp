@@ -17,6 +17,7 @@
 #include <torch/extension.h>
 
 #include <cmath>
+#include <initializer_list>
 #include <optional>
 #include <sstream>
 #include <string>
@@ -48,6 +49,13 @@ void require_cuda(const char* what, const Tensor& t, const at::Device& dev) {
 const at::Device first_device(const char* what, const Tensor& t) {
   BFA_RUNTIME(t.is_cuda(), what, " (B200 build) needs CUDA tensors; there is no CPU path");
   return t.device();
+}
+
+// A tangent of forward-mode differentiation would be lost: the outputs are new
+// tensors that know nothing of it.
+void refuse_tangents(const char* what, std::initializer_list<const Tensor*> inputs) {
+  for (const Tensor* t : inputs)
+    BFA_RUNTIME(!(t->defined() && t->_fw_grad(/*level=*/0).defined()), what, " has no forward-mode derivative (an input carries a tangent)");
 }
 
 int64_t dtype_of(const Tensor& t) {
@@ -200,6 +208,7 @@ QkPair rotary_embedding(const OptTensor& query, const OptTensor& key, const Tens
                "query and key must agree in batch, length and head dim");
     BFA_RUNTIME(k.scalar_type() == q.scalar_type(), "query and key must have one dtype");
   }
+  refuse_tangents(what, {&q, &k, &cos, &sin});
   const at::Device dev = first_device(what, first);
   for (const Tensor* t : {&k, &cos, &sin, &pos, &off})
     if (t->defined()) require_cuda(what, *t, dev);
@@ -286,6 +295,8 @@ std::tuple<Tensor, OptTensor> tree_attention(const Tensor& query, const Tensor& 
   BFA_VALUE(sliding_window >= 0 && soft_cap >= 0, "sliding_window and soft_cap must be >= 0");
   const at::ScalarType dt = query.scalar_type();
   BFA_RUNTIME(key.scalar_type() == dt && value.scalar_type() == dt, "query, key and value must have one dtype");
+  refuse_tangents(what, {&query, &key, &value, &k_pages, &v_pages});
+  if (alibi_slope) refuse_tangents(what, {&*alibi_slope});
   const at::Device dev = first_device(what, query);
   require_cuda(what, key, dev);
   require_cuda(what, value, dev);
@@ -371,6 +382,7 @@ Tensor cache_append(const Tensor& k_pages, const Tensor& v_pages, const Tensor& 
   BFA_ASSERT(key.dim() == 4 && value.sizes() == key.sizes(), "key and value are [B, Hkv, S, D]");
   const int64_t B = key.size(0), Hkv = key.size(1), S = key.size(2), D = key.size(3);
   BFA_RUNTIME(value.scalar_type() == key.scalar_type(), "key and value must have one dtype");
+  refuse_tangents(what, {&key, &value, &k_pages, &v_pages});
   const at::Device dev = first_device(what, key);
   require_cuda(what, value, dev);
   check_cache(what, {k_pages, v_pages, table, lens}, B, Hkv, D, key.scalar_type(), dev);

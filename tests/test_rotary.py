@@ -55,3 +55,15 @@ def test_cpu_tensors_are_refused():
         rotary.rotary_embedding(None, None, cos, sin)
     with pytest.raises(AssertionError):
         rotary.rotary_embedding(q, torch.randn(1, 2, 15, 64), cos, sin)
+
+
+def test_tangents_are_refused():
+    """Forward-mode differentiation would lose the tangent without a word."""
+    import torch.autograd.forward_ad as fwd
+    cos, sin = rotary.rotary_table(64, 16)
+    q, k = torch.randn(1, 2, 16, 64), torch.randn(1, 1, 16, 64)
+    with fwd.dual_level():
+        for args in ((fwd.make_dual(q, torch.ones_like(q)), k, cos, sin), (None, fwd.make_dual(k, torch.ones_like(k)), cos, sin),
+                     (q, k, fwd.make_dual(cos, torch.ones_like(cos)), sin)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                rotary.rotary_embedding(*args)

@@ -176,3 +176,21 @@ def test_depths_take_few_operations():
     with Count():
         td.tree_depths(torch.tensor([[-1] + list(range(63))], dtype=torch.int32))
     assert Count.n <= 50
+
+
+def test_tangents_are_refused():
+    """Forward-mode differentiation would lose the tangent without a word."""
+    import torch.autograd.forward_ad as fwd
+    q, k = torch.randn(1, 2, 3, 64), torch.randn(1, 1, 3, 64)
+    pages = torch.zeros(1, 1, 16, 64)
+    cache = td.PagedKVCache(pages, pages, torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32))
+    slopes = torch.ones(2)
+    with fwd.dual_level():
+        def dual(t):
+            return fwd.make_dual(t, torch.ones_like(t))
+        for call in (lambda: td.tree_attention(dual(q), k, k, cache), lambda: td.tree_attention(q, k, dual(k), cache),
+                     lambda: td.tree_attention(q, k, k, cache._replace(k_pages=dual(pages))),
+                     lambda: td.tree_attention(q, k, k, cache, alibi_slope=dual(slopes)),
+                     lambda: td.cache_append(cache, dual(k), k), lambda: td.cache_append(cache._replace(v_pages=dual(pages)), k, k)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
