@@ -58,6 +58,12 @@ void refuse_tangents(const char* what, std::initializer_list<const Tensor*> inpu
     BFA_RUNTIME(!(t->defined() && t->_fw_grad(/*level=*/0).defined()), what, " has no forward-mode derivative (an input carries a tangent)");
 }
 
+// Written in place: autograd finds out from the version that a tensor it saved
+// has changed. (Inference tensors have none.)
+void note_written(const Tensor& t) {
+  if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 int64_t dtype_of(const Tensor& t) {
   switch (t.scalar_type()) {
     case at::kFloat: return BFA_DTYPE_F32;
@@ -239,6 +245,7 @@ QkPair rotary_embedding(const OptTensor& query, const OptTensor& key, const Tens
     BFA_VALUE(fits(q, qo), "out for query must match it in shape, dtype and device");
     BFA_VALUE(fits(k, ko), "out for key must match it in shape, dtype and device");
     rope_launch(q, k, cos, sin, pos, off, interleaved, false, qo, ko);
+    note_written(qo), note_written(ko);
     return {std::get<0>(*out), std::get<1>(*out)};
   }
   Tensor qo, ko;
@@ -411,6 +418,7 @@ Tensor cache_append(const Tensor& k_pages, const Tensor& v_pages, const Tensor& 
   a.lens_out = out.data_ptr<int32_t>();
   a.status = status_word(dev);
   check(bfa_cache_append(&a, stream_of(dev)));
+  note_written(k_pages), note_written(v_pages);
   return out;
 }
 

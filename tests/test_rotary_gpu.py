@@ -213,3 +213,21 @@ def test_gradient_of_one_output(which):
     pos = torch.arange(9, device=DEV)[None]
     close(grads[which], *exact(w, cos, sin, pos, True, True))
     assert grads[1 - which] is None
+
+
+@pytest.mark.gpu
+def test_out_is_written_in_place_for_autograd():
+    """A tensor that autograd has saved and out= overwrites: the backward raises."""
+    cos, sin = rotary.rotary_table(64, 40, device=DEV)
+    q, k = make(1, 2, 2, 9, 64, torch.float32)
+    w = torch.ones_like(q, requires_grad=True)
+    before = q._version, k._version
+    y = (w * q).sum()
+    with torch.no_grad():
+        rotary.rotary_embedding(q, k, cos, sin, out=(q, k))
+    assert q._version > before[0] and k._version > before[1]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        x = torch.randn(1, 2, 9, 64, device=DEV)
+    rotary.rotary_embedding(x, None, cos, sin, out=(x, None))

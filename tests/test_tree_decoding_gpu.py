@@ -655,3 +655,24 @@ def test_bad_lengths_are_reported_wherever_they_stand(dtype):
                 nfa.check_device_status(DEV)
     td.tree_attention(q, k, v, td.PagedKVCache(kp, vp, table, torch.full((B,), 16, dtype=torch.int32, device=DEV)))
     nfa.check_device_status(DEV)
+
+
+@pytest.mark.gpu
+def test_append_is_written_in_place_for_autograd():
+    """Pages that autograd has saved and an append overwrites: the backward raises."""
+    g = gen(2)
+    cache = td.PagedKVCache(*page_cache([10, 4], 32, 16, 2, 64, FP, DEV, g, extra_pages=4, poison=0.0))
+    cache.page_table[:, 1] = torch.tensor([2, 3], device=DEV)
+    k, v = (torch.randn(2, 2, 4, 64, generator=g, device=DEV) for _ in range(2))
+    for pages in (cache.k_pages, cache.v_pages):
+        w = torch.ones_like(pages, requires_grad=True)
+        before = pages._version
+        y = (w * pages).sum()
+        td.cache_append(cache, k, v)
+        assert pages._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():
+        other = td.PagedKVCache(*(t.clone() for t in cache))
+    td.cache_append(other, k, v)
+    nfa.check_device_status(DEV)
