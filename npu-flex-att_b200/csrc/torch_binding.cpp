@@ -58,6 +58,13 @@ void refuse_tangents(const char* what, std::initializer_list<const Tensor*> inpu
     BFA_RUNTIME(!(t->defined() && t->_fw_grad(/*level=*/0).defined()), what, " has no forward-mode derivative (an input carries a tangent)");
 }
 
+// Operators without a backward: a gradient that an input wants would be lost.
+void refuse_gradients(const char* what, std::initializer_list<const Tensor*> inputs) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor* t : inputs)
+    BFA_RUNTIME(!(t->defined() && t->requires_grad()), what, " has no backward; call it under torch.no_grad()");
+}
+
 // Written in place: autograd finds out from the version that a tensor it saved
 // has changed. (Inference tensors have none.)
 void note_written(const Tensor& t) {
@@ -235,9 +242,10 @@ QkPair rotary_embedding(const OptTensor& query, const OptTensor& key, const Tens
   }
   auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
   if (out) {
-    BFA_VALUE(!(at::GradMode::is_enabled() && ((q.defined() && q.requires_grad()) || (k.defined() && k.requires_grad()))),
-              "out= is not differentiable; call it under torch.no_grad()");
     const Tensor qo = std::get<0>(*out).value_or(Tensor()), ko = std::get<1>(*out).value_or(Tensor());
+    for (const Tensor* t : {&q, &k, &qo, &ko})
+      BFA_VALUE(!(at::GradMode::is_enabled() && t->defined() && t->requires_grad()), "out= is not differentiable; call it under torch.no_grad()");
+    refuse_tangents(what, {&qo, &ko});
     auto fits = [](const Tensor& t, const Tensor& o) {
       return t.defined() == o.defined() &&
              (!t.defined() || (o.sizes() == t.sizes() && o.scalar_type() == t.scalar_type() && o.device() == t.device()));
@@ -307,8 +315,8 @@ std::tuple<Tensor, OptTensor> tree_attention(const Tensor& query, const Tensor& 
   const at::Device dev = first_device(what, query);
   require_cuda(what, key, dev);
   require_cuda(what, value, dev);
-  BFA_RUNTIME(!(at::GradMode::is_enabled() && (query.requires_grad() || key.requires_grad() || value.requires_grad())),
-              "tree_attention has no backward; call it under torch.no_grad()");
+  refuse_gradients(what, {&query, &key, &value, &k_pages, &v_pages});
+  if (alibi_slope) refuse_gradients(what, {&*alibi_slope});
   check_cache(what, {k_pages, v_pages, table, lens}, B, Hkv, D, dt, dev);
   const auto up = check_parents(what, parents, B, N, dev);
   Tensor slopes;
@@ -392,6 +400,7 @@ Tensor cache_append(const Tensor& k_pages, const Tensor& v_pages, const Tensor& 
   refuse_tangents(what, {&key, &value, &k_pages, &v_pages});
   const at::Device dev = first_device(what, key);
   require_cuda(what, value, dev);
+  refuse_gradients(what, {&key, &value, &k_pages, &v_pages});
   check_cache(what, {k_pages, v_pages, table, lens}, B, Hkv, D, key.scalar_type(), dev);
   bfa_append_args a{};
   if (take) {

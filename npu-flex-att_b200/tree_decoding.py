@@ -131,7 +131,8 @@ def cache_append(cache, key, value, *, take=None, count=None):
     (``count`` int32 [B]; None: all S), or with ``take`` (int32 [B, S], a path of
     verify_tree) the tokens take[b, :count[b]] in that order. The page table
     must hold pages for them; a token past it, or with an index outside its
-    table, is not written and is reported by ``check_device_status``.
+    table, is not written and is reported by ``check_device_status``. Not
+    differentiable: inputs that require a gradient are refused.
     """
     out = _binding().cache_append(cache[0], cache[1], cache[2], cache[3], key, value, take, count)
     if _CHECK_STATUS:

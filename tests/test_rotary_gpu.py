@@ -231,3 +231,14 @@ def test_out_is_written_in_place_for_autograd():
     with torch.inference_mode():
         x = torch.randn(1, 2, 9, 64, device=DEV)
     rotary.rotary_embedding(x, None, cos, sin, out=(x, None))
+
+
+@pytest.mark.gpu
+def test_out_that_requires_a_gradient_is_refused():
+    cos, sin = rotary.rotary_table(64, 40, device=DEV)
+    q, k = make(1, 2, 2, 9, 64, torch.float32)
+    for out in ((torch.empty_like(q).requires_grad_(True), torch.empty_like(k)), (torch.empty_like(q), torch.empty_like(k).requires_grad_(True))):
+        with pytest.raises(ValueError, match="not differentiable"):
+            rotary.rotary_embedding(q, k, cos, sin, out=out)
+        with torch.no_grad():
+            rotary.rotary_embedding(q, k, cos, sin, out=out)

@@ -676,3 +676,25 @@ def test_append_is_written_in_place_for_autograd():
         other = td.PagedKVCache(*(t.clone() for t in cache))
     td.cache_append(other, k, v)
     nfa.check_device_status(DEV)
+
+
+@pytest.mark.gpu
+def test_gradients_are_refusals():
+    """No operator of the cache drops a gradient that one of its inputs wants."""
+    g = gen(2)
+    cache = td.PagedKVCache(*page_cache([10], 16, 16, 2, 64, FP, DEV, g, poison=0.0))
+    q, k, v = (torch.randn(1, h, 3, 64, generator=g, device=DEV) for h in (4, 2, 2))
+    slopes = torch.ones(4, device=DEV)
+
+    def grad(t):
+        return t.clone().requires_grad_(True)
+    for call in (lambda: td.tree_attention(grad(q), k, v, cache), lambda: td.tree_attention(q, k, grad(v), cache),
+                 lambda: td.tree_attention(q, k, v, cache._replace(k_pages=grad(cache.k_pages))),
+                 lambda: td.tree_attention(q, k, v, cache, alibi_slope=grad(slopes)),
+                 lambda: td.cache_append(cache, grad(k), v), lambda: td.cache_append(cache, k, grad(v)),
+                 lambda: td.cache_append(cache._replace(v_pages=grad(cache.v_pages)), k, v)):
+        with pytest.raises(RuntimeError, match="no backward"):
+            call()
+        with torch.no_grad():
+            call()
+    nfa.check_device_status(DEV)
