@@ -31,6 +31,7 @@ using at::Tensor;
 using OptTensor = std::optional<Tensor>;
 
 [[noreturn]] void raise(PyObject* type, const std::string& msg) {
+  const py::gil_scoped_acquire gil;  // autograd runs a backward without it
   PyErr_SetString(type, msg.c_str());
   throw py::error_already_set();
 }
@@ -98,6 +99,7 @@ int32_t* status_word(const at::Device& dev) {
   static int32_t* words[64] = {};
   const int i = dev.index();
   if (i < 64 && words[i]) return words[i];
+  const py::gil_scoped_acquire gil;
   const auto at = py::module_::import("bfa_lib").attr("status_ptr")(i).cast<uintptr_t>();
   if (i < 64) words[i] = reinterpret_cast<int32_t*>(at);
   return reinterpret_cast<int32_t*>(at);

@@ -242,3 +242,23 @@ def test_out_that_requires_a_gradient_is_refused():
             rotary.rotary_embedding(q, k, cos, sin, out=out)
         with torch.no_grad():
             rotary.rotary_embedding(q, k, cos, sin, out=out)
+
+
+@pytest.mark.gpu
+def test_a_backward_that_fails_raises():
+    """The backward runs on autograd's own thread, without the interpreter's
+    lock; an error there comes back as an exception (here from saved positions
+    of another dtype)."""
+    cos, sin = rotary.rotary_table(64, 40, device=DEV)
+    q, _ = make(1, 2, 2, 9, 64, torch.float32)
+    q.requires_grad_(True)
+    pos = torch.arange(9, device=DEV)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.double() if t.dtype == torch.int64 else t):
+        out, _ = rotary.rotary_embedding(q, None, cos, sin, pos)
+    torch.cuda.synchronize()
+    with pytest.raises(ValueError, match="int32 or int64"):
+        out.sum().backward()
+    assert q.grad is None
+    out, _ = rotary.rotary_embedding(q, None, cos, sin, pos)
+    out.sum().backward()
+    assert q.grad is not None
