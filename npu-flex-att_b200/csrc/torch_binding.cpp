@@ -12,6 +12,7 @@
 // A failed check raises what the attention functions raise: AssertionError for
 // shapes that do not fit together, ValueError for arguments that make no
 // sense, RuntimeError for dtypes and devices.
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -207,6 +208,22 @@ std::tuple<Tensor, Tensor> rope_apply(const Tensor& q, const Tensor& k, const Te
   return {q.defined() ? out[0] : Tensor(), k.defined() ? out.back() : Tensor()};
 }
 
+// Whether two tensors of one shape are the same elements (strides of dims of
+// length 1 do not count).
+bool same_elements(const Tensor& a, const Tensor& b) {
+  if (a.data_ptr() != b.data_ptr()) return false;
+  for (int i = 0; i < 4; ++i)
+    if (a.size(i) > 1 && a.stride(i) != b.stride(i)) return false;
+  return true;
+}
+// Whether they are known to share memory (ATen's rule, which leaves views that
+// interleave in one buffer to the caller, plus equal addresses).
+bool share_memory(const Tensor& a, const Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const auto status = at::get_overlap_status(a, b);
+  return status == at::MemOverlapStatus::Full || status == at::MemOverlapStatus::Partial || a.data_ptr() == b.data_ptr();
+}
+
 using QkPair = std::tuple<OptTensor, OptTensor>;
 
 QkPair rotary_embedding(const OptTensor& query, const OptTensor& key, const Tensor& cos, const Tensor& sin, const OptTensor& positions,
@@ -254,6 +271,14 @@ QkPair rotary_embedding(const OptTensor& query, const OptTensor& key, const Tens
     };
     BFA_VALUE(fits(q, qo), "out for query must match it in shape, dtype and device");
     BFA_VALUE(fits(k, ko), "out for key must match it in shape, dtype and device");
+    for (const Tensor* t : {&qo, &ko})
+      BFA_VALUE(!t->defined() || at::has_internal_overlap(*t) != at::MemOverlap::Yes, "out has elements that share memory");
+    // The heads are turned side by side, in no order: a result may lie where its
+    // own input does and nowhere else among what the call reads and writes.
+    auto apart = [](const Tensor& a, const Tensor& b) { return !a.defined() || !b.defined() || !share_memory(a, b); };
+    BFA_VALUE((!q.defined() || same_elements(q, qo) || apart(q, qo)) && (!k.defined() || same_elements(k, ko) || apart(k, ko)) &&
+                  apart(qo, k) && apart(ko, q) && apart(qo, ko),
+              "out may be the inputs themselves, but not overlap them, or itself, in another way");
     rope_launch(q, k, cos, sin, pos, off, interleaved, false, qo, ko);
     note_written(qo), note_written(ko);
     return {std::get<0>(*out), std::get<1>(*out)};

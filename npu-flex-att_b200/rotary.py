@@ -79,8 +79,9 @@ def rotary_embedding(query, key, cos, sin, positions=None, offsets=None, *, inte
     (x[2i], x[2i+1]). A position outside the table gives NaN rows and is
     reported by ``check_device_status``.
 
-    ``out`` (a pair like (query, key), which may be the inputs themselves)
-    receives the results in place of new tensors; not differentiable.
+    ``out`` (a pair like (query, key), which may be the inputs themselves but may
+    not overlap them, or itself, in another way) receives the results in place
+    of new tensors; not differentiable.
     """
     pair = _binding().rotary_embedding(query, key, cos, sin, positions, offsets, bool(interleaved), out)
     if _CHECK_STATUS:

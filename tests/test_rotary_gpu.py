@@ -262,3 +262,35 @@ def test_a_backward_that_fails_raises():
     out, _ = rotary.rotary_embedding(q, None, cos, sin, pos)
     out.sum().backward()
     assert q.grad is not None
+
+
+@pytest.mark.gpu
+def test_out_may_not_overlap_but_in_place():
+    cos, sin = rotary.rotary_table(64, 40, device=DEV)
+    flat = torch.randn(4, 2, 2, 9, 64, device=DEV)
+    q, k, a, b = flat
+    late = flat.view(-1)[64:64 + q.numel()].view(q.shape)       # q, a row later
+    wide = torch.empty(2, 1, 9, 64, device=DEV).expand(2, 2, 9, 64)
+    turned = q.view(2, 9, 2, 64).transpose(1, 2)                # q's memory in another order
+    for out in ((late, b), (wide, b), (turned, b), (k, q), (k, b), (a, q), (a, a), (a, flat.view(-1)[2 * q.numel() + 64:][:k.numel()].view(k.shape))):
+        with pytest.raises(ValueError, match="overlap|share memory"):
+            rotary.rotary_embedding(q, k, cos, sin, out=out)
+    want = rotary.rotary_embedding(q, k, cos, sin)
+    for out in ((a, b), (a, k.clone()), (q.clone(), b)):
+        rotary.rotary_embedding(q, k, cos, sin, out=out)
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+    # In place: dense, one of the two, and interleaved in one projection's output.
+    x, y = q.clone(), k.clone()
+    rotary.rotary_embedding(x, y, cos, sin, out=(x, a))
+    assert torch.equal(x, want[0]) and torch.equal(a, want[1])
+    both = torch.cat((q, k), 1).transpose(1, 2).contiguous()    # [B, S, Hq + Hkv, D]
+    x, y = both.transpose(1, 2).split(2, 1)
+    rotary.rotary_embedding(x, y, cos, sin, out=(x, y))
+    assert torch.equal(x, want[0]) and torch.equal(y, want[1])
+    with pytest.raises(ValueError, match="overlap"):
+        rotary.rotary_embedding(x, y, cos, sin, out=(y, x))
+    # One head: its stride says nothing.
+    x = q[:, :1].clone()
+    other = x.as_strided(x.shape, (x.stride(0), 7, 64, 1))
+    rotary.rotary_embedding(x, None, cos, sin, out=(other, None))
+    assert torch.equal(x, want[0][:, :1])
