@@ -175,18 +175,25 @@ struct RotaryEmbedding : torch::autograd::Function<RotaryEmbedding> {
     ctx->saved_data["interleaved"] = interleaved;
     ctx->saved_data["inverse"] = inverse;
     ctx->saved_data["q"] = qt.defined();
-    ctx->saved_data["k"] = kt.defined();
+    // An input that needs no gradient gets none, and its output wants none.
+    const bool need_q = qt.defined() && qt.requires_grad(), need_k = kt.defined() && kt.requires_grad();
+    ctx->saved_data["need_q"] = need_q;
+    ctx->saved_data["need_k"] = need_k;
     const Tensor qo = like(qt), ko = like(kt);
     rope_launch(qt, kt, cos, sin, pt, ot, interleaved, inverse, qo, ko);
-    torch::autograd::variable_list out;
+    torch::autograd::variable_list out, constant;
     if (qo.defined()) out.push_back(qo);
     if (ko.defined()) out.push_back(ko);
+    if (qo.defined() && !need_q) constant.push_back(qo);
+    if (ko.defined() && !need_k) constant.push_back(ko);
+    ctx->mark_non_differentiable(constant);
     return out;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const bool has_q = ctx->saved_data["q"].toBool(), has_k = ctx->saved_data["k"].toBool();
-    const Tensor dq = has_q ? grads[0] : Tensor(), dk = has_k ? grads[has_q ? 1 : 0] : Tensor();
+    const bool has_q = ctx->saved_data["q"].toBool();
+    const Tensor dq = ctx->saved_data["need_q"].toBool() ? grads[0] : Tensor();
+    const Tensor dk = ctx->saved_data["need_k"].toBool() ? grads[has_q ? 1 : 0] : Tensor();
     Tensor gq, gk;
     if (dq.defined() || dk.defined())
       std::tie(gq, gk) = rope_apply(dq, dk, saved[0], saved[1], saved[2], saved[3], ctx->saved_data["interleaved"].toBool(),

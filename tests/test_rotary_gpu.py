@@ -294,3 +294,24 @@ def test_out_may_not_overlap_but_in_place():
     other = x.as_strided(x.shape, (x.stride(0), 7, 64, 1))
     rotary.rotary_embedding(x, None, cos, sin, out=(other, None))
     assert torch.equal(x, want[0][:, :1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", [0, 1])
+def test_an_input_without_gradient_gets_none(which):
+    """Its output requires none either, and the backward turns the other's alone."""
+    cos, sin = rotary.rotary_table(64, 40, device=DEV)
+    pair = list(make(1, 2, 1, 9, 64, torch.bfloat16, seed=8))
+    pair[which].requires_grad_(True)
+    out = rotary.rotary_embedding(*pair, cos, sin)
+    assert out[which].requires_grad and not out[1 - which].requires_grad
+    w = torch.randn_like(out[which])
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_stats()["allocation.all.allocated"]
+    (g,) = torch.autograd.grad((out[which],), (pair[which],), (w,))
+    assert torch.cuda.memory_stats()["allocation.all.allocated"] - before == 1
+    close(g, *exact(w, cos, sin, torch.arange(9, device=DEV)[None], False, True))
+    # Through a sum of both outputs, and through a second derivative.
+    out = rotary.rotary_embedding(*pair, cos, sin)
+    (g,) = torch.autograd.grad(sum((t.float() ** 2).sum() for t in out), pair[which], create_graph=True)
+    assert g.requires_grad and torch.autograd.grad(g.float().sum(), pair[which])[0] is not None
