@@ -178,8 +178,8 @@ int launch_typed(RopeParams& p, const bfa_rope_args& a, cudaStream_t st) {
   constexpr int E = 16 / (int)sizeof(T);
   const bool il = a.interleaved != 0;
   const bool in_place = same_place(a.q, a.q_out) && (a.heads_k == 0 || same_place(a.k, a.k_out));
-  bool vec = p.R % (il ? E : 2 * E) == 0 && p.D % E == 0 && vector_rows(a.q, sizeof(T)) && vector_rows(a.q_out, sizeof(T));
-  vec = vec && (((uintptr_t)a.cos | (uintptr_t)a.sin) & 15u) == 0 && a.table_stride % 4 == 0;
+  bool vec = p.R % (il ? E : 2 * E) == 0 && p.D % E == 0 && (((uintptr_t)a.cos | (uintptr_t)a.sin) & 15u) == 0 && a.table_stride % 4 == 0;
+  if (a.heads_q > 0) vec = vec && vector_rows(a.q, sizeof(T)) && vector_rows(a.q_out, sizeof(T));
   if (a.heads_k > 0) vec = vec && vector_rows(a.k, sizeof(T)) && vector_rows(a.k_out, sizeof(T));
   if (il) return vec ? launch_rope<T, true, E>(p, in_place, st) : launch_rope<T, true, 1>(p, in_place, st);
   return vec ? launch_rope<T, false, E>(p, in_place, st) : launch_rope<T, false, 1>(p, in_place, st);

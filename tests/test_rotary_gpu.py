@@ -315,3 +315,27 @@ def test_an_input_without_gradient_gets_none(which):
     out = rotary.rotary_embedding(*pair, cos, sin)
     (g,) = torch.autograd.grad(sum((t.float() ** 2).sum() for t in out), pair[which], create_graph=True)
     assert g.requires_grad and torch.autograd.grad(g.float().sum(), pair[which])[0] is not None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_a_key_alone_costs_what_a_query_alone_does(interleaved):
+    """The same tensor in either place takes the same (vector) form of the kernel."""
+    cos, sin = rotary.rotary_table(128, 4096, device=DEV)
+    x, _ = make(4, 32, 1, 4096, 128, torch.bfloat16)
+    out = torch.empty_like(x)
+
+    def best(call):
+        times = []
+        for _ in range(8):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record(), call(), b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+    alone = best(lambda: rotary.rotary_embedding(x, None, cos, sin, interleaved=interleaved, out=(out, None)))
+    want = out.clone()
+    key = best(lambda: rotary.rotary_embedding(None, x, cos, sin, interleaved=interleaved, out=(None, out)))
+    assert torch.equal(out, want)
+    # The element-wise form takes several times as long; boxes vary by a few percent.
+    assert key < 1.5 * alone, (key, alone)
