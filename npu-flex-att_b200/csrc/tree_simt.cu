@@ -30,19 +30,18 @@ struct SimtShared {
   alignas(16) float alpha[kRows];
 };
 
-template <typename T>
 __device__ __forceinline__ void copy_row_piece(float* dst, const char* src, int d, int D, bool vec) {
   // 4 elements of a row; zeros past D and for a missing row.
-  if (sizeof(T) == 4 && vec && src && d < D) {
+  if (vec && src && d < D) {
     const uint32_t s = (uint32_t)__cvta_generic_to_shared(dst);
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(src + (int64_t)d * 4) : "memory");
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) dst[i] = (src && d + i < D) ? to_f32<T>(reinterpret_cast<const T*>(src)[d + i]) : 0.f;
+  for (int i = 0; i < 4; ++i) dst[i] = (src && d + i < D) ? reinterpret_cast<const float*>(src)[d + i] : 0.f;
 }
 
-template <typename T, int D>  // D: head dim rounded up to 64, 128 or 256
+template <int D>  // head dim rounded up to 64, 128 or 256
 __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const TreeParams p, bool vec) {
   constexpr int kPitch = D + 4;  // floats; 16-byte rows shifted against each other
   constexpr int kPieces = D / 4;                    // 16-byte pieces of a row
@@ -78,7 +77,7 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const TreeParams p,
   auto lookup = [&](int buf) {  // fills the row addresses of chunk `ahead`
     if (tid < kKeys) {
       const char *kr, *vr;
-      tree_key_rows<(int)sizeof(T)>(p, ahead, tid, &kr, &vr);
+      tree_key_rows<4>(p, ahead, tid, &kr, &vr);
       sh.krow[buf][tid] = kr;
       sh.vrow[buf][tid] = vr;
     }
@@ -87,8 +86,8 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const TreeParams p,
   auto load = [&](int buf) {
     for (int i = tid; i < kKeys * kPieces; i += kThreads) {
       const int n = i / kPieces, d = (i % kPieces) * 4;
-      copy_row_piece<T>(ks + (buf * kKeys + n) * kPitch + d, sh.krow[buf][n], d, p.D, vec);
-      copy_row_piece<T>(vs + (buf * kKeys + n) * kPitch + d, sh.vrow[buf][n], d, p.D, vec);
+      copy_row_piece(ks + (buf * kKeys + n) * kPitch + d, sh.krow[buf][n], d, p.D, vec);
+      copy_row_piece(vs + (buf * kKeys + n) * kPitch + d, sh.vrow[buf][n], d, p.D, vec);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -118,7 +117,7 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const TreeParams p,
         if (r < R && d < p.D) {
           int hq, n;
           tree_row(p, hkv, rb0 + r, &hq, &n);
-          x_ = to_f32<T>(static_cast<const T*>(p.q)[cur.b * p.sq[0] + hq * p.sq[1] + n * p.sq[2] + d]);
+          x_ = static_cast<const float*>(p.q)[cur.b * p.sq[0] + hq * p.sq[1] + n * p.sq[2] + d];
         }
         qs[r * kPitch + d] = x_;
       }
@@ -258,7 +257,7 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const TreeParams p,
           if (d >= p.D) continue;
           const float o = inv != 0.f ? acc[a][i][c] * inv : 0.f;
           if (whole)
-            static_cast<T*>(p.o)[done.b * p.so[0] + hq * p.so[1] + n * p.so[2] + d] = from_f32<T>(o);
+            static_cast<float*>(p.o)[done.b * p.so[0] + hq * p.so[1] + n * p.so[2] + d] = o;
           else
             p.part_o[(prow + r) * p.D + d] = o;
         }
@@ -273,10 +272,10 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const TreeParams p,
   }
 }
 
-template <typename T, int D>
+template <int D>
 int launch(const TreeParams& p, cudaStream_t st) {
   const int bytes = (int)(sizeof(SimtShared) + 15) / 16 * 16 + (kRows + 4 * kKeys) * (D + 4) * 4;
-  auto kernel = tree_simt_kernel<T, D>;
+  auto kernel = tree_simt_kernel<D>;
   static std::atomic<uint64_t> done;
   const int rc = allow_shared(kernel, bytes, done, "tree attention shared memory");
   if (rc) return rc;
@@ -292,9 +291,9 @@ int launch(const TreeParams& p, cudaStream_t st) {
 }  // namespace
 
 int tree_simt(const TreeParams& p, cudaStream_t st) {
-  if (p.D <= 64) return launch<float, 64>(p, st);
-  if (p.D <= 128) return launch<float, 128>(p, st);
-  return launch<float, 256>(p, st);
+  if (p.D <= 64) return launch<64>(p, st);
+  if (p.D <= 128) return launch<128>(p, st);
+  return launch<256>(p, st);
 }
 
 }  // namespace bfa
