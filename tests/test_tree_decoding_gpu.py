@@ -698,3 +698,49 @@ def test_gradients_are_refusals():
         with torch.no_grad():
             call()
     nfa.check_device_status(DEV)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,N,Hq,D", [(BF, 6, 8, 128), (HF, 40, 8, 64), (BF, 9, 4, 256), (FP, 5, 4, 64)])
+def test_a_step_inside_a_cuda_graph(dtype, N, Hq, D):
+    """A captured step (rotary at the nodes' positions, attention, verification,
+    append) gives on other inputs what the calls give outside the graph."""
+    import rotary
+    g = gen(17)
+    B, Hkv, V, page = 3, 2, 1000, 16
+    lens = [300, 41, 0]
+    cos, sin = rotary.rotary_table(D, 500, device=DEV)
+    kp, vp, table, ln = page_cache([n + N for n in lens], 352, page, Hkv, D, dtype, DEV, g, poison=0.0)
+    ln.copy_(torch.tensor(lens, device=DEV))
+    up = torch.tensor(tree("binary", N, B), dtype=torch.int32, device=DEV)
+
+    def fresh(seed):
+        h = gen(seed)
+        q, k, v = (torch.randn(B, n, N, D, generator=h, device=DEV).to(dtype) for n in (Hq, Hkv, Hkv))
+        p = torch.softmax(torch.randn(B, N, V, generator=h, device=DEV) * 3, -1).to(dtype)
+        tokens = p.float().topk(2, -1).indices.flatten(1)[:, :N].contiguous()
+        noise = torch.empty(B, V, device=DEV).exponential_(generator=h).clamp_(min=1e-20)
+        return [q, k, v, p, tokens, torch.rand(B, N, generator=h, device=DEV), noise, kp.clone(), vp.clone(), ln + seed % 3 * (ln > 0).int(), up.clone()]
+
+    def step(q, k, v, p, tokens, u, noise, kp, vp, ln, up):
+        cache = td.PagedKVCache(kp, vp, table, ln)
+        q, k = rotary.rotary_embedding(q, k, cos, sin, td.tree_depths(up), ln)
+        o, lse = td.tree_attention(q, k, v, cache, up, return_lse=True)
+        path, count, token = td.verify_tree(p, tokens, up, u, noise)
+        return [q, k, o, lse, path, count, token, td.cache_append(cache, k, v, take=path, count=count), kp, vp]
+    held = fresh(0)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step(*(t.clone() for t in held))  # first calls set the kernels up
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        got = step(*held)
+    for seed in (1, 2, 5):
+        for t, x in zip(held, fresh(seed)):
+            t.copy_(x)
+        graph.replay()
+        for a, b in zip(got, step(*fresh(seed))):
+            assert torch.equal(a, b)
+    nfa.check_device_status(DEV)
