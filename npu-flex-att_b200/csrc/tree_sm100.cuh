@@ -21,7 +21,8 @@
 //               TMA, a lane per box, into a ring that runs on across items
 //   warp 1      MMA issuer
 //   warp 2      also allocates TMEM
-//   warp 3      the tree's ancestor sets, one item ahead
+//   warp 3      the tree's ancestor sets, one item ahead; REP = 4: items whose O
+//               holds columns that are not finite
 //   warps 4..   softmax, 8 warps per 128-row tile: two threads share a row (TMEM
 //               lane), each with half of the chunk's keys and of O's columns;
 //               they agree on the row's maximum through shared memory. P (16-bit)
@@ -103,7 +104,11 @@ struct TreeMisc {
   unsigned long long bad[3][2];  // by the chunk's number mod 3: its keys whose values are not finite
   float top[2][2][2][kBM];       // row maxima: chunk's parity, tile, half of the keys, row
   float sum[2][2][kBM];          // row sums at an item's end: tile, half, row
-  float quarter[2][kBM];         // REP = 4: maxima and sums of the quarters
+  float quarter[kBM];            // REP = 4: maxima of the quarters, their sums by the item's parity,
+  float total[2][kBM];
+  int odd[2];                    // whether its O holds columns that are not finite,
+  TreeCursor item[2];            // and its place, with the chunks of it that are this block's
+  int count[2];
   TreeMasks masks[2];            // by the item's parity
 };
 static_assert(sizeof(TreeMisc) <= 10240, "misc");
@@ -163,35 +168,80 @@ __device__ __forceinline__ bool any_not_finite(uint32_t w) {
   return (w & e) == e || ((w >> 16) & e) == e;
 }
 
-// Eight columns of O, from column d on, of a row that sees cached keys [from, to)
-// and the nodes `seen` of this block's keys: where a column is not finite, it
-// is the sum of the values of V there that are not (a positive weight changes
-// none). With the rows stored four times such a value meets the zeros that P
-// holds for three of the quarters, and comes out as NaN in place of infinity.
-// Only broken inputs come here, so nothing is done for speed.
-template <bool BF16>
-__device__ __noinline__ void sum_not_finite(const TreeParams& p, int b, int hkv, int from, int to, uint64_t seen, int d, float* f) {
-  float sum[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) sum[e] = 0.f;
-  auto add = [&](const void* v, int64_t at) {
-    const uint4 w4 = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(v) + at + d);
+// With the rows stored four times, a value of V that is not finite meets the
+// zeros that P holds for three of the quarters, and comes out as NaN in place of
+// infinity. So where columns of an item's rows are not finite, they are formed
+// again: the sum of the values of V there that are not finite, over this
+// block's keys that the row sees (a positive weight changes none of them). Only
+// broken inputs come here. Called by the warp of the ancestor sets once the item
+// is stored: one token over 4095 takes 13.4 us with it and 13.1 without (called
+// by the softmax warps 14.0, inlined into that warp's part 14.2).
+// `cur`: the item and the first of `count` chunks; sums: the quarters' row sums.
+template <int D, bool BF16>
+__device__ __noinline__ void sum_not_finite(const TreeParams& p, const TreeMasks& masks, const float* sums, TreeCursor cur, int count) {
+  const int lane = threadIdx.x & 31;
+  const int hkv = cur.item / p.n_rb, r = (cur.item - hkv * p.n_rb) * p.rb + lane, end = cur.c + count;
+  auto finite = [](float x) { return fabsf(x) < __int_as_float(0x7f800000); };
+  auto row_of = [&](int key) -> int64_t {  // of a cached key in v_pages, -1: a bad page
+    const int page = p.table[cur.b * p.table_stride + key / p.page];
+    return page >= 0 && page < p.num_pages ? page * p.svp[0] + hkv * p.svp[1] + key % p.page * p.svp[2] : -1;
+  };
+  // Cached keys [from, some): in chunks where rows differ in what they see;
+  // [some, to): seen by all. Of those, a lane collects which signs (NaN: both)
+  // its 8 columns hold.
+  const int from = cur.lo + cur.c * p.chunk, to = min(cur.len, cur.lo + end * p.chunk);
+  const int all_from = p.window > 0 ? cur.len + p.N - 1 - p.window : 0;
+  const int some = min(to, max(from, cur.lo + (max(all_from - cur.lo, 0) + p.chunk - 1) / p.chunk * p.chunk));
+  uint32_t up = 0, down = 0;
+#pragma unroll 1
+  for (int key = some; key < to; ++key) {
+    const int64_t at = row_of(key);
+    if (at < 0 || lane * 8 >= p.D) continue;
+    const uint4 w4 = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.vp) + at + lane * 8);
     const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float x = half_of<BF16>(w[e >> 1], e & 1);
-      if (!(fabsf(x) < __int_as_float(0x7f800000))) sum[e] += x;
+      if (!finite(x)) {
+        if (!(x < 0.f)) up |= 1u << e;
+        if (!(x > 0.f)) down |= 1u << e;
+      }
     }
-  };
-  for (int key = from; key < to; ++key) {
-    const int page = p.table[b * p.table_stride + key / p.page];
-    if (page >= 0 && page < p.num_pages) add(p.vp, page * p.svp[0] + hkv * p.svp[1] + key % p.page * p.svp[2]);
   }
-  for (int n = 0; n < p.N; ++n)
-    if ((seen >> n) & 1) add(p.v, b * p.sv[0] + hkv * p.sv[1] + n * p.sv[2]);
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (!(fabsf(f[e]) < __int_as_float(0x7f800000)) && sum[e] != 0.f) f[e] = sum[e];
+  // Then a lane per row.
+  const float all = (sums[lane] + sums[32 + lane]) + (sums[64 + lane] + sums[96 + lane]);
+  const bool live = r < p.G * p.N && all == all;  // a row sum that is NaN: the logits were no numbers, and O stays NaN
+  int hq, node;
+  tree_row(p, hkv, live ? r : 0, &hq, &node);
+  const int depth = masks.depth[node];
+  const int low = p.window > 0 ? max(from, cur.len + depth - p.window) : from;
+  const bool whole = cur.c == 0 && count == cur.n;
+#pragma unroll 1
+  for (int d = 0; d < p.D; ++d) {
+    const bool pos = (__shfl_sync(0xffffffffu, up, d >> 3) >> (d & 7)) & 1, neg = (__shfl_sync(0xffffffffu, down, d >> 3) >> (d & 7)) & 1;
+    uint16_t* out = static_cast<uint16_t*>(p.o) + cur.b * p.so[0] + hq * p.so[1] + node * p.so[2] + d;
+    float* part = p.part_o + (((int64_t)blockIdx.x * 2 + (cur.c > 0 ? 0 : 1)) * p.rb + lane) * p.D + d;
+    if (!live || finite(whole ? half_of<BF16>(*out, 0) : *part)) continue;
+    float sum = (pos ? __int_as_float(0x7f800000) : 0.f) + (neg ? __int_as_float(0xff800000) : 0.f);
+    auto add = [&](const void* v, int64_t at) {
+      const float x = half_of<BF16>(static_cast<const uint16_t*>(v)[at + d], 0);
+      if (!finite(x)) sum += x;
+    };
+#pragma unroll 1
+    for (int key = low; key < some; ++key) {
+      const int64_t at = row_of(key);
+      if (at >= 0) add(p.vp, at);
+    }
+    if (end > cur.n - p.tree_chunks)
+#pragma unroll 1
+      for (int n = 0; n < p.N; ++n)
+        if (((masks.anc[node] >> n) & 1) && (p.window == 0 || depth - masks.depth[n] <= p.window))
+          add(p.v, cur.b * p.sv[0] + hkv * p.sv[1] + n * p.sv[2]);
+    if (sum == 0.f) continue;
+    if (whole) *out = (uint16_t)pack2<BF16>(sum, 0.f);
+    else *part = sum;
+  }
+  __syncwarp();
 }
 
 template <int D, int NT, int REP, bool BF16, bool CAP, bool ALIBI>
@@ -244,6 +294,7 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
     for (int i = 0; i < kNumBars; ++i)
       mbar_init(bar(i), i == kQFull || i == kMaskFree || i == kMaskFree + 1 ? 8u * NT : i >= kPFull && i < kODone ? 8u : 1u);
     mi.abort = 0;
+    mi.odd[0] = mi.odd[1] = 0;
     fence_barrier_init();
   }
   if (warp == 2) {
@@ -442,6 +493,10 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
     for (int x = 0; x < n_x && ok; ++seg) {
       const int count = min(cur.n - cur.c, n_x - x);
       if (seg > 1) ok = warp_wait(bar(kMaskFree + (seg & 1)), (uint32_t)(((seg >> 1) - 1) & 1), ctl);
+      if constexpr (REP == 4) {
+        if (ok && mi.odd[seg & 1]) sum_not_finite<D, BF16>(p, mi.masks[seg & 1], mi.total[seg & 1], mi.item[seg & 1], mi.count[seg & 1]);
+        if (lane == 0) mi.odd[seg & 1] = 0, mi.item[seg & 1] = cur, mi.count[seg & 1] = count;
+      }
       tree_masks(p, cur.b, mi.masks[seg & 1]);
       if (lane == 0) {
         if (p.status && p.lens[cur.b] != cur.len) *p.status = BFA_ERR_INDEX;
@@ -794,16 +849,16 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
         if constexpr (REP == 4) {
           // The quarters' maxima and sums: weights 2^(m - top) / sum.
           if (h == 0) {
-            mi.quarter[0][trow] = l != 0.f ? m : neg_inf();
-            mi.quarter[1][trow] = l;
+            mi.quarter[trow] = l != 0.f ? m : neg_inf();
+            mi.total[seg & 1][trow] = l;
           }
           named_sync(3, kSoft);
           float top = neg_inf(), sum = 0.f;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) top = fmaxf(top, mi.quarter[0][q * 32 + lane]);
+          for (int q = 0; q < 4; ++q) top = fmaxf(top, mi.quarter[q * 32 + lane]);
           const float use = top == neg_inf() ? 0.f : top;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) sum += mi.quarter[1][q * 32 + lane] * ex2(mi.quarter[0][q * 32 + lane] - use);
+          for (int q = 0; q < 4; ++q) sum += mi.total[seg & 1][q * 32 + lane] * ex2(mi.quarter[q * 32 + lane] - use);
           scale = l != 0.f ? ex2(m - use) / sum : 0.f;
           m = top;
           l = sum;
@@ -842,6 +897,7 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
           constexpr int kU = D / 8;
           float4* join = reinterpret_cast<float4*>(smem);
           auto unit = [&](int q, int r, int u) { return join + (q * 32 + r) * kU + (u ^ (r & 7)); };
+          bool odd = false;  // columns that are not finite
 #pragma unroll 1
           for (int c0 = 0; c0 < D / 2; c0 += D / 4) {
 #pragma unroll
@@ -863,32 +919,14 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
                 y.x += b.x, y.y += b.y, y.z += b.z, y.w += b.w;
               }
               const int64_t at = __shfl_sync(0xffffffffu, place, r);
-              const int d = u / (kU / 2) * (D / 2) + c0 + u % (kU / 2) * 4;
               // 0·x is 0, or NaN where x is not finite.
-              const float probe = ((x.x * 0.f + x.y * 0.f) + (x.z * 0.f + x.w * 0.f)) + ((y.x * 0.f + y.y * 0.f) + (y.z * 0.f + y.w * 0.f));
-              if (probe != 0.f && at >= 0 && d < p.D) {
-                const float all = (mi.quarter[1][r] + mi.quarter[1][32 + r]) + (mi.quarter[1][64 + r] + mi.quarter[1][96 + r]);
-                if (all == all) {  // else the logits were no numbers, and O stays NaN
-                  int hq_, node_;
-                  const int hkv = cur.item / p.n_rb;
-                  tree_row(p, hkv, (cur.item - hkv * p.n_rb) * p.rb + r, &hq_, &node_);
-                  const int depth = masks.depth[node_], end = cur.c + count;
-                  uint64_t sees = end > cur.n - p.tree_chunks ? masks.anc[node_] : 0ull;
-                  if (p.window > 0)
-                    for (int m_ = 0; m_ < p.N; ++m_)
-                      if (depth - masks.depth[m_] > p.window) sees &= ~(1ull << m_);
-                  int from = cur.lo + cur.c * CH;
-                  if (p.window > 0) from = max(from, cur.len + depth - p.window);
-                  float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-                  sum_not_finite<BF16>(p, cur.b, hkv, from, min(cur.len, cur.lo + end * CH), sees, d, f);
-                  x = make_float4(f[0], f[1], f[2], f[3]);
-                  y = make_float4(f[4], f[5], f[6], f[7]);
-                }
-              }
-              put8(at, d, x, y);
+              const float probe = ((x.x + x.y) + (x.z + x.w)) * 0.f + ((y.x + y.y) + (y.z + y.w)) * 0.f;
+              odd |= probe != 0.f && at >= 0;
+              put8(at, u / (kU / 2) * (D / 2) + c0 + u % (kU / 2) * 4, x, y);
             }
             named_sync(3, kSoft);
           }
+          if (odd) mi.odd[seg & 1] = 1;
         } else {
           // Turned in shared memory, kW columns at a time, so that lanes side by
           // side store one row's pieces (a lane per row: 32 lines a store). The
@@ -933,6 +971,9 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  if (REP == 4 && warp == 3 && (mi.odd[0] | mi.odd[1]))  // the block's last two items
+    for (int i = 0; i < 2; ++i)
+      if (mi.odd[i]) sum_not_finite<D, BF16>(p, mi.masks[i], mi.total[i], mi.item[i], mi.count[i]);
 }
 
 constexpr uint64_t kTimeoutNs = 1000000000ull;

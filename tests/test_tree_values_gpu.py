@@ -215,3 +215,23 @@ def test_values_behind_the_window_do_not_spread(dtype, bad, N, Hq, D, window):
     o, lse = td.tree_attention(q, k, v, cache, up, sliding_window=window, return_lse=True)
     compare(o[keep], lse[keep], ref[0][keep], ref[1][keep], ref[2][keep])
     nfa.check_device_status(DEV)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("N,window", [(1, 0), (2, 0), (2, 9)])
+def test_infinite_values_in_many_short_sequences(dtype, N, window):
+    """Several items to a block, each with columns of its own that are infinite."""
+    B = 700
+    lens = [20 + b % 3 for b in range(B)]
+    q, k, v, cache, parents, up = problem(lens, N, 1, 64, dtype, "chain", 29)
+    for b in range(0, B, 3 if N == 1 else 1):
+        cache.v_pages[slot(cache, b, lens[b] - 3)[:3] + (b % 64,)] = math.inf if b % 2 else -math.inf
+    ref = attention(q, k, v, cache, parents, window=window)
+    o, lse = td.tree_attention(q, k, v, cache, up, sliding_window=window, return_lse=True)
+    same_values(o, ref[0])
+    fine = ref[0].isfinite()
+    u = 2.0 ** -24 if dtype == FP else 2.0 ** -8
+    tol = 1.5 * u * ref[2] + u * ref[0].abs() + 1e-4 * (ref[2] + 1)
+    assert ((o.double() - ref[0]).abs() <= tol)[fine].all()
+    assert ((lse.double() - ref[1]).abs() <= 1e-4 * (1 + ref[1].abs())).all()
