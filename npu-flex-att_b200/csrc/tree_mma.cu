@@ -465,7 +465,10 @@ __global__ void __launch_bounds__(32 * RW * KW, (Tile<D, RW, KW>::kPerSm)) tree_
     const bool whole = seg_c0 == 0 && last;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      if (anc[h] == 0) l[h] = 0.f;  // an absent node: chunks that are not masked were summed for it too
+      if (anc[h] == 0) {  // an absent node: chunks that are not masked were summed for it too
+        l[h] = 0.f;
+        m[h] = neg_inf();  // which an infinite logit may have made infinite
+      }
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
     }

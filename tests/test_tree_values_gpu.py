@@ -235,3 +235,18 @@ def test_infinite_values_in_many_short_sequences(dtype, N, window):
     tol = 1.5 * u * ref[2] + u * ref[0].abs() + 1e-4 * (ref[2] + 1)
     assert ((o.double() - ref[0]).abs() <= tol)[fine].all()
     assert ((lse.double() - ref[1]).abs() <= 1e-4 * (1 + ref[1].abs())).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("D", [64, 136])
+@pytest.mark.parametrize("N,Hq", [(5, 1), (12, 2), (31, 4), (64, 4)])
+def test_absent_rows_stay_empty_over_infinite_logits(dtype, D, N, Hq):
+    """One infinite entry of an absent node's query makes its logits infinite,
+    not NaN, over whole chunks of cached keys: the row is empty all the same."""
+    q, k, v, cache, parents, up = problem([900, 22], N, Hq, D, dtype, "star", 30)
+    up[:, 2:4] = -1
+    for h, bad in enumerate([math.inf, -math.inf, math.inf, math.nan][:Hq]):
+        q[:, h, 2, h], q[:, h, 3, D - 1] = bad, -bad
+    ref = attention(q, k, v, cache, up.tolist())
+    compare(*td.tree_attention(q, k, v, cache, up, return_lse=True), *ref)
