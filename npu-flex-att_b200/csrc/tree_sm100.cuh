@@ -153,6 +153,13 @@ __device__ __forceinline__ bool elect_one() {
   return r != 0;
 }
 
+// tanh by sign(x)·(1 - 2/(1 + e^{2|x|})). Where tanh_any keeps its exponent below
+// 126, e^{2|x|} may run to infinity here (the quotient is 0 either way): the
+// bound would turn NaN into 1.
+__device__ __forceinline__ float tanh_of(float x) {
+  return copysignf(1.0f - 2.0f * rcp(1.0f + ex2(2.0f * kLog2e * fabsf(x))), x);
+}
+
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return BF16 ? pack_bf16(a, b) : pack_f16(a, b);
@@ -670,8 +677,12 @@ __global__ void __launch_bounds__(TreeLayout<D, NT, REP>::kThreads, 1)
               }
             }
             if (CAP) {
-              float2 th;
-              y = cap_logit2x2<TIER>(raw, cap_in, cap_out, &th);
+              if constexpr (TIER == 0) {
+                y = make_float2(cap_out * tanh_of(cap_in * raw.x), cap_out * tanh_of(cap_in * raw.y));
+              } else {
+                float2 th;
+                y = cap_logit2x2<TIER>(raw, cap_in, cap_out, &th);
+              }
               if (ALIBI) y = __fadd2_rn(y, bias);
             } else {
               y = __ffma2_rn(raw, make_float2(sl2, sl2), bias);

@@ -250,3 +250,25 @@ def test_absent_rows_stay_empty_over_infinite_logits(dtype, D, N, Hq):
         q[:, h, 2, h], q[:, h, 3, D - 1] = bad, -bad
     ref = attention(q, k, v, cache, up.tolist())
     compare(*td.tree_attention(q, k, v, cache, up, return_lse=True), *ref)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("cap", [0.5, 5.0, 100.0])
+@pytest.mark.parametrize("N,Hq,D", [(9, 2, 64), (40, 2, 128), (64, 4, 128), (6, 2, 256)])
+def test_a_cap_passes_nan_on_and_bounds_infinities(dtype, cap, N, Hq, D):
+    """NaN under the cap stays NaN, whichever form of tanh the logits beside it
+    take; an infinite logit is a finite one there, plus or minus the cap."""
+    q, k, v, cache, parents, up = problem([300, 50], N, Hq, D, dtype, "binary", 31)
+    q.mul_(3)
+    q[0, 0, 2] = math.nan
+    k[1, :, 1] = math.nan
+    q[1, 1, 3, 5] = math.inf                   # infinite logits of both signs
+    cache.k_pages[slot(cache, 0, 77)][:, 0] = -math.inf
+    ref = attention(q, k, v, cache, parents, cap=cap)
+    o, lse = td.tree_attention(q, k, v, cache, up, soft_cap=cap, return_lse=True)
+    bad = ref[1].isnan()
+    assert bad[0, 0, 2] and bad[1, :, 1].all() and not bad[0, 1].any()
+    assert o[bad].isnan().all() and lse[bad].isnan().all()
+    # Of the cap of 100 an fp32 tanh keeps 1e-7·100 in the logits.
+    compare(o[~bad], lse[~bad], ref[0][~bad], ref[1][~bad], ref[2][~bad])
