@@ -266,7 +266,8 @@ typedef struct bfa_rope_args {
   int64_t interleaved;      /* 0: pairs (x[i], x[i + R/2]); 1: pairs (x[2i], x[2i + 1]) */
   int64_t inverse;          /* 1: the transposed rotation (the backward) */
   bfa_tensor q, k;          /* [B, H, S, D], any strides */
-  bfa_tensor q_out, k_out;  /* written; each may be its input itself (same data and strides) */
+  bfa_tensor q_out, k_out;  /* written; each may be its input itself (same data and strides), and
+                               overlaps nothing else here */
   const float* cos;         /* [table_rows, R/2], unit inner stride, row stride table_stride */
   const float* sin;
   int64_t table_rows, table_stride;
@@ -313,7 +314,9 @@ size_t bfa_tree_workspace_bytes(const bfa_tree_args* args);
 
 /* Attention of a tree of drafted tokens over a paged cache: node n sees the
  * sequence's cached tokens, itself and the nodes above it. O and natural-log
- * LSE; rows of absent nodes get O = 0, LSE = -inf. A page number outside
+ * LSE; rows of absent nodes get O = 0, LSE = -inf. Values that are not finite
+ * reach the rows that see them and no other: a NaN or +inf logit gives NaN in
+ * the row's O and LSE, values of V their own columns. A page number outside
  * [0, num_pages) reads as zero keys and values, a length outside
  * [0, max_pages * page_size] is clamped, a parent outside its range makes the
  * node absent; each reports BFA_ERR_INDEX. */

@@ -6,8 +6,8 @@
 //
 // These calls run once or more per layer of a decoding step whose kernels take
 // a few microseconds. The same checks and argument blocks written in Python
-// take 12 to 25 us a call on the host, several times what the kernels take;
-// here they take 2 to 3.
+// made a call 16 to 33 us of host time, several times what the kernels take; from
+// here one takes 6 to 7, the attention, with four tensor maps and two launches, 12.
 //
 // A failed check raises what the attention functions raise: AssertionError for
 // shapes that do not fit together, ValueError for arguments that make no

@@ -277,8 +277,8 @@ extern "C" int bfa_tree_fwd(const bfa_tree_args* a, void* stream) {
   const int64_t rows = a->heads_q / a->heads_kv * a->nodes;
   const bool f32 = a->dtype == BFA_DTYPE_F32;
   // tcgen05 wherever TMA can read the layouts: it was the faster one at every
-  // size tried (B=16, L=8192, 8 KV heads of 128: 4 rows a KV head 91 against
-  // 125 us, 64 rows 103 against 184, 256 rows 171 against 551).
+  // size tried (B=16, L=8192, 8 KV heads of 128: 4 rows a KV head 90 against
+  // 120 us, 64 rows 103 against 175, 256 rows 173 against 551).
   const bool tc = !f32 && tcgen05_on() && tree_sm100_layout(a);
   const Plan pl = make_plan(a, f32  ? simt_tile(a)
                                : tc ? tree_sm100_tile(rows, (int)a->head_dim, a->soft_cap > 0)

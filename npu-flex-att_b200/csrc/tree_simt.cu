@@ -9,7 +9,7 @@
 //   P·V: thread = 2 or 4 columns x 4 or 8 rows, P read as vectors of 4 rows.
 // Bound: shared-memory reads and FMA issue from about 8 rows per KV head on,
 // HBM below. 13.5 TFLOP/s with 32 rows per KV head (B=4, L=4096, 4 KV heads of
-// 128: 79 us, 13% of the HBM floor; 69 us with 4 rows, whose warps are mostly
+// 128: 78 us, 13% of the HBM floor; 68 us with 4 rows, whose warps are mostly
 // idle). The next chunk's rows come by cp.async while a chunk is worked on.
 #include <cuda_runtime.h>
 

@@ -8,10 +8,10 @@
 //
 // Bound: HBM (K/V read once) up to about 256 rows per KV head, the tensor cores
 // above. Measured with its merge, bf16, 8 KV heads of 128, B=16, L=8192 (537 MB
-// of K/V): 4 to 32 rows per KV head 91 to 94 us (90 to 87% of the HBM floor),
-// 64 rows 103, 128 rows 113; 256 rows 171 us, where one tile's chain of softmax
+// of K/V): 4 to 32 rows per KV head 90 to 95 us (91 to 87% of the HBM floor),
+// 64 rows 103, 128 rows 113; 256 rows 173 us, where one tile's chain of softmax
 // and products sets the pace (2.4 us per 128 keys for 1.1 us of products). Head
-// dim 64, L=8192, 16 rows (268 MB): 61 us, the softmax's chain of latencies, 0.85
+// dim 64, L=8192, 16 rows (268 MB): 62 us, the softmax's chain of latencies, 0.85
 // us per chunk. A call that reads next to nothing takes 13 us: launch, work
 // split, page table, one chunk, merge, each waiting for the one before.
 //
@@ -44,8 +44,9 @@
 //
 // A box is gcd(page_size, chunk) tokens of one page, so any page size that is a
 // multiple of 8 works (8 rows of 128 bytes are the swizzle's atom). A lane per
-// box issues, 45 ns a box: pages of 16 tokens and more cost the same, pages of 8
-// 108 us where the others take 90 (one elected lane for all: 121). Tokens past a
+// box issues. B=16, L=8192, 4 rows per KV head: pages of 64 and more 92 us, of
+// 16 95, of 8 110 (121 with one elected lane for all boxes); head dim 64, 16
+// rows: 63, 64 and 76. Tokens past a
 // sequence's end arrive as whatever the page holds: their logits are masked,
 // P·V stops at the last 16 keys that hold one, and the softmax warps clear the
 // rest of those 16 in V before the product may read it.
